@@ -147,6 +147,135 @@ int shp_run_kernel(shp_ctx* ctx, const char* kernel, const float* in0, size_t n0
                    const float* in1, size_t n1, float* out, size_t n_out, const int32_t* push,
                    size_t n_push, uint32_t grid_hint, shp_run_info* info);
 
+/* ---- key/value cache in 8 bits ---------------------------------------------------
+ * Keys and values of n_seqs sequences, one byte an element, with an fp32 scale for each block
+ * of `block` tokens of each KV head: a code c of a block with scale s stands for the fp32 number
+ * c * s.  All arrays are the caller's, on the context's device:
+ *   k        [n_seqs][n_kv_heads][capacity][head_dim]
+ *   v        [n_seqs][n_kv_heads][capacity / 64][head_dim][64]   (64 tokens next to each other)
+ *   k_scale, v_scale  [n_seqs][n_kv_heads][capacity / block]
+ *   lengths  [n_seqs]: tokens each sequence holds, the call's own new rows included (values
+ *            outside 0 .. capacity count as the nearest of the two)
+ * Nothing needs to be cleared first: what lies behind a sequence's length is never used.
+ * head_dim 64 or 128; block 16, 32, 64 or 128; capacity a multiple of 64 and of block, up to
+ * 4,194,304; at most 65,535 heads of all sequences together; k and v 16-byte aligned; scales
+ * positive.  No counterpart in the reference, which caches
+ * nothing (run_llama_spirv.py:194-295 recomputes every position).
+ *
+ * Where a call takes n rows a sequence, counts[s] (device, may be NULL: all) says how many of
+ * them are real, and row i < counts[s] belongs to token lengths[s] - counts[s] + i.  Rows from
+ * counts[s] on are neither read nor written.  Strides are in floats, between sequences (_seq),
+ * rows (_row) and heads (_head); the head_dim floats of a row lie next to each other; rows and
+ * strides are multiples of 16 bytes.  n = 0 does nothing.
+ *
+ * All calls are asynchronous on the context stream and can be captured. */
+enum {
+    SHP_CACHE8_I8 = 0,  /* -127 .. 127 */
+    SHP_CACHE8_E4M3 = 1 /* 8-bit floats, 4 bits of exponent and 3 of mantissa, up to 448 */
+};
+typedef struct shp_cache8 {
+    void *k, *v;
+    float *k_scale, *v_scale;
+    int32_t* lengths;
+    int32_t n_seqs, n_kv_heads, head_dim, capacity, block, format;
+} shp_cache8;
+
+/* Writes new rows.  A block's scale is its largest |x| / 127 (448 for e4m3), at least 2^-60, and
+ * codes are the exact x / scale rounded to nearest, ties to even.  Rows that go behind tokens
+ * which a block already holds can only raise its scale; the codes of those tokens are then
+ * rounded again at the new one.  An infinity or a NaN makes the block's scale NaN until the
+ * block is begun again, and with it every result that uses a token of the block.  Rows of tokens
+ * before the first (lengths[s] < counts[s]) are dropped. */
+typedef struct shp_cache8_append_args {
+    const float *k, *v;
+    int64_t k_seq, k_row, k_head;
+    int64_t v_seq, v_row, v_head;
+    const int32_t* counts;
+    int32_t n;
+} shp_cache8_append_args;
+int shp_cache8_append(shp_ctx* ctx, const shp_cache8* cache, const shp_cache8_append_args* args);
+
+/* The values of the newest n tokens of every sequence, k and v [n_seqs][n_kv_heads][n][head_dim]
+ * (either may be NULL): row i is token lengths[s] - n + i, zeros where that is negative. */
+int shp_cache8_read(shp_ctx* ctx, const shp_cache8* cache, int32_t n, float* k, float* v);
+
+/* Attention: out = softmax(scale * q . K) V over the tokens up to the row's own.  n_heads query
+ * heads share the n_kv_heads KV heads in order, n_heads / n_kv_heads each.  A row that sees no
+ * token (its sequence is empty, or holds fewer tokens than rows) gets zeros.  lse (may be NULL)
+ * [n_seqs][n_heads][n]: log of the sum of exp(scale * q . k), minus infinity for such a row.
+ * Statistics and sums are fp32, and q and the weights enter the products with 22 bits.
+ * The tokens are split over workgroups whose partial results go through the context's workspace;
+ * it grows on an eager call that needs more, and a captured call that finds it too small runs
+ * without the split: run the call once before it is captured. */
+typedef struct shp_cache8_attend_args {
+    const float* q;
+    float* out;
+    int64_t q_seq, q_row, q_head;
+    int64_t o_seq, o_row, o_head;
+    const int32_t* counts;
+    float* lse;
+    int32_t n, n_heads;
+    float scale;
+} shp_cache8_attend_args;
+int shp_cache8_attend(shp_ctx* ctx, const shp_cache8* cache, const shp_cache8_attend_args* args);
+
+/* Accounts of attention weight: acc_out = acc_in + the weights exp(scale * q . k - lse) that the
+ * rows of all query heads of a KV head give a token, [n_seqs][n_kv_heads][capacity]; lse is what
+ * shp_cache8_attend wrote for the same rows.  acc_in may be acc_out, or NULL for zeros.  What
+ * lies behind a sequence's length is left as it was: clear it once before the first call, so that
+ * tokens appended later start from zero.  The order of the sums is fixed. */
+typedef struct shp_cache8_weights_args {
+    const float* q;
+    int64_t q_seq, q_row, q_head;
+    const int32_t* counts;
+    const float* lse;
+    const float* acc_in;
+    float* acc_out;
+    int32_t n, n_heads;
+    float scale;
+} shp_cache8_weights_args;
+int shp_cache8_weights(shp_ctx* ctx, const shp_cache8* cache,
+                       const shp_cache8_weights_args* args);
+
+/* Eviction: copies what is worth keeping of every sequence and KV head of src to dst.  A sequence
+ * of at most `keep` tokens keeps all.  A longer one keeps its newest `recent` and, of the others,
+ * the keep - recent with the largest weights (of equal ones the oldest; NaN is the smallest), in
+ * their old order, each KV head its own.  Blocks are made anew from the values of src.  Writes
+ * dst->lengths, kept [n_seqs][n_kv_heads][keep] (the tokens' places in src, -1 behind the last)
+ * and dst_weights [n_seqs][n_kv_heads][dst->capacity] (may be NULL: their weights, zero behind the
+ * last).  weights is [n_seqs][n_kv_heads][src->capacity].  src and dst agree in all but capacity and
+ * share no memory; 1 <= keep <= dst->capacity and 0 <= recent <= keep. */
+typedef struct shp_cache8_evict_args {
+    const float* weights;
+    int32_t* kept;
+    float* dst_weights;
+    int32_t keep, recent;
+} shp_cache8_evict_args;
+int shp_cache8_evict(shp_ctx* ctx, const shp_cache8* src, const shp_cache8* dst,
+                     const shp_cache8_evict_args* args);
+
+/* ---- how likely a token is -----------------------------------------------------------
+ * For each of `rows` rows of vocab logits (row_stride floats apart): logprob = log softmax at
+ * targets[r] (minus infinity for an id outside the vocabulary), entropy = -sum p log p, both in
+ * natural logarithms, and the n_top likeliest ids with their log probabilities, [rows][n_top], the
+ * likeliest first and of equal ones the lowest id first.  targets with logprob, entropy, and
+ * top_ids with top_logprobs may be NULL.  0 <= n_top <= 64 and at most vocab.  A logit of minus
+ * infinity is a token that cannot be; a row that holds a NaN or plus infinity, or nothing but minus
+ * infinity, has NaN in place of logarithms, and its ids go by the logits with NaN last.  Rows of
+ * more than 32,768 logits use the context's workspace, as shp_cache8_attend does, and are refused
+ * in a capture that finds it too small. */
+typedef struct shp_logprobs_args {
+    const float* logits;
+    int64_t row_stride;
+    const int32_t* targets;
+    float* logprob;
+    float* entropy;
+    int32_t* top_ids;
+    float* top_logprobs;
+    int32_t rows, vocab, n_top;
+} shp_logprobs_args;
+int shp_token_logprobs(shp_ctx* ctx, const shp_logprobs_args* args);
+
 /* ---- captured launch sequences (hipGraph) ------------------------------------
  * The reference records and submits a command buffer per dispatch
  * (source/tflite_loader/src/vulkan.rs:132-171).  A caller that repeats one sequence of

@@ -60,6 +60,46 @@ class LlamaConfig(C.Structure):
                 ("rope_theta", C.c_float)]
 
 
+class Cache8Struct(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p),
+                ("v_scale", C.c_void_p), ("lengths", C.c_void_p), ("n_seqs", C.c_int32),
+                ("n_kv_heads", C.c_int32), ("head_dim", C.c_int32), ("capacity", C.c_int32),
+                ("block", C.c_int32), ("format", C.c_int32)]
+
+
+class Cache8AppendArgs(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_seq", C.c_int64), ("k_row", C.c_int64),
+                ("k_head", C.c_int64), ("v_seq", C.c_int64), ("v_row", C.c_int64),
+                ("v_head", C.c_int64), ("counts", C.c_void_p), ("n", C.c_int32)]
+
+
+class Cache8AttendArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_seq", C.c_int64),
+                ("q_row", C.c_int64), ("q_head", C.c_int64), ("o_seq", C.c_int64),
+                ("o_row", C.c_int64), ("o_head", C.c_int64), ("counts", C.c_void_p),
+                ("lse", C.c_void_p), ("n", C.c_int32), ("n_heads", C.c_int32),
+                ("scale", C.c_float)]
+
+
+class Cache8WeightsArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("q_seq", C.c_int64), ("q_row", C.c_int64),
+                ("q_head", C.c_int64), ("counts", C.c_void_p), ("lse", C.c_void_p),
+                ("acc_in", C.c_void_p), ("acc_out", C.c_void_p), ("n", C.c_int32),
+                ("n_heads", C.c_int32), ("scale", C.c_float)]
+
+
+class Cache8EvictArgs(C.Structure):
+    _fields_ = [("weights", C.c_void_p), ("kept", C.c_void_p), ("dst_weights", C.c_void_p),
+                ("keep", C.c_int32), ("recent", C.c_int32)]
+
+
+class LogprobsArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_int64), ("targets", C.c_void_p),
+                ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("top_ids", C.c_void_p),
+                ("top_logprobs", C.c_void_p), ("rows", C.c_int32), ("vocab", C.c_int32),
+                ("n_top", C.c_int32)]
+
+
 # (name, restype, argtypes) of every exported entry point, in header order.
 SIGNATURES = [
     ("shp_create", C.c_int, [C.c_char_p, C.POINTER(C.c_void_p)]),
@@ -90,6 +130,17 @@ SIGNATURES = [
     ("shp_run_kernel", C.c_int, [C.c_void_p, C.c_char_p, C.c_void_p, C.c_size_t, C.c_void_p,
                                  C.c_size_t, C.c_void_p, C.c_size_t, C.POINTER(C.c_int32),
                                  C.c_size_t, C.c_uint32, C.POINTER(RunInfo)]),
+    ("shp_cache8_append", C.c_int, [C.c_void_p, C.POINTER(Cache8Struct),
+                                    C.POINTER(Cache8AppendArgs)]),
+    ("shp_cache8_read", C.c_int, [C.c_void_p, C.POINTER(Cache8Struct), C.c_int32, C.c_void_p,
+                                  C.c_void_p]),
+    ("shp_cache8_attend", C.c_int, [C.c_void_p, C.POINTER(Cache8Struct),
+                                    C.POINTER(Cache8AttendArgs)]),
+    ("shp_cache8_weights", C.c_int, [C.c_void_p, C.POINTER(Cache8Struct),
+                                     C.POINTER(Cache8WeightsArgs)]),
+    ("shp_cache8_evict", C.c_int, [C.c_void_p, C.POINTER(Cache8Struct), C.POINTER(Cache8Struct),
+                                   C.POINTER(Cache8EvictArgs)]),
+    ("shp_token_logprobs", C.c_int, [C.c_void_p, C.POINTER(LogprobsArgs)]),
     ("shp_capture_begin", C.c_int, [C.c_void_p]),
     ("shp_capture_end", C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     ("shp_graph_launch", C.c_int, [C.c_void_p]),

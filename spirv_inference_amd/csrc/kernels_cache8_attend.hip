@@ -1,0 +1,519 @@
+// Attention over the 8-bit cache, and the accounts of the weight each cached token gets.
+//
+// A wavefront owns 16 * MT query rows (the rows of all query heads of a KV head, row r = new token
+// r / group, head r % group) and walks the sequence's tokens 64 at a time, with the running maximum
+// and sum of a softmax.  Codes are exact as fp16, q and the weights are cut into two fp16 pieces of
+// 11 bits, so the products run on v_mfma_f32_16x16x32_f16 and keep fp32's accuracy.
+//
+// Scores are computed transposed, S^T = K Q^T.  Row m of token tile j is given to token
+// (m / 4) * 16 + 4 j + m % 4 of the 64: the lane (query l % 16, group g = l / 16) then holds the
+// scores of tokens 16 g .. 16 g + 15, all of one block (one scale), and these are the k slots that
+// the lane's 16 bytes of a dimension of V stand for in O^T = V^T P^T.  So K and V go from memory to
+// the matrix cores without LDS, in 16-byte loads, and P never leaves its registers.
+//
+// With u_t = log2 of (weight * scale of V), the running maximum m is taken over u, and
+// w_t = 2^(u_t - m + 12) is what multiplies V's codes: it spans fp16's range whatever the scales
+// are, and the row's sum is that of w_t / scale.
+#include "cache8.h"
+
+namespace {
+
+using namespace shpd;
+using shp::Cache8;
+using shp::Cache8Query;
+using shp::kCacheTile;
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef float f2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kLift = 12.0f;  // weights reach 2^12: the low piece stays a normal fp16 number longer
+constexpr float kLargeScore = 262144.0f;
+constexpr int kQBits = 14;      // a row of q is scaled to reach 2^13 .. 2^14
+
+// Four codes as fp16 numbers.
+template <int FMT>
+__device__ __forceinline__ void codes4(unsigned w, h2& a, h2& b) {
+    if constexpr (FMT == kI8) {
+        // the bytes of c + 128 under an exponent of 1024, less 1152
+        const unsigned u = w ^ 0x80808080u;
+        const h2 off = {(_Float16)-1152.0f, (_Float16)-1152.0f};
+        a = __builtin_bit_cast(h2, __builtin_amdgcn_perm(u, 0x64646464u, 0x01050104u)) + off;
+        b = __builtin_bit_cast(h2, __builtin_amdgcn_perm(u, 0x64646464u, 0x01070106u)) + off;
+    } else {
+        a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false);
+        b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true);
+    }
+}
+template <int FMT>
+__device__ __forceinline__ h8 codes8(unsigned lo, unsigned hi) {
+    h2 a, b, c, d;
+    codes4<FMT>(lo, a, b);
+    codes4<FMT>(hi, c, d);
+    return h8{a.x, a.y, b.x, b.y, c.x, c.y, d.x, d.y};
+}
+
+// Two numbers as the sum of two fp16 each.
+__device__ __forceinline__ void pieces(float x, float y, h2& hi, h2& lo) {
+    hi = __builtin_convertvector(f2{x, y}, h2);
+    lo = __builtin_convertvector(f2{x - (float)hi.x, y - (float)hi.y}, h2);
+}
+
+__device__ __forceinline__ float max_over_groups(float x) {
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+
+// A KV head of a sequence and its query rows.
+struct RowSpan {
+    int s, h, len, count, rows;
+};
+
+// Row r (another one for each l % 16): the pieces of q * scale * log2 e in the B layout, scaled by a
+// power of two, in `back` the inverse of that power, and in `limit` how many tokens the row sees.
+// Rows behind the last repeat it.
+template <int D>
+__device__ __forceinline__ void load_q(const Cache8Query& q, const RowSpan& p, int r, h8* hi, h8* lo,
+                                       float& back, int& limit) {
+    const int g = (threadIdx.x & 63) >> 4;
+    const bool real = r < p.rows;
+    const int rr = real ? r : p.rows - 1, i = rr / q.group, head = p.h * q.group + rr - i * q.group;
+    limit = max(p.len - p.count + i + 1, 0);
+    const float* x = q.q + p.s * q.q_seq + i * q.q_row + head * q.q_head + 16 * g;
+    f4 v[D / 16];
+    float top = 0.0f;
+#pragma unroll
+    for (int a = 0; a < D / 64; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) v[4 * a + b] = *reinterpret_cast<const f4*>(x + 64 * a + 4 * b);
+#pragma unroll
+    for (int a = 0; a < D / 16; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            v[a][b] *= q.scale * kLog2e;
+            top = fmaxf(top, fabsf(v[a][b]));
+        }
+    top = max_over_groups(top);
+    const int e = kQBits - __builtin_amdgcn_frexp_expf(top);
+    back = __builtin_amdgcn_ldexpf(1.0f, -e);
+#pragma unroll
+    for (int a = 0; a < D / 32; ++a)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const f4 t = v[2 * a + b / 2];
+            h2 ph, pl;
+            pieces(__builtin_amdgcn_ldexpf(t[2 * (b & 1)], e),
+                   __builtin_amdgcn_ldexpf(t[2 * (b & 1) + 1], e), ph, pl);
+            hi[a][2 * b] = ph.x;
+            hi[a][2 * b + 1] = ph.y;
+            lo[a][2 * b] = pl.x;
+            lo[a][2 * b + 1] = pl.y;
+        }
+}
+
+// K of a 64-token tile: raw[j][a] = 16 dimensions (64 a + 16 g) of token (m / 4) * 16 + 4 j + m % 4.
+template <int D>
+__device__ __forceinline__ void load_k(const uint8_t* tile, u4 raw[4][D / 64]) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+    const uint8_t* p = tile + ((m >> 2) * 16 + (m & 3)) * D + 16 * g;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int a = 0; a < D / 64; ++a)
+            raw[j][a] = *reinterpret_cast<const u4*>(p + 4 * j * D + 64 * a);
+}
+// V of a 64-token tile: raw[d] = tokens 16 g .. 16 g + 15 of dimension 16 d + m.
+template <int D>
+__device__ __forceinline__ void load_v(const uint8_t* tile, u4 raw[D / 16]) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+    const uint8_t* p = tile + m * kCacheTile + 16 * g;
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d)
+        raw[d] = *reinterpret_cast<const u4*>(p + d * 16 * kCacheTile);
+}
+
+template <int D, int FMT, int MT>
+__global__ __launch_bounds__(256) void cache8_attend_kernel(Cache8 c, Cache8Query q, int row_waves,
+                                                            int splits, float* part) {
+    constexpr int NO = D / 16;  // accumulators of 16 rows
+    __shared__ __attribute__((aligned(16))) float ex[2][MT * (NO * 4 + 2) * 64];
+    const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int sh = blockIdx.x, tok_waves = 4 / row_waves;
+    const int wr = wave % row_waves, wt = wave / row_waves;
+    RowSpan p;
+    p.s = sh / c.kv;
+    p.h = sh - p.s * c.kv;
+    p.len = seq_length(c, p.s);
+    p.count = seq_count(q.counts, q.n, p.s);
+    p.rows = p.count * q.group;
+    const int wg_rows = 16 * MT * row_waves, base = (int)blockIdx.y * wg_rows;
+    if (base >= p.rows) return;
+    const int r0 = base + wr * 16 * MT;
+
+    // tokens the workgroup's last row sees, and its share of their tiles
+    const int last = min(p.rows, base + wg_rows) - 1;
+    const int sees = max(p.len - p.count + last / q.group + 1, 0);
+    const int tiles = (sees + kCacheTile - 1) / kCacheTile;
+    const int share = (tiles + splits - 1) / splits;
+    const int tile0 = (int)blockIdx.z * share, tile1 = min(tiles, tile0 + share);
+
+    float m[MT], l[MT], back[MT];
+    int limit[MT];
+    f4 o[MT][NO];
+    h8 qh[MT][D / 32], ql[MT][D / 32];
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        load_q<D>(q, p, r0 + 16 * t + li, qh[t], ql[t], back[t], limit[t]);
+        m[t] = -__builtin_inff();
+        l[t] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < NO; ++d) o[t][d] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    // tokens that every row of this wavefront sees
+    const int open = max(p.len - p.count + min(r0, p.rows - 1) / q.group + 1, 0);
+
+    const uint8_t* kp = c.k + (int64_t)sh * c.cap * D;
+    const uint8_t* vp = c.v + (int64_t)sh * c.cap * D;
+    const int64_t sbase = (int64_t)sh * (c.cap >> c.block_log2);
+    const int last_block = max(p.len - 1, 0) >> c.block_log2;
+
+    for (int tile = tile0 + wt; tile < tile1; tile += tok_waves) {
+        const int t0 = tile * kCacheTile;
+        u4 kr[4][D / 64], vr[NO];
+        load_k<D>(kp + (int64_t)t0 * D, kr);
+        load_v<D>(vp + (int64_t)t0 * D, vr);
+        const int64_t b = sbase + min((t0 + 16 * g) >> c.block_log2, last_block);
+        const float ks = c.k_scale[b];
+        float vs = c.v_scale[b];
+        vs = vs < kScaleFloor ? kScaleFloor : vs;
+        const bool edge = t0 + kCacheTile > open;
+        if (FMT == kE4M3 && t0 + kCacheTile > p.len) {
+            // bytes behind the last token may be NaN codes, which a weight of zero does not cancel
+#pragma unroll
+            for (int d = 0; d < NO; ++d)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const int left = p.len - t0 - 16 * g - 4 * w;
+                    vr[d][w] &= left >= 4 ? ~0u : left <= 0 ? 0u : (1u << 8 * left) - 1;
+                }
+        }
+
+        f4 sc[MT][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t) sc[t][j] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int a = 0; a < D / 32; ++a) {
+                const u4 w = kr[j][a >> 1];
+                const h8 kf = a & 1 ? codes8<FMT>(w.z, w.w) : codes8<FMT>(w.x, w.y);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    sc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[t][a], sc[t][j], 0, 0, 0);
+                    sc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[t][a], sc[t][j], 0, 0, 0);
+                }
+            }
+        }
+        // sc[t][j][i]: token t0 + 16 g + 4 j + i, row r0 + 16 t + li
+        const float lv = __builtin_amdgcn_logf(vs);
+        h8 wh[MT][2], wl[MT][2];
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const float f = ks * back[t];
+            float mx = -__builtin_inff();
+            if (edge) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (t0 + 16 * g + 4 * j + i >= limit[t]) sc[t][j][i] = -__builtin_inff();
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[t][j][i]);
+            const float top = fmaxf(m[t], max_over_groups(__builtin_fmaf(mx, f, lv)));
+            if (__any(top > m[t])) {
+                const float down = m[t] == top ? 1.0f : __builtin_amdgcn_exp2f(m[t] - top);
+                l[t] *= down;
+#pragma unroll
+                for (int d = 0; d < NO; ++d) o[t][d] *= down;
+                m[t] = top;
+            }
+            // u - m as one fused step; where u is so large that the rounding of m would show (a
+            // weight of more than 2^12, or none), u is rounded as m was
+            const float at = lv + kLift - m[t];
+            const bool large = fabsf(m[t]) > kLargeScore;
+            float sum = 0.0f;
+            if (edge || __any(large)) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float x = sc[t][j][i];
+                        const float u = large ? __builtin_fmaf(x, f, lv) - m[t] + kLift
+                                              : __builtin_fmaf(x, f, at);
+                        sc[t][j][i] = t0 + 16 * g + 4 * j + i < limit[t]
+                                          ? __builtin_amdgcn_exp2f(u) : 0.0f;
+                    }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        sc[t][j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j][i], f, at));
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum += sc[t][j][i];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    h2 ph, pl;
+                    pieces(sc[t][j][2 * i], sc[t][j][2 * i + 1], ph, pl);
+                    const int e = 4 * (j & 1) + 2 * i;
+                    wh[t][j >> 1][e] = ph.x;
+                    wh[t][j >> 1][e + 1] = ph.y;
+                    wl[t][j >> 1][e] = pl.x;
+                    wl[t][j >> 1][e + 1] = pl.y;
+                }
+            }
+            if (sum != 0.0f) l[t] += sum / vs;  // of a block nobody sees, the scale may be NaN
+        }
+#pragma unroll
+        for (int d = 0; d < NO; ++d) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const h8 vf = e ? codes8<FMT>(vr[d].z, vr[d].w) : codes8<FMT>(vr[d].x, vr[d].y);
+#pragma unroll
+                for (int t = 0; t < MT; ++t) {
+                    o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wl[t][e], o[t][d], 0, 0, 0);
+                    o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wh[t][e], o[t][d], 0, 0, 0);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        l[t] += __shfl_xor(l[t], 16);
+        l[t] += __shfl_xor(l[t], 32);
+    }
+
+    // wavefronts of the same rows, in pairs: the upper one's part goes through LDS
+    for (int step = tok_waves >> 1; step > 0; step >>= 1) {
+        const int slot = (wt & (step - 1)) * row_waves + wr;
+        float* x = ex[slot];
+        if (wt >= step && wt < 2 * step)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+#pragma unroll
+                for (int d = 0; d < NO; ++d)
+                    *reinterpret_cast<f4*>(&x[((t * NO + d) * 64 + lane) * 4]) = o[t][d];
+                x[(MT * NO * 4 + 2 * t) * 64 + lane] = m[t];
+                x[(MT * NO * 4 + 2 * t + 1) * 64 + lane] = l[t];
+            }
+        __syncthreads();
+        if (wt < step)
+#pragma unroll
+            for (int t = 0; t < MT; ++t) {
+                const float m1 = x[(MT * NO * 4 + 2 * t) * 64 + lane];
+                const float l1 = x[(MT * NO * 4 + 2 * t + 1) * 64 + lane];
+                const float top = fmaxf(m[t], m1);
+                const float f0 = m[t] == top ? 1.0f : __builtin_amdgcn_exp2f(m[t] - top);
+                const float f1 = m1 == top ? 1.0f : __builtin_amdgcn_exp2f(m1 - top);
+                l[t] = l[t] * f0 + l1 * f1;
+                m[t] = top;
+#pragma unroll
+                for (int d = 0; d < NO; ++d)
+                    o[t][d] = o[t][d] * f0 +
+                              *reinterpret_cast<const f4*>(&x[((t * NO + d) * 64 + lane) * 4]) * f1;
+            }
+        __syncthreads();
+    }
+    if (wt) return;
+
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int r = r0 + 16 * t + li;
+        if (r >= p.rows) continue;
+        if (splits > 1) {
+            // part: [sh][split][row][D + 2], rows of the launch's row blocks
+            const int64_t at = ((int64_t)sh * splits + blockIdx.z) * gridDim.y * wg_rows + r;
+            float* x = part + at * (D + 4);
+#pragma unroll
+            for (int d = 0; d < NO; ++d) *reinterpret_cast<f4*>(x + 16 * d + 4 * g) = o[t][d];
+            if (g == 0) *reinterpret_cast<f4*>(x + D) = f4{m[t], l[t], 0.f, 0.f};
+            continue;
+        }
+        const int i = r / q.group, head = p.h * q.group + r - i * q.group;
+        const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+        float* x = q.out + p.s * q.o_seq + i * q.o_row + head * q.o_head + 4 * g;
+#pragma unroll
+        for (int d = 0; d < NO; ++d) *reinterpret_cast<f4*>(x + 16 * d) = o[t][d] * inv;
+        if (q.lse && g == 0)
+            q.lse[((int64_t)p.s * q.heads + head) * q.n + i] =
+                l[t] == 0.0f ? -__builtin_inff()
+                             : (m[t] - kLift + __builtin_amdgcn_logf(l[t])) * kLn2;
+    }
+}
+
+// Joins the parts of a row: thread = 4 dimensions.
+template <int D>
+__global__ __launch_bounds__(256) void cache8_join_kernel(Cache8 c, Cache8Query q, int splits,
+                                                          int row_slots, const float* part) {
+    constexpr int T = D / 4;
+    const int sh = blockIdx.x, s = sh / c.kv, h = sh - s * c.kv;
+    const int r = (int)blockIdx.y * (256 / T) + threadIdx.x / T, d = threadIdx.x % T * 4;
+    if (r >= seq_count(q.counts, q.n, s) * q.group) return;
+    const int64_t stride = (int64_t)row_slots * (D + 4);
+    const float* x = part + ((int64_t)sh * splits * row_slots + r) * (D + 4);
+    float m = -__builtin_inff();
+    for (int i = 0; i < splits; ++i) m = fmaxf(m, x[i * stride + D]);
+    float l = 0.0f;
+    f4 o = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < splits; ++i) {
+        const float mi = x[i * stride + D];
+        const float f = mi == m ? 1.0f : __builtin_amdgcn_exp2f(mi - m);
+        l += x[i * stride + D + 1] * f;
+        o += *reinterpret_cast<const f4*>(x + i * stride + d) * f;
+    }
+    const int i = r / q.group, head = h * q.group + r - i * q.group;
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    *reinterpret_cast<f4*>(q.out + s * q.o_seq + i * q.o_row + head * q.o_head + d) = o * inv;
+    if (q.lse && d == 0)
+        q.lse[((int64_t)s * q.heads + head) * q.n + i] =
+            l == 0.0f ? -__builtin_inff() : (m - kLift + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
+// Accounts: a wavefront owns 64 tokens of a head and walks the rows, 16 at a time.
+template <int D, int FMT>
+__global__ __launch_bounds__(256) void cache8_weights_kernel(Cache8 c, Cache8Query q) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int sh = blockIdx.y;
+    RowSpan p;
+    p.s = sh / c.kv;
+    p.h = sh - p.s * c.kv;
+    p.len = seq_length(c, p.s);
+    p.count = seq_count(q.counts, q.n, p.s);
+    p.rows = p.count * q.group;
+    const int t0 = ((int)blockIdx.x * 4 + wave) * kCacheTile;
+    if (t0 >= p.len) return;
+    u4 kr[4][D / 64];
+    load_k<D>(c.k + ((int64_t)sh * c.cap + t0) * D, kr);
+    const float ks = c.k_scale[(int64_t)sh * (c.cap >> c.block_log2) +
+                               (min(t0 + 16 * g, p.len - 1) >> c.block_log2)];
+    float acc[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
+    // the first row that sees a token of the tile
+    const int first = max(t0 - (p.len - p.count), 0) * q.group;
+    for (int r0 = first & ~15; r0 < p.rows; r0 += 16) {
+        h8 qh[D / 32], ql[D / 32];
+        float back;
+        int limit;
+        load_q<D>(q, p, r0 + li, qh, ql, back, limit);
+        const int r = r0 + li, i = r / q.group;
+        const float lse = r < p.rows
+            ? q.lse[((int64_t)p.s * q.heads + p.h * q.group + r - i * q.group) * q.n + i]
+            : -__builtin_inff();
+        if (!(lse > -__builtin_inff()) && lse == lse) limit = 0;  // no such row, or an empty one
+        const float f = ks * back, at = -lse * kLog2e;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            f4 sc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int a = 0; a < D / 32; ++a) {
+                const u4 w = kr[j][a >> 1];
+                const h8 kf = a & 1 ? codes8<FMT>(w.z, w.w) : codes8<FMT>(w.x, w.y);
+                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[a], sc, 0, 0, 0);
+                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[a], sc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], f, at));
+                acc[4 * j + e] += t0 + 16 * g + 4 * j + e < limit ? w : 0.0f;
+            }
+        }
+    }
+    // over the 16 rows of a lane group: each step halves the tokens a lane answers for
+    float v[16];
+#pragma unroll
+    for (int e = 0; e < 16; ++e) v[e] = acc[e];
+#pragma unroll
+    for (int step = 8; step > 0; step >>= 1) {
+        const bool up = li & step;
+#pragma unroll
+        for (int e = 0; e < step; ++e) {
+            const float mine = up ? v[e + step] : v[e], other = up ? v[e] : v[e + step];
+            v[e] = mine + __shfl_xor(other, step);
+        }
+    }
+    const int t = t0 + lane;
+    if (t >= p.len) return;
+    const int64_t at = (int64_t)sh * c.cap + t;
+    q.acc_out[at] = (q.acc_in ? q.acc_in[at] : 0.0f) + v[0];
+}
+
+}  // namespace
+
+namespace shp {
+
+Cache8Plan cache8_attend_plan(const Cache8& c, int head_dim, int64_t rows, int cu_count,
+                              bool may_split) {
+    Cache8Plan p;
+    const int widest = head_dim == 64 ? 4 : 2;
+    p.row_tiles = rows <= 16 ? 1 : rows <= 32 || widest == 2 ? 2 : 4;
+    const int64_t tiles16 = (rows + 15) / 16;
+    p.row_waves = tiles16 > 2 * p.row_tiles ? 4 : tiles16 > p.row_tiles ? 2 : 1;
+    const int64_t per = 16 * p.row_tiles * p.row_waves;
+    p.row_blocks = (int)std::min<int64_t>((rows + per - 1) / per, 1 << 30);
+    // enough workgroups for four on every CU, none with fewer tokens than a tile a wavefront
+    const int64_t units = (int64_t)c.n_seqs * c.kv * p.row_blocks;
+    const int64_t want = (4ll * std::max(cu_count, 1) + units - 1) / units;
+    const int64_t most = std::max<int64_t>(c.cap / (kCacheTile * (4 / p.row_waves)), 1);
+    p.splits = may_split ? (int)std::min<int64_t>(std::min(want, most), 1024) : 1;
+    p.scratch = p.splits > 1 ? (size_t)units * per * p.splits * (head_dim + 4) : 0;
+    return p;
+}
+
+#define SHP_CACHE8_KERNEL(KERN, head_dim, format)                                   \
+    ((head_dim) == 64 ? ((format) == SHP_CACHE8_I8 ? KERN<64, shpd::kI8> : KERN<64, shpd::kE4M3>) \
+                      : ((format) == SHP_CACHE8_I8 ? KERN<128, shpd::kI8> : KERN<128, shpd::kE4M3>))
+
+int cache8_attend_launch(hipStream_t s, const Cache8& c, int head_dim, int format,
+                         const Cache8Query& q, const Cache8Plan& p, float* scratch) {
+    const bool i8 = format == SHP_CACHE8_I8;
+    auto kern = head_dim == 64
+        ? (p.row_tiles == 1   ? (i8 ? cache8_attend_kernel<64, kI8, 1> : cache8_attend_kernel<64, kE4M3, 1>)
+           : p.row_tiles == 2 ? (i8 ? cache8_attend_kernel<64, kI8, 2> : cache8_attend_kernel<64, kE4M3, 2>)
+                              : (i8 ? cache8_attend_kernel<64, kI8, 4> : cache8_attend_kernel<64, kE4M3, 4>))
+        : (p.row_tiles == 1   ? (i8 ? cache8_attend_kernel<128, kI8, 1> : cache8_attend_kernel<128, kE4M3, 1>)
+                              : (i8 ? cache8_attend_kernel<128, kI8, 2> : cache8_attend_kernel<128, kE4M3, 2>));
+    hipLaunchKernelGGL(kern, dim3(c.n_seqs * c.kv, p.row_blocks, p.splits), dim3(256), 0, s, c, q,
+                       p.row_waves, p.splits, scratch);
+    SHP_HIP_CHECK(hipGetLastError());
+    if (p.splits > 1) {
+        const int slots = p.row_blocks * 16 * p.row_tiles * p.row_waves, per = 1024 / head_dim;
+        const int64_t rows = (int64_t)q.n * q.group;
+        hipLaunchKernelGGL(head_dim == 64 ? cache8_join_kernel<64> : cache8_join_kernel<128>,
+                           dim3(c.n_seqs * c.kv, (unsigned)((rows + per - 1) / per)), dim3(256), 0, s,
+                           c, q, p.splits, slots, scratch);
+        SHP_HIP_CHECK(hipGetLastError());
+    }
+    return SHP_OK;
+}
+
+int cache8_weights_launch(hipStream_t s, const Cache8& c, int head_dim, int format,
+                          const Cache8Query& q) {
+    const int per = 4 * kCacheTile;
+    hipLaunchKernelGGL(SHP_CACHE8_KERNEL(cache8_weights_kernel, head_dim, format),
+                       dim3((c.cap + per - 1) / per, c.n_seqs * c.kv), dim3(256), 0, s, c, q);
+    SHP_HIP_CHECK(hipGetLastError());
+    return SHP_OK;
+}
+
+}  // namespace shp

@@ -172,28 +172,48 @@ int Ctx::launch(const char* name, const void* in0, const void* in1, void* out,
             if (rc) return rc;
         }
     }
-    Timer* t = nullptr;
-    if (timing) {
-        if (timer_used == timers.size()) {
-            Timer nt;
-            SHP_HIP_CHECK(hipEventCreate(&nt.a));
-            SHP_HIP_CHECK(hipEventCreate(&nt.b));
-            timers.push_back(nt);
-        }
-        t = &timers[timer_used++];
-        t->name = name;
-        SHP_HIP_CHECK(hipEventRecord(t->a, stream));
+    return timed(name, [&] {
+        return launch_kernel(stream, name, in0, in1, out, push, n_push, out_elems, epi, workspace,
+                             workspace_bytes, &tune);
+    });
+}
+
+int Ctx::timer_start(const char* name) {
+    if (!timing) return SHP_OK;
+    if (timer_used == timers.size()) {
+        Timer nt;
+        SHP_HIP_CHECK(hipEventCreate(&nt.a));
+        SHP_HIP_CHECK(hipEventCreate(&nt.b));
+        timers.push_back(nt);
     }
-    int rc = launch_kernel(stream, name, in0, in1, out, push, n_push, out_elems, epi, workspace,
-                           workspace_bytes, &tune);
-    if (t) {
-        if (rc) {
-            --timer_used;
-        } else {
-            SHP_HIP_CHECK(hipEventRecord(t->b, stream));
-        }
+    Timer* t = &timers[timer_used++];
+    t->name = name ? name : "";
+    SHP_HIP_CHECK(hipEventRecord(t->a, stream));
+    return SHP_OK;
+}
+
+int Ctx::timer_stop(int rc) {
+    if (!timing) return rc;
+    if (rc) {
+        --timer_used;
+    } else {
+        SHP_HIP_CHECK(hipEventRecord(timers[timer_used - 1].b, stream));
     }
     return rc;
+}
+
+int Ctx::scratch(size_t floats, float** p) {
+    *p = nullptr;
+    const size_t need = kSplitCounterBytes + floats * sizeof(float);
+    if (need > workspace_bytes) {
+        hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+        SHP_HIP_CHECK(hipStreamIsCapturing(stream, &cs));
+        if (cs != hipStreamCaptureStatusNone) return SHP_OK;
+        int rc = ensure_workspace(need);
+        if (rc) return rc;
+    }
+    *p = workspace + kSplitCounterBytes / sizeof(float);
+    return SHP_OK;
 }
 
 int Ctx::collect_timing() {

@@ -54,6 +54,19 @@ struct Ctx {
     int launch(const char* name, const void* in0, const void* in1, void* out,
                const int32_t* push, size_t n_push, uint64_t out_elems, const shp_epilogue* epi);
     int collect_timing();
+    // Runs `enqueue` (which returns a status) between the events of a timed launch of this name.
+    template <class F>
+    int timed(const char* name, F enqueue) {
+        int rc = timer_start(name);
+        if (rc) return rc;
+        rc = enqueue();
+        return timer_stop(rc);
+    }
+    int timer_start(const char* name);
+    int timer_stop(int rc);
+    // Scratch of at least `floats` for the kernels of one call, behind the workspace's split-K
+    // counters; *p is null where the stream is being captured and the workspace is too small.
+    int scratch(size_t floats, float** p);
 };
 
 // SHP_OK unless `stream` is being captured into a graph; then SHP_ERR_INVALID naming `what`.

@@ -14,7 +14,7 @@ from typing import Optional, Sequence
 
 import numpy as np
 
-from ._lib import ACT, Epilogue, RunInfo, check, lib
+from ._lib import ACT, Epilogue, LogprobsArgs, RunInfo, check, lib
 
 
 @dataclasses.dataclass
@@ -149,6 +149,20 @@ class Context:
             rc = lib().shp_launch_ex(self.handle, kernel.encode(), p0, p1, out.ptr, arr, n, oe,
                                      C.byref(epi))
         check(rc, f"launch {kernel}")
+
+    def token_logprobs(self, logits, targets, logprob, entropy, top_ids, top_logprobs, rows: int,
+                       vocab: int, n_top: int = 0, row_stride: Optional[int] = None) -> None:
+        """Log probabilities of given tokens, entropies and the n_top likeliest ids of each row of
+        logits (shp_token_logprobs); targets with logprob, entropy, and top_ids with top_logprobs
+        may be None.  Asynchronous."""
+        args = LogprobsArgs(logits.ptr, vocab if row_stride is None else row_stride,
+                            targets.ptr if targets is not None else None,
+                            logprob.ptr if logprob is not None else None,
+                            entropy.ptr if entropy is not None else None,
+                            top_ids.ptr if top_ids is not None else None,
+                            top_logprobs.ptr if top_logprobs is not None else None,
+                            rows, vocab, n_top)
+        check(lib().shp_token_logprobs(self.handle, C.byref(args)), "shp_token_logprobs")
 
     # -- captured launch sequences
     def capture_begin(self) -> None:
