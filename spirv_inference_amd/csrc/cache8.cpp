@@ -158,8 +158,17 @@ int shp_cache8_weights(shp_ctx* ctx, const shp_cache8* cache, const shp_cache8_w
     q.lse = const_cast<float*>(a->lse); q.counts = a->counts;
     q.n = a->n; q.heads = a->n_heads; q.group = a->n_heads / c.kv; q.scale = a->scale;
     q.acc_in = a->acc_in; q.acc_out = a->acc_out;
+    const int64_t rows = (int64_t)q.n * q.group;
+    shp::Cache8WeightsPlan plan = shp::cache8_weights_plan(c, cache->head_dim, rows, true);
+    float* scratch = nullptr;
+    if (plan.scratch) {
+        rc = x->scratch(plan.scratch, &scratch);
+        if (rc) return rc;
+        if (!scratch) plan = shp::cache8_weights_plan(c, cache->head_dim, rows, false);
+    }
     return x->timed("cache8_weights", [&] {
-        return shp::cache8_weights_launch(x->stream, c, cache->head_dim, cache->format, q);
+        return shp::cache8_weights_launch(x->stream, c, cache->head_dim, cache->format, q, plan,
+                                          scratch);
     });
 }
 

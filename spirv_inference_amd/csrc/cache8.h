@@ -56,8 +56,18 @@ Cache8Plan cache8_attend_plan(const Cache8& c, int head_dim, int64_t rows, int c
                               bool may_split);
 int cache8_attend_launch(hipStream_t s, const Cache8& c, int head_dim, int format,
                          const Cache8Query& q, const Cache8Plan& p, float* scratch);
+// How the accounts' rows and tokens are shared out, and the floats of scratch that takes (0: none).
+struct Cache8WeightsPlan {
+    int row_tiles;  // 16-row tiles a wavefront holds
+    int groups;     // row groups of a KV head, each of `chunks` times that many rows
+    int chunks;
+    int row_waves;  // wavefronts of a workgroup side by side over groups; the rest share its tokens
+    int workers;    // workgroups over the tokens
+    size_t scratch;
+};
+Cache8WeightsPlan cache8_weights_plan(const Cache8& c, int head_dim, int64_t rows, bool may_group);
 int cache8_weights_launch(hipStream_t s, const Cache8& c, int head_dim, int format,
-                          const Cache8Query& q);
+                          const Cache8Query& q, const Cache8WeightsPlan& p, float* scratch);
 int cache8_evict_launch(hipStream_t s, const Cache8& src, const Cache8& dst, int head_dim,
                         int format, const float* weights, int keep, int recent, int32_t* kept,
                         float* dst_weights);
@@ -110,17 +120,40 @@ __device__ __forceinline__ float quotient_odd(float x, float s) {
     return __int_as_float(b);
 }
 
-// The code (one byte) of x at scale s; of a block without a scale (NaN), 0.
+// The codes (one word) of four numbers at scale s, inv = 1 / s rounded; of a block without a scale
+// (NaN), 0.  x * inv is within 2^-23 of the quotient, which settles the code unless it lies next
+// to the middle of two codes (about one number in 16,000): only then the quotient itself is formed
+// (a division and its remainder, five times the work).
 template <int FMT>
-__device__ __forceinline__ unsigned encode(float x, float s) {
+__device__ __forceinline__ unsigned encode4(const float* x, float s, float inv) {
     if (!(s > 0.0f)) return 0u;
-    const float y = quotient_odd(x, s);
+    float y[4];
+    bool near = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        y[i] = x[i] * inv;
+        if constexpr (FMT == kI8) {
+            // 2^-23 of 127 is under 2^-16
+            near |= fabsf(fabsf(y[i] - rintf(y[i])) - 0.5f) < 0x1p-15f;
+        } else {
+            // the 20 bits behind a code's mantissa, 8 units around their middle; numbers that
+            // become denormal codes have fewer bits
+            const unsigned cut = (__float_as_uint(y[i]) & 0xfffffu) - 0x7fff8u;
+            near |= cut <= 16u || (fabsf(y[i]) < 0x1p-6f && y[i] != 0.0f);
+        }
+    }
+    if (near) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = quotient_odd(x[i], s);
+    }
     if constexpr (FMT == kI8) {
-        const int c = (int)rintf(fminf(fmaxf(y, -127.0f), 127.0f));
-        return (unsigned)c & 0xffu;
+        unsigned w = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w |= ((unsigned)(int)rintf(y[i]) & 0xffu) << (8 * i);
+        return w;
     } else {
-        const float c = fminf(fmaxf(y, -448.0f), 448.0f);
-        return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, c, 0, false) & 0xffu;
+        const int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+        return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
     }
 }
 

@@ -388,74 +388,142 @@ __global__ __launch_bounds__(256) void cache8_join_kernel(Cache8 c, Cache8Query 
             l == 0.0f ? -__builtin_inff() : (m - kLift + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// Accounts: a wavefront owns 64 tokens of a head and walks the rows, 16 at a time.
-template <int D, int FMT>
-__global__ __launch_bounds__(256) void cache8_weights_kernel(Cache8 c, Cache8Query q) {
+// Accounts.  A wavefront holds 16 * MT query rows, as for attention, and walks tiles of 64 tokens: the
+// weights of a lane's 16 tokens are added over the row tiles, then over the 16 rows of its group, and
+// lane l ends up with token l's.  Where a KV head has more rows than that, row groups leave their sums
+// in `part` [group][head][capacity] and cache8_weights_join_kernel adds them in order; a group of
+// several chunks of rows adds to what its own chunks before left there.  groups == 1 writes the
+// accounts themselves.  One query row in 16 lanes' worth of columns costs as much as 16, so a decode
+// step is bound by reading K; a prompt's chunk by the vector unit (exp2 and the conversions of K).
+template <int D, int FMT, int MT>
+__global__ __launch_bounds__(256) void cache8_weights_kernel(Cache8 c, Cache8Query q, int row_waves,
+                                                             int groups, int chunks, float* part) {
     const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int sh = blockIdx.y;
+    const int sh = blockIdx.x, tok_waves = 4 / row_waves;
+    const int group = (int)blockIdx.y * row_waves + wave % row_waves;
+    const int worker = (int)blockIdx.z * tok_waves + wave / row_waves;
+    const int workers = (int)gridDim.z * tok_waves;
     RowSpan p;
     p.s = sh / c.kv;
     p.h = sh - p.s * c.kv;
     p.len = seq_length(c, p.s);
     p.count = seq_count(q.counts, q.n, p.s);
     p.rows = p.count * q.group;
-    const int t0 = ((int)blockIdx.x * 4 + wave) * kCacheTile;
-    if (t0 >= p.len) return;
-    u4 kr[4][D / 64];
-    load_k<D>(c.k + ((int64_t)sh * c.cap + t0) * D, kr);
-    const float ks = c.k_scale[(int64_t)sh * (c.cap >> c.block_log2) +
-                               (min(t0 + 16 * g, p.len - 1) >> c.block_log2)];
-    float acc[16];
+    const uint8_t* kp = c.k + (int64_t)sh * c.cap * D;
+    const float* ksp = c.k_scale + (int64_t)sh * (c.cap >> c.block_log2);
+    const int last_block = max(p.len - 1, 0) >> c.block_log2;
+    const int64_t at0 = (int64_t)sh * c.cap;
+    float* const out = groups == 1 ? q.acc_out + at0
+                                   : part + ((int64_t)group * gridDim.x + sh) * c.cap;
+    if (groups == 1 && p.rows == 0) {
+        for (int t = worker * 64 + lane; t < p.len; t += workers * 64)
+            out[t] = q.acc_in ? q.acc_in[at0 + t] : 0.0f;
+        return;
+    }
+
+    int before = 0;  // tiles that the group's chunks so far have written
+    for (int chunk = 0; chunk < chunks; ++chunk) {
+        const int r0 = (group * chunks + chunk) * 16 * MT;
+        if (r0 >= p.rows) return;
+        const int last = min(p.rows, r0 + 16 * MT) - 1;
+        const int tiles = (max(p.len - p.count + last / q.group + 1, 0) + kCacheTile - 1) / kCacheTile;
+        const int open = max(p.len - p.count + r0 / q.group + 1, 0);  // seen by every row
+        h8 qh[MT][D / 32], ql[MT][D / 32];
+        float back[MT], at[MT];
+        int limit[MT];
+        bool whole = true;
 #pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
-    // the first row that sees a token of the tile
-    const int first = max(t0 - (p.len - p.count), 0) * q.group;
-    for (int r0 = first & ~15; r0 < p.rows; r0 += 16) {
-        h8 qh[D / 32], ql[D / 32];
-        float back;
-        int limit;
-        load_q<D>(q, p, r0 + li, qh, ql, back, limit);
-        const int r = r0 + li, i = r / q.group;
-        const float lse = r < p.rows
-            ? q.lse[((int64_t)p.s * q.heads + p.h * q.group + r - i * q.group) * q.n + i]
-            : -__builtin_inff();
-        if (!(lse > -__builtin_inff()) && lse == lse) limit = 0;  // no such row, or an empty one
-        const float f = ks * back, at = -lse * kLog2e;
+        for (int t = 0; t < MT; ++t) {
+            const int r = r0 + 16 * t + li;
+            load_q<D>(q, p, r, qh[t], ql[t], back[t], limit[t]);
+            const int i = min(r, p.rows - 1) / q.group, head = p.h * q.group + min(r, p.rows - 1) - i * q.group;
+            const float lse = q.lse[((int64_t)p.s * q.heads + head) * q.n + i];
+            // no such row, or one that saw nothing
+            if (r >= p.rows || lse == -__builtin_inff()) limit[t] = 0;
+            whole = whole && limit[t] > 0;
+            at[t] = -lse * kLog2e;
+        }
+        const bool gaps = !__all(whole);
+        int tile = worker;
+        u4 kr[4][D / 64];
+        float ks = 0.0f;
+        auto fetch = [&](int t) __attribute__((always_inline)) {
+            load_k<D>(kp + (int64_t)t * kCacheTile * D, kr);
+            ks = ksp[min((t * kCacheTile + 16 * g) >> c.block_log2, last_block)];
+        };
+        if (tile < tiles) fetch(tile);
+        for (; tile < tiles; tile += workers) {
+            const int t0 = tile * kCacheTile;
+            float v[16], f[MT];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            f4 sc = {0.f, 0.f, 0.f, 0.f};
+            for (int e = 0; e < 16; ++e) v[e] = 0.0f;
 #pragma unroll
-            for (int a = 0; a < D / 32; ++a) {
-                const u4 w = kr[j][a >> 1];
-                const h8 kf = a & 1 ? codes8<FMT>(w.z, w.w) : codes8<FMT>(w.x, w.y);
-                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[a], sc, 0, 0, 0);
-                sc = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[a], sc, 0, 0, 0);
+            for (int t = 0; t < MT; ++t) f[t] = ks * back[t];
+            const bool edge = gaps || t0 + kCacheTile > open;
+            f4 sc[MT][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t) sc[t][j] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int a = 0; a < D / 32; ++a) {
+                    const u4 w = kr[j][a >> 1];
+                    const h8 kf = a & 1 ? codes8<FMT>(w.z, w.w) : codes8<FMT>(w.x, w.y);
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        sc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, ql[t][a], sc[t][j], 0, 0, 0);
+                        sc[t][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qh[t][a], sc[t][j], 0, 0, 0);
+                    }
+                }
             }
+            if (tile + workers < tiles) fetch(tile + workers);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], f, at));
-                acc[4 * j + e] += t0 + 16 * g + 4 * j + e < limit ? w : 0.0f;
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j][e], f[t], at[t]));
+                        if (edge && t0 + 16 * g + 4 * j + e >= limit[t]) w = 0.0f;
+                        v[4 * j + e] += w;
+                    }
+            // over the 16 rows of a lane group: each step halves the tokens a lane answers for
+#pragma unroll
+            for (int step = 8; step > 0; step >>= 1) {
+                const bool up = li & step;
+#pragma unroll
+                for (int e = 0; e < step; ++e) {
+                    const float mine = up ? v[e + step] : v[e], other = up ? v[e] : v[e + step];
+                    v[e] = mine + __shfl_xor(other, step);
+                }
+            }
+            const int t = t0 + lane;
+            if (t < p.len) {
+                float sum = v[0];
+                if (tile < before) sum = out[t] + sum;
+                else if (groups == 1 && q.acc_in) sum = q.acc_in[at0 + t] + sum;
+                out[t] = sum;
             }
         }
+        before = tiles;
     }
-    // over the 16 rows of a lane group: each step halves the tokens a lane answers for
-    float v[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = acc[e];
-#pragma unroll
-    for (int step = 8; step > 0; step >>= 1) {
-        const bool up = li & step;
-#pragma unroll
-        for (int e = 0; e < step; ++e) {
-            const float mine = up ? v[e + step] : v[e], other = up ? v[e] : v[e + step];
-            v[e] = mine + __shfl_xor(other, step);
-        }
-    }
-    const int t = t0 + lane;
-    if (t >= p.len) return;
-    const int64_t at = (int64_t)sh * c.cap + t;
-    q.acc_out[at] = (q.acc_in ? q.acc_in[at] : 0.0f) + v[0];
+}
+
+// acc_out = acc_in + the row groups' sums, in order.
+__global__ __launch_bounds__(256) void cache8_weights_join_kernel(Cache8 c, Cache8Query q, int groups,
+                                                                  int rows_of_group, const float* part) {
+    const int sh = blockIdx.y, s = sh / c.kv, t = (int)blockIdx.x * 256 + threadIdx.x;
+    const int len = seq_length(c, s), count = seq_count(q.counts, q.n, s);
+    if (t >= len) return;
+    // the groups with a row that sees token t
+    const int first = max(t - (len - count), 0) * q.group / rows_of_group;
+    const int end = (count * q.group + rows_of_group - 1) / rows_of_group;
+    const int64_t at = (int64_t)sh * c.cap + t, stride = (int64_t)gridDim.y * c.cap;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int i = first; i < end; ++i) sum += part[i * stride + at];
+    q.acc_out[at] = (q.acc_in ? q.acc_in[at] : 0.0f) + sum;
 }
 
 }  // namespace
@@ -480,10 +548,6 @@ Cache8Plan cache8_attend_plan(const Cache8& c, int head_dim, int64_t rows, int c
     return p;
 }
 
-#define SHP_CACHE8_KERNEL(KERN, head_dim, format)                                   \
-    ((head_dim) == 64 ? ((format) == SHP_CACHE8_I8 ? KERN<64, shpd::kI8> : KERN<64, shpd::kE4M3>) \
-                      : ((format) == SHP_CACHE8_I8 ? KERN<128, shpd::kI8> : KERN<128, shpd::kE4M3>))
-
 int cache8_attend_launch(hipStream_t s, const Cache8& c, int head_dim, int format,
                          const Cache8Query& q, const Cache8Plan& p, float* scratch) {
     const bool i8 = format == SHP_CACHE8_I8;
@@ -507,12 +571,41 @@ int cache8_attend_launch(hipStream_t s, const Cache8& c, int head_dim, int forma
     return SHP_OK;
 }
 
+// A row group a wavefront, as long as their sums fit 64 MiB; about 8,192 wavefronts, each with four
+// tiles or more.
+Cache8WeightsPlan cache8_weights_plan(const Cache8& c, int head_dim, int64_t rows, bool may_group) {
+    Cache8WeightsPlan p;
+    p.row_tiles = rows <= 16 ? 1 : rows <= 32 || head_dim == 128 ? 2 : 4;
+    const int64_t per = 16 * p.row_tiles, all = std::max<int64_t>((rows + per - 1) / per, 1);
+    const int64_t heads = (int64_t)c.n_seqs * c.kv, one = heads * c.cap;
+    int64_t groups = may_group ? std::min(all, std::max<int64_t>((16ll << 20) / one, 1)) : 1;
+    p.chunks = (int)((all + groups - 1) / groups);
+    p.groups = (int)((all + p.chunks - 1) / p.chunks);
+    p.row_waves = p.groups >= 4 ? 4 : p.groups >= 2 ? 2 : 1;
+    const int64_t tok_waves = 4 / p.row_waves, tiles = c.cap / kCacheTile;
+    const int64_t want = 8192 / std::max<int64_t>(heads * p.groups, 1), most = (tiles + 3) / 4;
+    p.workers = (int)((std::max<int64_t>(std::min(want, most), 1) + tok_waves - 1) / tok_waves);
+    p.scratch = p.groups > 1 ? (size_t)(one * p.groups) : 0;
+    return p;
+}
+
 int cache8_weights_launch(hipStream_t s, const Cache8& c, int head_dim, int format,
-                          const Cache8Query& q) {
-    const int per = 4 * kCacheTile;
-    hipLaunchKernelGGL(SHP_CACHE8_KERNEL(cache8_weights_kernel, head_dim, format),
-                       dim3((c.cap + per - 1) / per, c.n_seqs * c.kv), dim3(256), 0, s, c, q);
+                          const Cache8Query& q, const Cache8WeightsPlan& p, float* scratch) {
+    const bool i8 = format == SHP_CACHE8_I8;
+    auto kern = head_dim == 64
+        ? (p.row_tiles == 1   ? (i8 ? cache8_weights_kernel<64, kI8, 1> : cache8_weights_kernel<64, kE4M3, 1>)
+           : p.row_tiles == 2 ? (i8 ? cache8_weights_kernel<64, kI8, 2> : cache8_weights_kernel<64, kE4M3, 2>)
+                              : (i8 ? cache8_weights_kernel<64, kI8, 4> : cache8_weights_kernel<64, kE4M3, 4>))
+        : (p.row_tiles == 1   ? (i8 ? cache8_weights_kernel<128, kI8, 1> : cache8_weights_kernel<128, kE4M3, 1>)
+                              : (i8 ? cache8_weights_kernel<128, kI8, 2> : cache8_weights_kernel<128, kE4M3, 2>));
+    hipLaunchKernelGGL(kern, dim3(c.n_seqs * c.kv, (p.groups + p.row_waves - 1) / p.row_waves, p.workers),
+                       dim3(256), 0, s, c, q, p.row_waves, p.groups, p.chunks, scratch);
     SHP_HIP_CHECK(hipGetLastError());
+    if (p.groups > 1) {
+        hipLaunchKernelGGL(cache8_weights_join_kernel, dim3((c.cap + 255) / 256, c.n_seqs * c.kv),
+                           dim3(256), 0, s, c, q, p.groups, 16 * p.row_tiles * p.chunks, scratch);
+        SHP_HIP_CHECK(hipGetLastError());
+    }
     return SHP_OK;
 }
 
