@@ -135,7 +135,7 @@ __device__ __forceinline__ void load_v(const uint8_t* tile, u4 raw[D / 16]) {
 }
 
 template <int D, int FMT, int MT>
-__global__ __launch_bounds__(256) void cache8_attend_kernel(Cache8 c, Cache8Query q, int row_waves,
+__global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Query q, int row_waves,
                                                             int splits, float* part) {
     constexpr int NO = D / 16;  // accumulators of 16 rows
     __shared__ __attribute__((aligned(16))) float ex[2][MT * (NO * 4 + 2) * 64];
@@ -388,6 +388,18 @@ __global__ __launch_bounds__(256) void cache8_join_kernel(Cache8 c, Cache8Query 
             l == 0.0f ? -__builtin_inff() : (m - kLift + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
+// v[e] of lanes l and l ^ STEP added, for the half of the 2 * STEP indices whose STEP bit is the
+// lane's own: after steps 8, 4, 2 and 1, v[0] is the sum of v[l % 16] over the 16 lanes.
+template <int STEP>
+__device__ __forceinline__ void halve(float* v) {
+    const bool up = threadIdx.x & STEP;
+#pragma unroll
+    for (int e = 0; e < STEP; ++e) {
+        const float mine = up ? v[e + STEP] : v[e], other = up ? v[e] : v[e + STEP];
+        v[e] = mine + __shfl_xor(other, STEP);
+    }
+}
+
 // Accounts.  A wavefront holds 16 * MT query rows, as for attention, and walks tiles of 64 tokens: the
 // weights of a lane's 16 tokens are added over the row tiles, then over the 16 rows of its group, and
 // lane l ends up with token l's.  Where a KV head has more rows than that, row groups leave their sums
@@ -396,7 +408,7 @@ __global__ __launch_bounds__(256) void cache8_join_kernel(Cache8 c, Cache8Query 
 // accounts themselves.  One query row in 16 lanes' worth of columns costs as much as 16, so a decode
 // step is bound by reading K; a prompt's chunk by the vector unit (exp2 and the conversions of K).
 template <int D, int FMT, int MT>
-__global__ __launch_bounds__(256) void cache8_weights_kernel(Cache8 c, Cache8Query q, int row_waves,
+__global__ __launch_bounds__(256, 2) void cache8_weights_kernel(Cache8 c, Cache8Query q, int row_waves,
                                                              int groups, int chunks, float* part) {
     const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -478,26 +490,28 @@ __global__ __launch_bounds__(256) void cache8_weights_kernel(Cache8 c, Cache8Que
                 }
             }
             if (tile + workers < tiles) fetch(tile + workers);
+            if (edge) {
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+                for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        float w = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j][e], f[t], at[t]));
-                        if (edge && t0 + 16 * g + 4 * j + e >= limit[t]) w = 0.0f;
-                        v[4 * j + e] += w;
+                    for (int e = 0; e < 16; ++e) {
+                        const float w = __builtin_amdgcn_exp2f(
+                            __builtin_fmaf(sc[t][e >> 2][e & 3], f[t], at[t]));
+                        v[e] += t0 + 16 * g + e < limit[t] ? w : 0.0f;
                     }
-            // over the 16 rows of a lane group: each step halves the tokens a lane answers for
+            } else {
 #pragma unroll
-            for (int step = 8; step > 0; step >>= 1) {
-                const bool up = li & step;
+                for (int t = 0; t < MT; ++t)
 #pragma unroll
-                for (int e = 0; e < step; ++e) {
-                    const float mine = up ? v[e + step] : v[e], other = up ? v[e] : v[e + step];
-                    v[e] = mine + __shfl_xor(other, step);
-                }
+                    for (int e = 0; e < 16; ++e)
+                        v[e] += __builtin_amdgcn_exp2f(
+                            __builtin_fmaf(sc[t][e >> 2][e & 3], f[t], at[t]));
             }
+            // over the 16 rows of a lane group
+            halve<8>(v);
+            halve<4>(v);
+            halve<2>(v);
+            halve<1>(v);
             const int t = t0 + lane;
             if (t < p.len) {
                 float sum = v[0];
