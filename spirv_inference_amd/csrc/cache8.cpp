@@ -137,7 +137,7 @@ int shp_cache8_attend(shp_ctx* ctx, const shp_cache8* cache, const shp_cache8_at
     q.n = a->n; q.heads = a->n_heads; q.group = group; q.scale = a->scale;
     return x->timed("cache8_attend", [&] {
         return shp::cache8_attend_launch(x->stream, c, cache->head_dim, cache->format, q, plan,
-                                         scratch);
+                                         scratch, (int*)x->workspace);
     });
 }
 

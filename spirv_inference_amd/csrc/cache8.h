@@ -46,16 +46,17 @@ int cache8_read_launch(hipStream_t s, const Cache8& c, int head_dim, int format,
                        float* v);
 // How attention splits the tokens of a sequence, and the floats of scratch that takes (0: none).
 struct Cache8Plan {
-    int row_tiles;   // 16-row tiles a wavefront owns
-    int row_waves;   // wavefronts of a workgroup side by side over rows; the rest split its tokens
+    int row_tiles;   // 16-row tiles a workgroup owns
     int row_blocks;  // workgroups over the rows of one KV head
-    int splits;      // workgroups over the tokens
+    int splits;      // workgroups over the tokens of a sequence at most
+    int least;       // tiles a workgroup takes at least
     size_t scratch;
 };
 Cache8Plan cache8_attend_plan(const Cache8& c, int head_dim, int64_t rows, int cu_count,
                               bool may_split);
 int cache8_attend_launch(hipStream_t s, const Cache8& c, int head_dim, int format,
-                         const Cache8Query& q, const Cache8Plan& p, float* scratch);
+                         const Cache8Query& q, const Cache8Plan& p, float* scratch,
+                         int* counters);
 // How the accounts' rows and tokens are shared out, and the floats of scratch that takes (0: none).
 struct Cache8WeightsPlan {
     int row_tiles;  // 16-row tiles a wavefront holds

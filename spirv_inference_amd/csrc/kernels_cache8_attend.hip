@@ -15,6 +15,8 @@
 // w_t = 2^(u_t - m + 12) is what multiplies V's codes: it spans fp16's range whatever the scales
 // are, and the row's sum is that of w_t / scale.
 #include "cache8.h"
+#include "coherent.h"
+#include "gemm.h"
 
 namespace {
 
@@ -134,30 +136,44 @@ __device__ __forceinline__ void load_v(const uint8_t* tile, u4 raw[D / 16]) {
         raw[d] = *reinterpret_cast<const u4*>(p + d * 16 * kCacheTile);
 }
 
+// 2^(m - top), also where both are minus infinity or infinity.
+__device__ __forceinline__ float factor_of(float m, float top) {
+    return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+}
+
+// The log of a row's sum from its maximum and weight as the wavefronts keep them.
+__device__ __forceinline__ float log_sum(float m, float l) {
+    return l == 0.0f ? -__builtin_inff() : (m - kLift + __builtin_amdgcn_logf(l)) * kLn2;
+}
+
 template <int D, int FMT, int MT>
-__global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Query q, int row_waves,
-                                                            int splits, float* part) {
-    constexpr int NO = D / 16;  // accumulators of 16 rows
+__global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Query q, int least,
+                                                               float* part, int* counters) {
+    constexpr int NO = D / 16;   // accumulators of 16 rows
+    constexpr int PW = D + 4;    // floats of a row's part: sums, maximum, weight, two of padding
     __shared__ __attribute__((aligned(16))) float ex[2][MT * (NO * 4 + 2) * 64];
+    __shared__ int arrived;
+    constexpr int ROWS = 16 * MT, WAVES = 4;
     const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int sh = blockIdx.x, tok_waves = 4 / row_waves;
-    const int wr = wave % row_waves, wt = wave / row_waves;
+    const int sh = blockIdx.x;
     RowSpan p;
     p.s = sh / c.kv;
     p.h = sh - p.s * c.kv;
     p.len = seq_length(c, p.s);
     p.count = seq_count(q.counts, q.n, p.s);
     p.rows = p.count * q.group;
-    const int wg_rows = 16 * MT * row_waves, base = (int)blockIdx.y * wg_rows;
-    if (base >= p.rows) return;
-    const int r0 = base + wr * 16 * MT;
+    const int r0 = (int)(gridDim.y - 1 - blockIdx.y) * ROWS;  // those that see most begin first
+    if (r0 >= p.rows) return;
 
-    // tokens the workgroup's last row sees, and its share of their tiles
-    const int last = min(p.rows, base + wg_rows) - 1;
+    // tokens the workgroup's last row sees, in as many shares as there are workgroups for it, none of
+    // fewer tiles than `least` but the last
+    const int last = min(p.rows, r0 + ROWS) - 1;
     const int sees = max(p.len - p.count + last / q.group + 1, 0);
     const int tiles = (sees + kCacheTile - 1) / kCacheTile;
-    const int share = (tiles + splits - 1) / splits;
+    const int share = max((tiles + (int)gridDim.z - 1) / (int)gridDim.z, least);
+    const int splits = max((tiles + share - 1) / share, 1);
+    if ((int)blockIdx.z >= splits) return;
     const int tile0 = (int)blockIdx.z * share, tile1 = min(tiles, tile0 + share);
 
     float m[MT], l[MT], back[MT];
@@ -172,15 +188,15 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
 #pragma unroll
         for (int d = 0; d < NO; ++d) o[t][d] = f4{0.f, 0.f, 0.f, 0.f};
     }
-    // tokens that every row of this wavefront sees
-    const int open = max(p.len - p.count + min(r0, p.rows - 1) / q.group + 1, 0);
+    // tokens that every row sees
+    const int open = max(p.len - p.count + r0 / q.group + 1, 0);
 
     const uint8_t* kp = c.k + (int64_t)sh * c.cap * D;
     const uint8_t* vp = c.v + (int64_t)sh * c.cap * D;
     const int64_t sbase = (int64_t)sh * (c.cap >> c.block_log2);
     const int last_block = max(p.len - 1, 0) >> c.block_log2;
 
-    for (int tile = tile0 + wt; tile < tile1; tile += tok_waves) {
+    for (int tile = tile0 + wave; tile < tile1; tile += WAVES) {
         const int t0 = tile * kCacheTile;
         u4 kr[4][D / 64], vr[NO];
         load_k<D>(kp + (int64_t)t0 * D, kr);
@@ -190,17 +206,6 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
         float vs = c.v_scale[b];
         vs = vs < kScaleFloor ? kScaleFloor : vs;
         const bool edge = t0 + kCacheTile > open;
-        if (FMT == kE4M3 && t0 + kCacheTile > p.len) {
-            // bytes behind the last token may be NaN codes, which a weight of zero does not cancel
-#pragma unroll
-            for (int d = 0; d < NO; ++d)
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const int left = p.len - t0 - 16 * g - 4 * w;
-                    vr[d][w] &= left >= 4 ? ~0u : left <= 0 ? 0u : (1u << 8 * left) - 1;
-                }
-        }
-
         f4 sc[MT][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -237,7 +242,7 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[t][j][i]);
             const float top = fmaxf(m[t], max_over_groups(__builtin_fmaf(mx, f, lv)));
             if (__any(top > m[t])) {
-                const float down = m[t] == top ? 1.0f : __builtin_amdgcn_exp2f(m[t] - top);
+                const float down = factor_of(m[t], top);
                 l[t] *= down;
 #pragma unroll
                 for (int d = 0; d < NO; ++d) o[t][d] *= down;
@@ -283,6 +288,16 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
             }
             if (sum != 0.0f) l[t] += sum / vs;  // of a block nobody sees, the scale may be NaN
         }
+        if (FMT == kE4M3 && t0 + kCacheTile > p.len) {
+            // bytes behind the last token may be NaN codes, which a weight of zero does not cancel
+#pragma unroll
+            for (int d = 0; d < NO; ++d)
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const int left = p.len - t0 - 16 * g - 4 * w;
+                    vr[d][w] &= left >= 4 ? ~0u : left <= 0 ? 0u : (1u << 8 * left) - 1;
+                }
+        }
 #pragma unroll
         for (int d = 0; d < NO; ++d) {
 #pragma unroll
@@ -302,11 +317,11 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
         l[t] += __shfl_xor(l[t], 32);
     }
 
-    // wavefronts of the same rows, in pairs: the upper one's part goes through LDS
-    for (int step = tok_waves >> 1; step > 0; step >>= 1) {
-        const int slot = (wt & (step - 1)) * row_waves + wr;
-        float* x = ex[slot];
-        if (wt >= step && wt < 2 * step)
+    // the wavefronts' parts, in pairs: the upper one's goes through LDS
+#pragma unroll
+    for (int step = WAVES / 2; step > 0; step >>= 1) {
+        float* x = ex[wave & (step - 1)];
+        if (wave >= step && wave < 2 * step)
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
 #pragma unroll
@@ -316,14 +331,13 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
                 x[(MT * NO * 4 + 2 * t + 1) * 64 + lane] = l[t];
             }
         __syncthreads();
-        if (wt < step)
+        if (wave < step)
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
                 const float m1 = x[(MT * NO * 4 + 2 * t) * 64 + lane];
                 const float l1 = x[(MT * NO * 4 + 2 * t + 1) * 64 + lane];
                 const float top = fmaxf(m[t], m1);
-                const float f0 = m[t] == top ? 1.0f : __builtin_amdgcn_exp2f(m[t] - top);
-                const float f1 = m1 == top ? 1.0f : __builtin_amdgcn_exp2f(m1 - top);
+                const float f0 = factor_of(m[t], top), f1 = factor_of(m1, top);
                 l[t] = l[t] * f0 + l1 * f1;
                 m[t] = top;
 #pragma unroll
@@ -333,59 +347,102 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
             }
         __syncthreads();
     }
-    if (wt) return;
 
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int r = r0 + 16 * t + li;
-        if (r >= p.rows) continue;
-        if (splits > 1) {
-            // part: [sh][split][row][D + 2], rows of the launch's row blocks
-            const int64_t at = ((int64_t)sh * splits + blockIdx.z) * gridDim.y * wg_rows + r;
-            float* x = part + at * (D + 4);
-#pragma unroll
-            for (int d = 0; d < NO; ++d) *reinterpret_cast<f4*>(x + 16 * d + 4 * g) = o[t][d];
-            if (g == 0) *reinterpret_cast<f4*>(x + D) = f4{m[t], l[t], 0.f, 0.f};
-            continue;
-        }
+    // a row's place in out and lse
+    auto place = [&](int r, int64_t& at, int64_t& at_lse) __attribute__((always_inline)) {
         const int i = r / q.group, head = p.h * q.group + r - i * q.group;
-        const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
-        float* x = q.out + p.s * q.o_seq + i * q.o_row + head * q.o_head + 4 * g;
+        at = p.s * q.o_seq + i * q.o_row + head * q.o_head;
+        at_lse = ((int64_t)p.s * q.heads + head) * q.n + i;
+    };
+    if (splits == 1) {
+        if (wave) return;
 #pragma unroll
-        for (int d = 0; d < NO; ++d) *reinterpret_cast<f4*>(x + 16 * d) = o[t][d] * inv;
-        if (q.lse && g == 0)
-            q.lse[((int64_t)p.s * q.heads + head) * q.n + i] =
-                l[t] == 0.0f ? -__builtin_inff()
-                             : (m[t] - kLift + __builtin_amdgcn_logf(l[t])) * kLn2;
+        for (int t = 0; t < MT; ++t) {
+            const int r = r0 + 16 * t + li;
+            if (r >= p.rows) continue;
+            int64_t at, at_lse;
+            place(r, at, at_lse);
+            const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+#pragma unroll
+            for (int d = 0; d < NO; ++d)
+                *reinterpret_cast<f4*>(q.out + at + 16 * d + 4 * g) = o[t][d] * inv;
+            if (q.lse && g == 0) q.lse[at_lse] = log_sum(m[t], l[t]);
+        }
+        return;
     }
-}
 
-// Joins the parts of a row: thread = 4 dimensions.
-template <int D>
-__global__ __launch_bounds__(256) void cache8_join_kernel(Cache8 c, Cache8Query q, int splits,
-                                                          int row_slots, const float* part) {
-    constexpr int T = D / 4;
-    const int sh = blockIdx.x, s = sh / c.kv, h = sh - s * c.kv;
-    const int r = (int)blockIdx.y * (256 / T) + threadIdx.x / T, d = threadIdx.x % T * 4;
-    if (r >= seq_count(q.counts, q.n, s) * q.group) return;
-    const int64_t stride = (int64_t)row_slots * (D + 4);
-    const float* x = part + ((int64_t)sh * splits * row_slots + r) * (D + 4);
-    float m = -__builtin_inff();
-    for (int i = 0; i < splits; ++i) m = fmaxf(m, x[i * stride + D]);
-    float l = 0.0f;
-    f4 o = {0.f, 0.f, 0.f, 0.f};
-    for (int i = 0; i < splits; ++i) {
-        const float mi = x[i * stride + D];
-        const float f = mi == m ? 1.0f : __builtin_amdgcn_exp2f(mi - m);
-        l += x[i * stride + D + 1] * f;
-        o += *reinterpret_cast<const f4*>(x + i * stride + d) * f;
+    // Every share stores its rows' parts past the caches that other XCDs do not see; the last to
+    // arrive joins them, and leaves the counter at zero for the next launch.
+    const int unit = (int)blockIdx.y * (int)gridDim.x + sh, rows = min(p.rows - r0, ROWS);
+    const __amdgpu_buffer_rsrc_t pr =
+        buffer_rsrc(part + (int64_t)unit * gridDim.z * ROWS * PW, (int64_t)gridDim.z * ROWS * PW);
+    if (wave == 0) {
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            const int r = 16 * t + li;
+            if (r >= rows) continue;
+            const unsigned at = (unsigned)(((int)blockIdx.z * ROWS + r) * PW) * 4u;
+#pragma unroll
+            for (int d = 0; d < NO; ++d)
+                st_coh16(pr, at + (16 * d + 4 * g) * 4u,
+                         make_float4(o[t][d].x, o[t][d].y, o[t][d].z, o[t][d].w));
+            if (g == 0) st_coh16(pr, at + D * 4u, make_float4(m[t], l[t], 0.f, 0.f));
+        }
     }
-    const int i = r / q.group, head = h * q.group + r - i * q.group;
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    *reinterpret_cast<f4*>(q.out + s * q.o_seq + i * q.o_row + head * q.o_head + d) = o * inv;
-    if (q.lse && d == 0)
-        q.lse[((int64_t)s * q.heads + head) * q.n + i] =
-            l == 0.0f ? -__builtin_inff() : (m - kLift + __builtin_amdgcn_logf(l)) * kLn2;
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's parts are stored
+    __syncthreads();
+    if (threadIdx.x == 0)
+        arrived = __hip_atomic_fetch_add((SHP_GLOBAL int*)(counters + unit), 1, __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (arrived != splits - 1) return;
+    if (threadIdx.x == 0)
+        __hip_atomic_store((SHP_GLOBAL int*)(counters + unit), 0, __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+    // factors 2^(m_i - m) of every share and row [splits][rows], then the rows' m and l
+    float* const factor = &ex[0][0];
+    float* const weight = factor + splits * rows;
+    float* const rm = weight + splits * rows;
+    for (int e = threadIdx.x; e < splits * rows; e += 256) {
+        const int i = e / rows, r = e - i * rows;
+        const float4 x = ld_coh16(pr, (unsigned)((i * ROWS + r) * PW + D) * 4u, 0);
+        factor[e] = x.x;
+        weight[e] = x.y;
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < rows) {
+        const int r = threadIdx.x;
+        float top = -__builtin_inff(), sum = 0.0f;
+        for (int i = 0; i < splits; ++i) top = fmaxf(top, factor[i * rows + r]);
+        for (int i = 0; i < splits; ++i) {
+            const float f = factor_of(factor[i * rows + r], top);
+            factor[i * rows + r] = f;
+            sum += weight[i * rows + r] * f;
+        }
+        rm[r] = top;
+        rm[rows + r] = sum;
+    }
+    __syncthreads();
+    constexpr int T = D / 4;
+    for (int e = threadIdx.x; e < rows * T; e += 256) {
+        const int r = e / T, d = e % T * 4;
+        f4 sum = {0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < splits; i0 += 8) {  // eight loads in flight
+            float4 x[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x[i] = ld_coh16(pr, (unsigned)((min(i0 + i, splits - 1) * ROWS + r) * PW + d) * 4u, 0);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i0 + i < splits)
+                    sum += f4{x[i].x, x[i].y, x[i].z, x[i].w} * factor[(i0 + i) * rows + r];
+        }
+        int64_t at, at_lse;
+        place(r0 + r, at, at_lse);
+        const float total = rm[rows + r];
+        *reinterpret_cast<f4*>(q.out + at + d) = sum * (total == 0.0f ? 0.0f : 1.0f / total);
+        if (q.lse && d == 0) q.lse[at_lse] = log_sum(rm[r], total);
+    }
 }
 
 // v[e] of lanes l and l ^ STEP added, for the half of the 2 * STEP indices whose STEP bit is the
@@ -547,41 +604,32 @@ namespace shp {
 Cache8Plan cache8_attend_plan(const Cache8& c, int head_dim, int64_t rows, int cu_count,
                               bool may_split) {
     Cache8Plan p;
-    const int widest = head_dim == 64 ? 4 : 2;
-    p.row_tiles = rows <= 16 ? 1 : rows <= 32 || widest == 2 ? 2 : 4;
-    const int64_t tiles16 = (rows + 15) / 16;
-    p.row_waves = tiles16 > 2 * p.row_tiles ? 4 : tiles16 > p.row_tiles ? 2 : 1;
-    const int64_t per = 16 * p.row_tiles * p.row_waves;
-    p.row_blocks = (int)std::min<int64_t>((rows + per - 1) / per, 1 << 30);
-    // enough workgroups for four on every CU, none with fewer tokens than a tile a wavefront
+    p.row_tiles = rows <= 16 ? 1 : 2;
+    const int64_t per = 16 * p.row_tiles;
+    p.row_blocks = (int)((rows + per - 1) / per);
+    // Workgroups for 8 on every CU with 16 rows, which evens out sequences of different length, and
+    // for the two that it holds at once with 32; a workgroup takes two tiles a wavefront or more.
     const int64_t units = (int64_t)c.n_seqs * c.kv * p.row_blocks;
-    const int64_t want = (4ll * std::max(cu_count, 1) + units - 1) / units;
-    const int64_t most = std::max<int64_t>(c.cap / (kCacheTile * (4 / p.row_waves)), 1);
-    p.splits = may_split ? (int)std::min<int64_t>(std::min(want, most), 1024) : 1;
+    const int64_t want = ((p.row_tiles == 2 ? 2 : 8) * (int64_t)std::max(cu_count, 1) + units - 1) / units;
+    p.least = 8;
+    const int64_t most = (c.cap / kCacheTile + p.least - 1) / p.least;
+    p.splits = (int)std::max<int64_t>(std::min<int64_t>(std::min(want, most), 32), 1);
+    if (!may_split || units * (int64_t)sizeof(int) > (int64_t)kSplitCounterBytes) p.splits = 1;
     p.scratch = p.splits > 1 ? (size_t)units * per * p.splits * (head_dim + 4) : 0;
     return p;
 }
 
 int cache8_attend_launch(hipStream_t s, const Cache8& c, int head_dim, int format,
-                         const Cache8Query& q, const Cache8Plan& p, float* scratch) {
+                         const Cache8Query& q, const Cache8Plan& p, float* scratch, int* counters) {
     const bool i8 = format == SHP_CACHE8_I8;
     auto kern = head_dim == 64
         ? (p.row_tiles == 1   ? (i8 ? cache8_attend_kernel<64, kI8, 1> : cache8_attend_kernel<64, kE4M3, 1>)
-           : p.row_tiles == 2 ? (i8 ? cache8_attend_kernel<64, kI8, 2> : cache8_attend_kernel<64, kE4M3, 2>)
-                              : (i8 ? cache8_attend_kernel<64, kI8, 4> : cache8_attend_kernel<64, kE4M3, 4>))
+                              : (i8 ? cache8_attend_kernel<64, kI8, 2> : cache8_attend_kernel<64, kE4M3, 2>))
         : (p.row_tiles == 1   ? (i8 ? cache8_attend_kernel<128, kI8, 1> : cache8_attend_kernel<128, kE4M3, 1>)
                               : (i8 ? cache8_attend_kernel<128, kI8, 2> : cache8_attend_kernel<128, kE4M3, 2>));
     hipLaunchKernelGGL(kern, dim3(c.n_seqs * c.kv, p.row_blocks, p.splits), dim3(256), 0, s, c, q,
-                       p.row_waves, p.splits, scratch);
+                       p.least, scratch, counters);
     SHP_HIP_CHECK(hipGetLastError());
-    if (p.splits > 1) {
-        const int slots = p.row_blocks * 16 * p.row_tiles * p.row_waves, per = 1024 / head_dim;
-        const int64_t rows = (int64_t)q.n * q.group;
-        hipLaunchKernelGGL(head_dim == 64 ? cache8_join_kernel<64> : cache8_join_kernel<128>,
-                           dim3(c.n_seqs * c.kv, (unsigned)((rows + per - 1) / per)), dim3(256), 0, s,
-                           c, q, p.splits, slots, scratch);
-        SHP_HIP_CHECK(hipGetLastError());
-    }
     return SHP_OK;
 }
 
