@@ -14,6 +14,7 @@ using shp::LogprobArgs;
 typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kThreads = 1024, kHeld = 32, kChunk = kThreads * kHeld;
+constexpr int kCandidates = 512;  // logits at a row's threshold that are put in order by counting
 constexpr float kLog2e = 1.4426950408889634f;
 
 // A float as an unsigned number of the same order: NaN lowest, both zeros alike.
@@ -27,9 +28,22 @@ __device__ __forceinline__ unsigned long long rank_of(float x, int id) {
     return ((unsigned long long)order_of(x) << 32) | (unsigned)(0x7fffffff - id);
 }
 
+// The id in a rank that was raised by one (0: nothing).
+__device__ __forceinline__ int id_of(unsigned long long r) {
+    return 0x7fffffff - (int)(unsigned)(r - 1);
+}
+
 struct Sums {
     float m, z, x;
 };
+
+// Adds a part to sums whose maximum is t.m already.
+__device__ __forceinline__ void add_part(Sums& t, float m, float z, float x) {
+    if (z == 0.0f) return;  // nothing but minus infinity
+    const float d = m - t.m, f = __builtin_amdgcn_exp2f(d * kLog2e);
+    t.z += z * f;
+    t.x += (x + d * z) * f;
+}
 
 __device__ __forceinline__ float lp_of(float x, const Sums& t) {
     // no sum at all: nothing but minus infinity
@@ -64,6 +78,10 @@ struct Part {
 __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a, int chunks, Part* parts) {
     __shared__ float red[3][16];
     __shared__ unsigned long long best[2][16];
+    __shared__ unsigned bests[kThreads];
+    __shared__ unsigned long long candidates[kCandidates];
+    __shared__ float threshold;
+    __shared__ int found;
     const int row = blockIdx.x / chunks, chunk = blockIdx.x - row * chunks;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const float* x = a.logits + row * a.row_stride;
@@ -81,15 +99,13 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a, int c
             for (int c = 0; c < 4; ++c) v[4 * p + c] = i + c < end ? x[i + c] : -__builtin_inff();
         }
     }
-    float m = -__builtin_inff();
+    // each wavefront's own maximum and sums, then everybody joins the sixteen
+    float mine = -__builtin_inff();  // the thread's best
 #pragma unroll
-    for (int e = 0; e < kHeld; ++e) m = fmaxf(m, v[e]);
+    for (int e = 0; e < kHeld; ++e) mine = fmaxf(mine, v[e]);
+    float m = mine;
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    if (lane == 0) red[0][wave] = m;
-    __syncthreads();
-    m = red[0][0];
-    for (int w = 1; w < 16; ++w) m = fmaxf(m, red[0][w]);
     const float at = m == -__builtin_inff() ? 0.0f : m;
     float z = 0.0f, s = 0.0f;
 #pragma unroll
@@ -104,30 +120,101 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a, int c
         s += __shfl_xor(s, o);
     }
     if (lane == 0) {
+        red[0][wave] = m;
         red[1][wave] = z;
         red[2][wave] = s;
     }
+    const bool any = i0 + tid * 4 < end;  // the thread holds a logit
+    bests[tid] = any ? order_of(mine) : 0;
+    if (tid == 0) found = 0;
     __syncthreads();
-    z = red[1][0];
-    s = red[2][0];
-    for (int w = 1; w < 16; ++w) {
-        z += red[1][w];
-        s += red[2][w];
-    }
-    const Sums t = {m, z, s};
+    Sums t = {-__builtin_inff(), 0.0f, 0.0f};
+#pragma unroll
+    for (int w = 0; w < 16; ++w) t.m = fmaxf(t.m, red[0][w]);
+#pragma unroll
+    for (int w = 0; w < 16; ++w) add_part(t, red[0][w], red[1][w], red[2][w]);
     Part* part = parts + blockIdx.x;
     if (tid == 0) {
         if (chunks == 1) finish(a, row, t);
         else {
-            part->m = m;
-            part->z = z;
-            part->x = s;
+            part->m = t.m;
+            part->z = t.z;
+            part->x = t.x;
         }
     }
     if (!a.top) return;
-    // the best of what each thread holds; whoever gives the best of all looks for its next
+    const bool one = chunks == 1;
+    auto put = [&](int k, unsigned long long r) {
+        if (!one) {
+            part->rank[k] = r;
+        } else if (r) {
+            const int id = id_of(r);
+            a.top_ids[(int64_t)row * a.top + k] = id;
+            a.top_logprobs[(int64_t)row * a.top + k] = lp_of(x[id], t);
+        }
+    };
+
+    // A threshold that `top` threads reach with the best they hold, so that `top` logits or more do:
+    // one wavefront halves the range of the threads' best until no more than twice as many pass.
+    if (tid < 64) {
+        unsigned b[kThreads / 64], lo = ~0u, hi = 0;
+#pragma unroll
+        for (int i = 0; i < kThreads / 64; ++i) {
+            b[i] = bests[i * 64 + tid];
+            lo = min(lo, b[i]);
+            hi = max(hi, b[i]);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            lo = min(lo, (unsigned)__shfl_xor((int)lo, o));
+            hi = max(hi, (unsigned)__shfl_xor((int)hi, o));
+        }
+        for (int turn = 0; turn < 24 && hi - lo > 1; ++turn) {
+            const unsigned next = lo + (hi - lo) / 2;
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < kThreads / 64; ++i) n += __popcll(__ballot(b[i] >= next));
+            if (n < a.top) {
+                hi = next;
+            } else {
+                lo = next;
+                if (n <= 2 * a.top) break;
+            }
+        }
+        // as a float of that order; lo 0: some threads hold nothing, and the others all they have
+        if (tid == 0) threshold = lo & 0x80000000u ? __uint_as_float(lo ^ 0x80000000u)
+                                  : lo            ? __uint_as_float(~lo) : -__builtin_inff();
+    }
+    __syncthreads();
+    const float least = threshold;
+    if (any && mine >= least) {
+#pragma unroll
+        for (int e = 0; e < kHeld; ++e) {
+            const int id = i0 + ((e >> 2) * kThreads + tid) * 4 + (e & 3);
+            if (id < end && v[e] >= least) {
+                const int c = atomicAdd(&found, 1);
+                if (c < kCandidates) candidates[c] = rank_of(v[e], id) + 1;
+            }
+        }
+    }
+    __syncthreads();
+    const int n = found;
+    if (n <= kCandidates && n >= min(a.top, end - i0)) {
+        // a candidate's place is how many are better; their order in LDS does not matter
+        for (int i = tid; i < n; i += kThreads) {
+            const unsigned long long r = candidates[i];
+            int better = 0;
+            for (int j = 0; j < n; ++j) better += candidates[j] > r;
+            if (better < a.top) put(better, r);
+        }
+        for (int k = n + tid; k < a.top; k += kThreads) put(k, 0);  // a chunk of few logits
+        return;
+    }
+
+    // Too many logits about as large as the best (ties, or a few threads that hold them all), or too
+    // few that are numbers: the best of what each thread holds, and whoever gives the best of all looks for its next.
     unsigned taken = 0;
-    auto mine = [&]() {
+    auto next_best = [&]() {
         unsigned long long r = 0;
 #pragma unroll
         for (int e = 0; e < kHeld; ++e) {
@@ -137,58 +224,69 @@ __global__ __launch_bounds__(kThreads) void logprobs_kernel(LogprobArgs a, int c
         }
         return r;
     };
-    unsigned long long own = mine();
+    unsigned long long own = next_best();
     for (int k = 0; k < a.top; ++k) {
         const unsigned long long w = wave_max(own);
         if (lane == 0) best[k & 1][wave] = w;
         __syncthreads();
         unsigned long long r = best[k & 1][0];
         for (int q = 1; q < 16; ++q) r = best[k & 1][q] > r ? best[k & 1][q] : r;
-        const int id = 0x7fffffff - (int)(unsigned)(r - 1);
         if (r && own == r) {
-            const int o = id - i0;
+            const int o = id_of(r) - i0;
             taken |= 1u << ((o >> 2) / kThreads * 4 + (o & 3));
-            own = mine();
+            own = next_best();
         }
-        if (tid == 0) {
-            if (chunks > 1) part->rank[k] = r;
-            else {
-                a.top_ids[(int64_t)row * a.top + k] = id;
-                a.top_logprobs[(int64_t)row * a.top + k] = lp_of(x[id], t);
-            }
-        }
+        if (tid == 0) put(k, r);
     }
 }
 
-// Joins a row's parts: one wavefront.
-__global__ __launch_bounds__(64) void logprobs_join_kernel(LogprobArgs a, int chunks,
-                                                           const Part* parts) {
-    const int row = blockIdx.x, lane = threadIdx.x;
+// Joins a row's parts.  The best of each part come in order, so the merged ones are found by place:
+// how many of all are better.  With more of them than fit LDS, one after the other.
+constexpr int kJoin = 256, kJoinHeld = 2048;
+__global__ __launch_bounds__(kJoin) void logprobs_join_kernel(LogprobArgs a, int chunks,
+                                                              const Part* parts) {
+    __shared__ unsigned long long held[kJoinHeld];
+    __shared__ unsigned long long best[kJoin / 64];
+    const int row = blockIdx.x, tid = threadIdx.x;
     const Part* part = parts + (int64_t)row * chunks;
+    const int n = chunks * a.top;
+    const bool fits = n <= kJoinHeld;
+    if (fits)
+        for (int i = tid; i < n; i += kJoin) held[i] = part[i / a.top].rank[i % a.top];
     Sums t = {-__builtin_inff(), 0.0f, 0.0f};
     for (int c = 0; c < chunks; ++c) t.m = fmaxf(t.m, part[c].m);
-    for (int c = 0; c < chunks; ++c) {
-        const float z = part[c].z;
-        if (z == 0.0f) continue;
-        const float d = part[c].m - t.m, f = __builtin_amdgcn_exp2f(d * kLog2e);
-        t.z += z * f;
-        t.x += (part[c].x + d * z) * f;
+    for (int c = 0; c < chunks; ++c) add_part(t, part[c].m, part[c].z, part[c].x);
+    if (tid == 0) finish(a, row, t);
+    auto put = [&](int k, unsigned long long r) {
+        const int id = id_of(r);
+        a.top_ids[(int64_t)row * a.top + k] = id;
+        a.top_logprobs[(int64_t)row * a.top + k] = lp_of(a.logits[row * a.row_stride + id], t);
+    };
+    if (fits) {
+        __syncthreads();
+        for (int i = tid; i < n; i += kJoin) {
+            const unsigned long long r = held[i];
+            if (!r) continue;
+            int better = 0;
+            for (int j = 0; j < n && better < a.top; ++j) better += held[j] > r;
+            if (better < a.top) put(better, r);
+        }
+        return;
     }
-    if (lane == 0) finish(a, row, t);
-    const int n = chunks * a.top;
     unsigned long long above = ~0ull;
     for (int k = 0; k < a.top; ++k) {
         unsigned long long r = 0;
-        for (int i = lane; i < n; i += 64) {
+        for (int i = tid; i < n; i += kJoin) {
             const unsigned long long q = part[i / a.top].rank[i % a.top];
             if (q < above && q > r) r = q;
         }
-        above = wave_max(r);
-        if (lane == 0) {
-            const int id = 0x7fffffff - (int)(unsigned)(above - 1);
-            a.top_ids[(int64_t)row * a.top + k] = id;
-            a.top_logprobs[(int64_t)row * a.top + k] = lp_of(a.logits[row * a.row_stride + id], t);
-        }
+        r = wave_max(r);
+        if ((tid & 63) == 0) best[tid >> 6] = r;
+        __syncthreads();
+        above = best[0];
+        for (int w = 1; w < kJoin / 64; ++w) above = best[w] > above ? best[w] : above;
+        if (tid == 0) put(k, above);
+        __syncthreads();
     }
 }
 
@@ -210,7 +308,7 @@ int logprobs_launch(hipStream_t s, const LogprobArgs& a, float* scratch) {
     hipLaunchKernelGGL(logprobs_kernel, dim3(a.rows * c), dim3(kThreads), 0, s, a, c, parts);
     SHP_HIP_CHECK(hipGetLastError());
     if (c > 1) {
-        hipLaunchKernelGGL(logprobs_join_kernel, dim3(a.rows), dim3(64), 0, s, a, c, parts);
+        hipLaunchKernelGGL(logprobs_join_kernel, dim3(a.rows), dim3(kJoin), 0, s, a, c, parts);
         SHP_HIP_CHECK(hipGetLastError());
     }
     return SHP_OK;
