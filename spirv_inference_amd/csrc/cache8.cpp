@@ -220,7 +220,7 @@ int shp_token_logprobs(shp_ctx* ctx, const shp_logprobs_args* a) {
     const shp::LogprobArgs l = {a->logits, a->row_stride, a->rows, a->vocab, a->n_top, a->targets,
                                 a->logprob, a->entropy, a->top_ids, a->top_logprobs};
     float* scratch = nullptr;
-    const size_t need = shp::logprobs_scratch(a->rows, a->vocab, a->n_top);
+    const size_t need = shp::logprobs_scratch(a->rows, a->vocab);
     if (need) {
         int rc = x->scratch(need, &scratch);
         if (rc) return rc;

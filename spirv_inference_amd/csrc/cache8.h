@@ -83,8 +83,8 @@ struct LogprobArgs {
     float* top_logprobs;
 };
 constexpr int kMaxTop = 64;  // alternatives a row can ask for
-// Floats of scratch the rows' parts need (0: one workgroup takes a whole row).
-size_t logprobs_scratch(int rows, int vocab, int top);
+// Floats of scratch the rows' parts need (0: a workgroup takes a whole row).
+size_t logprobs_scratch(int rows, int vocab);
 int logprobs_launch(hipStream_t s, const LogprobArgs& a, float* scratch);
 
 }  // namespace shp

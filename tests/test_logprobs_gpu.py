@@ -48,7 +48,7 @@ def check(got, x, targets, top):
 @pytest.mark.parametrize("rows,vocab,top", [
     (1, 1, 1), (1, 1, 0), (3, 2, 2), (5, 63, 5), (2, 64, 64), (7, 65, 64), (4, 1000, 20),
     (3, 4097, 1), (2, 32000, 5), (1, 32768, 64), (2, 32769, 64), (3, 100003, 33), (1, 300000, 20),
-    (600, 777, 3)])
+    (600, 777, 3), (256, 8192, 20), (257, 8193, 64), (255, 33000, 5), (300, 30001, 20)])
 @pytest.mark.parametrize("std", [0.1, 4.0])
 def test_logprobs(ctx, rows, vocab, top, std):
     rng = np.random.default_rng(vocab)
@@ -66,6 +66,26 @@ def test_ties_go_to_the_lowest_id(ctx, vocab, kind):
          "descending": np.tile(np.arange(vocab)[::-1] * 1e-3, (2, 1)),
          "zeros": rng.choice([0.0, -0.0], (2, vocab))}[kind].astype(np.float32)
     check(run(ctx, x, [0, vocab - 1], 64), x, [0, vocab - 1], 64)
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 40000), (300, 20000)])
+def test_plateaus_and_chunks_of_one_kind(ctx, rows, vocab):
+    """Rows in which the best lie in one place, rise, tie, or are all that is allowed: the ways in
+    which a row's candidates can be too many or too few."""
+    rng = np.random.default_rng(12)
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    kinds = [lambda r: np.sort(r), lambda r: np.sort(r)[::-1], lambda r: np.round(r),
+             lambda r: np.where(np.arange(vocab) % 977 == 5, r, -np.inf),
+             lambda r: np.where(np.arange(vocab) < 3, r, -np.inf),
+             lambda r: np.where(np.arange(vocab) > vocab - 40, r, np.nan),
+             lambda r: np.where((np.arange(vocab) >= 9000) & (np.arange(vocab) < 9600), 50 + r, r),
+             lambda r: np.where(np.arange(vocab) // 4 % 256 == 7, 50 + r, r),
+             lambda r: np.minimum(r, 0.5)]
+    for i in range(rows):
+        x[i] = kinds[i % len(kinds)](x[i])
+    t = rng.integers(0, vocab, rows)
+    for top in (1, 20, 64):
+        check(run(ctx, x, t, top), x, t, top)
 
 
 @pytest.mark.parametrize("vocab", [50, 40000])
