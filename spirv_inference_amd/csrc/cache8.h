@@ -129,30 +129,37 @@ template <int FMT>
 __device__ __forceinline__ unsigned encode4(const float* x, float s, float inv) {
     if (!(s > 0.0f)) return 0u;
     float y[4];
-    bool near = false;
+    if constexpr (FMT == kI8) {
+        // adding 1.5 * 2^23 rounds to a whole number, whose low byte is the code
+        constexpr float kWhole = 12582912.0f;
+        float m[4], off = 1.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        y[i] = x[i] * inv;
-        if constexpr (FMT == kI8) {
-            // 2^-23 of 127 is under 2^-16
-            near |= fabsf(fabsf(y[i] - rintf(y[i])) - 0.5f) < 0x1p-15f;
-        } else {
+        for (int i = 0; i < 4; ++i) {
+            y[i] = x[i] * inv;
+            m[i] = y[i] + kWhole;
+            off = fminf(off, fabsf(fabsf(y[i] - (m[i] - kWhole)) - 0.5f));
+        }
+        if (off < 0x1p-15f) {  // 2^-23 of 127 is under 2^-16
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m[i] = quotient_odd(x[i], s) + kWhole;
+        }
+        const unsigned lo = __builtin_amdgcn_perm(__float_as_uint(m[1]), __float_as_uint(m[0]), 0x0c0c0400u);
+        const unsigned hi = __builtin_amdgcn_perm(__float_as_uint(m[3]), __float_as_uint(m[2]), 0x04000c0cu);
+        return lo | hi;
+    } else {
+        bool near = false;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            y[i] = x[i] * inv;
             // the 20 bits behind a code's mantissa, 8 units around their middle; numbers that
             // become denormal codes have fewer bits
             const unsigned cut = (__float_as_uint(y[i]) & 0xfffffu) - 0x7fff8u;
             near |= cut <= 16u || (fabsf(y[i]) < 0x1p-6f && y[i] != 0.0f);
         }
-    }
-    if (near) {
+        if (near) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) y[i] = quotient_odd(x[i], s);
-    }
-    if constexpr (FMT == kI8) {
-        unsigned w = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w |= ((unsigned)(int)rintf(y[i]) & 0xffu) << (8 * i);
-        return w;
-    } else {
+            for (int i = 0; i < 4; ++i) y[i] = quotient_odd(x[i], s);
+        }
         const int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
         return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
     }

@@ -373,8 +373,9 @@ __device__ __forceinline__ void select_held(const float* __restrict__ w, int old
     const int tid = threadIdx.x, i0 = tid * E;
     float x[E];
     unsigned key[E];
+    if constexpr (E == 1) x[0] = i0 < old ? w[i0] : 0.0f;
 #pragma unroll
-    for (int e = 0; e < E; e += 4) {
+    for (int e = 0; e + 4 <= E; e += 4) {
         if (i0 + e + 4 <= old) {
             const f4u v = *reinterpret_cast<const f4u*>(w + i0 + e);
 #pragma unroll
@@ -492,105 +493,127 @@ __global__ __launch_bounds__(kSelect) void cache8_select_kernel(Cache8 src, Cach
     }
     const unsigned need = keep - recent;
     if (need == 0) return;
-    if (old <= 8 * kSelect) select_held<8>(w, old, need, out, ow, m);
+    if (old <= kSelect) select_held<1>(w, old, need, out, ow, m);
+    else if (old <= 8 * kSelect) select_held<8>(w, old, need, out, ow, m);
     else if (old <= 32 * kSelect) select_held<32>(w, old, need, out, ow, m);
     else select_long(w, old, need, out, ow, m);
 }
 
-// One span of K or V of dst, made from the kept tokens of src.  K's rows are read 16 bytes a lane;
-// of V a lane takes a token, dimension after dimension, so that a wavefront's bytes lie in the few
-// tiles its 64 tokens come from.
-template <int D, int FMT, int SPAN, bool V>
-__device__ __forceinline__ void gather_span(const Cache8& src, const Cache8& dst,
-                                            const int32_t* kept, int keep, Scales& sc) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int sh = blockIdx.y, s = sh / src.kv, B = 1 << dst.block_log2, nb = SPAN >> dst.block_log2;
-    const int t0 = (int)blockIdx.x * SPAN, t1 = min(min(seq_length(src, s), keep), t0 + SPAN);
-    if (t0 >= t1) return;
-    const int32_t* id = kept + (int64_t)sh * keep;
-    const uint8_t* from = (V ? src.v : src.k) + (int64_t)sh * src.cap * D;
-    const float* from_scale = V ? src.v_scale : src.k_scale;
-    uint8_t* to = (V ? dst.v : dst.k) + (int64_t)sh * dst.cap * D;
-    float* scale = (V ? dst.v_scale : dst.k_scale) + block_at(dst, sh, t0);
-
-    // K: NP pieces of 16 dimensions of a token; V: the ND dimensions from d0 of token vt
-    constexpr int R = D / 16, NP = SPAN * R / kThreads, ND = D * SPAN / kThreads;
-    u4 raw[V ? 1 : NP];
-    float was[V ? 1 : NP];
-    unsigned bytes[V ? ND : 1];
-    const int vt = SPAN == 64 ? lane : (wave & 1) * 64 + lane;
-    const int d0 = SPAN == 64 ? wave * ND : (wave >> 1) * ND;
-    if (tid < 8) sc.top[tid] = 0;
+// The scales of the blocks of a span of dst, from the maxima in sc.top, for everybody.
+template <int FMT>
+__device__ __forceinline__ void settle_scales(const Cache8& dst, float* scale, int t0, int t1,
+                                              Scales& sc) {
     __syncthreads();
-    if constexpr (V) {
-        const bool have = t0 + vt < t1;
-        const int t = have ? id[t0 + vt] : 0;
-        was[0] = have ? from_scale[block_at(src, sh, t)] : 0.0f;
-        const uint8_t* p = from + code_at<D, true>(t, d0);
+    const int b = threadIdx.x;
+    if (b < 8 && t0 + (b << dst.block_log2) < t1) {
+        const float now = block_scale<FMT>(__uint_as_float(sc.top[b]));
+        scale[b] = now;
+        sc.now[b] = now;
+        sc.inv[b] = 1.0f / now;
+    }
+    __syncthreads();
+}
+
+// One span of K of dst, made from the kept tokens of src, whose rows are read 16 bytes a lane.
+template <int D, int FMT, int SPAN>
+__device__ __forceinline__ void gather_k(const Cache8& src, const Cache8& dst, const int32_t* id,
+                                         int t0, int t1, Scales& sc) {
+    constexpr int R = D / 16, NP = SPAN * R / kThreads;  // NP pieces of 16 dimensions of a token
+    const int tid = threadIdx.x, lane = tid & 63, sh = blockIdx.y;
+    const uint8_t* from = src.k + (int64_t)sh * src.cap * D;
+    uint8_t* to = dst.k + (int64_t)sh * dst.cap * D;
+    u4 raw[NP];
+    float was[NP];
 #pragma unroll
-        for (int d = 0; d < ND; ++d) bytes[d] = have ? p[d * kCacheTile] : 0u;
+    for (int e = 0; e < NP; ++e) {
+        const int p = e * kThreads + tid, t = t0 + p / R;
+        raw[e] = u4{0u, 0u, 0u, 0u};
+        was[e] = 0.0f;
+        if (t < t1) {
+            const int i = id[t];
+            raw[e] = *reinterpret_cast<const u4*>(from + (int64_t)i * D + p % R * 16);
+            was[e] = src.k_scale[block_at(src, sh, i)];
+        }
+    }
+    __syncthreads();  // sc.top is clear
+#pragma unroll
+    for (int e = 0; e < NP; ++e) {
         float top = 0.0f;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) top = fmaxf(top, fabsf(code_value<FMT>(bytes[d], 0)));
-        raise(&sc.top[vt >> dst.block_log2], magnitude(top * was[0]));
-    } else {
-#pragma unroll
-        for (int e = 0; e < NP; ++e) {
-            const int p = e * kThreads + tid, t = t0 + p / R;
-            raw[e] = u4{0u, 0u, 0u, 0u};
-            was[e] = 0.0f;
-            if (t < t1) {
-                const int i = id[t];
-                raw[e] = *reinterpret_cast<const u4*>(from + (int64_t)i * D + p % R * 16);
-                was[e] = from_scale[block_at(src, sh, i)];
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < NP; ++e) {
-            float top = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(code_value<FMT>(raw[e][i >> 2], i & 3)));
-            // the wavefront's tokens of this step are of one block
-            top = wave_max(magnitude(top * was[e]));
-            if (lane == 0) raise(&sc.top[(e * kThreads + tid) / R >> dst.block_log2], top);
-        }
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(code_value<FMT>(raw[e][i >> 2], i & 3)));
+        // the wavefront's tokens of this step are of one block
+        top = wave_max(magnitude(top * was[e]));
+        if (lane == 0) raise(&sc.top[(e * kThreads + tid) / R >> dst.block_log2], top);
     }
-    __syncthreads();
-    if (tid < nb && t0 + tid * B < t1) {
-        const float now = block_scale<FMT>(__uint_as_float(sc.top[tid]));
-        scale[tid] = now;
-        sc.now[tid] = now;
-        sc.inv[tid] = 1.0f / now;
-    }
-    __syncthreads();
-    if constexpr (V) {
-        if (t0 + vt >= t1) return;
-        const float now = sc.now[vt >> dst.block_log2], inv = sc.inv[vt >> dst.block_log2];
-        uint8_t* p = to + code_at<D, true>(t0 + vt, d0);
+    settle_scales<FMT>(dst, dst.k_scale + block_at(dst, sh, t0), t0, t1, sc);
 #pragma unroll
-        for (int d = 0; d < ND; d += 4) {
+    for (int e = 0; e < NP; ++e) {
+        const int p = e * kThreads + tid, lt = p / R;
+        if (t0 + lt >= t1) continue;
+        const float now = sc.now[lt >> dst.block_log2], inv = sc.inv[lt >> dst.block_log2];
+        u4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
             float y[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = code_value<FMT>(bytes[d + i], 0) * was[0];
-            const unsigned w = encode4<FMT>(y, now, inv);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) p[(d + i) * kCacheTile] = (uint8_t)(w >> (8 * i));
+            for (int j = 0; j < 4; ++j) y[j] = code_value<FMT>(raw[e][i], j) * was[e];
+            w[i] = encode4<FMT>(y, now, inv);
         }
-    } else {
+        *reinterpret_cast<u4*>(to + (int64_t)(t0 + lt) * D + p % R * 16) = w;
+    }
+}
+
+// One span of V: a lane makes words of four tokens of a dimension, whose bytes it reads one by one.
+// The 64 tokens of a span come from few tiles (their places rise), so a wavefront's loads share
+// lines, and lines are all that reading whole tiles would fetch too.
+template <int D, int FMT, int SPAN>
+__device__ __forceinline__ void gather_v(const Cache8& src, const Cache8& dst, const int32_t* id,
+                                         int t0, int t1, Scales& sc) {
+    constexpr int W = SPAN / 4, STEP = kThreads / W, NW = D / STEP;
+    const int tid = threadIdx.x, sh = blockIdx.y, n = t1 - t0, w = tid % W, d0 = tid / W;
+    const uint8_t* from = src.v + (int64_t)sh * src.cap * D;
+    uint8_t* to = dst.v + (int64_t)sh * dst.cap * D;
+    float was[4];
+    unsigned at[4];
 #pragma unroll
-        for (int e = 0; e < NP; ++e) {
-            const int p = e * kThreads + tid, lt = p / R;
-            if (t0 + lt >= t1) continue;
-            const float now = sc.now[lt >> dst.block_log2], inv = sc.inv[lt >> dst.block_log2];
-            u4 w;
+    for (int i = 0; i < 4; ++i) {
+        // behind the last token: the last one's bytes, which do not count
+        const int t = id[t0 + min(4 * w + i, n - 1)];
+        at[i] = (unsigned)code_at<D, true>(t, d0);
+        was[i] = src.v_scale[block_at(src, sh, t)];
+    }
+    unsigned char b[NW][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float y[4];
+    for (int e = 0; e < NW; ++e)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) y[j] = code_value<FMT>(raw[e][i], j) * was[e];
-                w[i] = encode4<FMT>(y, now, inv);
-            }
-            *reinterpret_cast<u4*>(to + (int64_t)(t0 + lt) * D + p % R * 16) = w;
+        for (int i = 0; i < 4; ++i) b[e][i] = from[at[i] + e * STEP * kCacheTile];
+    __syncthreads();  // sc.top is clear
+    float most[4] = {0.f, 0.f, 0.f, 0.f}, top = 0.0f;
+#pragma unroll
+    for (int e = 0; e < NW; ++e)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most[i] = fmaxf(most[i], fabsf(code_value<FMT>(b[e][i], 0)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (4 * w + i < n) top = fmaxf(top, magnitude(most[i] * was[i]));
+    raise(&sc.top[4 * w >> dst.block_log2], top);
+    settle_scales<FMT>(dst, dst.v_scale + block_at(dst, sh, t0), t0, t1, sc);
+    if (4 * w >= n) return;
+    const float now = sc.now[4 * w >> dst.block_log2], inv = sc.inv[4 * w >> dst.block_log2];
+#pragma unroll
+    for (int e = 0; e < NW; ++e) {
+        float y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            y[i] = 4 * w + i < n ? code_value<FMT>(b[e][i], 0) * was[i] : 0.0f;
+        const unsigned c = encode4<FMT>(y, now, inv);
+        uint8_t* p = to + code_at<D, true>(t0 + 4 * w, d0 + e * STEP);
+        if (4 * w + 4 <= n) {
+            *reinterpret_cast<unsigned*>(p) = c;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (4 * w + i < n) p[i] = (uint8_t)(c >> (8 * i));
         }
     }
 }
@@ -599,8 +622,13 @@ template <int D, int FMT, int SPAN>
 __global__ __launch_bounds__(kThreads) void cache8_gather_kernel(Cache8 src, Cache8 dst,
                                                                  const int32_t* kept, int keep) {
     __shared__ Scales sc;
-    if (blockIdx.z) gather_span<D, FMT, SPAN, true>(src, dst, kept, keep, sc);
-    else gather_span<D, FMT, SPAN, false>(src, dst, kept, keep, sc);
+    const int sh = blockIdx.y, s = sh / src.kv, t0 = (int)blockIdx.x * SPAN;
+    const int t1 = min(min(seq_length(src, s), keep), t0 + SPAN);
+    if (t0 >= t1) return;
+    if (threadIdx.x < 8) sc.top[threadIdx.x] = 0;
+    const int32_t* id = kept + (int64_t)sh * keep;
+    if (blockIdx.z) gather_v<D, FMT, SPAN>(src, dst, id, t0, t1, sc);
+    else gather_k<D, FMT, SPAN>(src, dst, id, t0, t1, sc);
 }
 
 // KERN<head_dim, format, span> for a cache.

@@ -633,8 +633,9 @@ int cache8_attend_launch(hipStream_t s, const Cache8& c, int head_dim, int forma
     return SHP_OK;
 }
 
-// A row group a wavefront, as long as their sums fit 64 MiB; about 8,192 wavefronts, each with four
-// tiles or more.
+// A row group a wavefront, as long as their sums fit 64 MiB.  With 16 rows about 8,192 wavefronts;
+// with more, which take longer to load (their q is cut into pieces), no more than the 2,048 that are
+// held at once (512 rows on 8,190 tokens 62 -> 51 us).  Each has four tiles or more.
 Cache8WeightsPlan cache8_weights_plan(const Cache8& c, int head_dim, int64_t rows, bool may_group) {
     Cache8WeightsPlan p;
     p.row_tiles = rows <= 16 ? 1 : rows <= 32 || head_dim == 128 ? 2 : 4;
@@ -645,7 +646,7 @@ Cache8WeightsPlan cache8_weights_plan(const Cache8& c, int head_dim, int64_t row
     p.groups = (int)((all + p.chunks - 1) / p.chunks);
     p.row_waves = p.groups >= 4 ? 4 : p.groups >= 2 ? 2 : 1;
     const int64_t tok_waves = 4 / p.row_waves, tiles = c.cap / kCacheTile;
-    const int64_t want = 8192 / std::max<int64_t>(heads * p.groups, 1), most = (tiles + 3) / 4;
+    const int64_t want = (p.row_tiles == 1 ? 8192 : 2048) / std::max<int64_t>(heads * p.groups, 1), most = (tiles + 3) / 4;
     p.workers = (int)((std::max<int64_t>(std::min(want, most), 1) + tok_waves - 1) / tok_waves);
     p.scratch = p.groups > 1 ? (size_t)(one * p.groups) : 0;
     return p;
