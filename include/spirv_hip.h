@@ -376,6 +376,13 @@ int shp_llama_tokens(shp_llama* lm, int32_t* out, int32_t cap, int32_t* n_out);
  * written through *n_out. */
 int shp_llama_generate(shp_llama* lm, const int32_t* prompt, int32_t n_prompt, int32_t n_new,
                        int32_t* out_tokens, int32_t* n_out);
+/* Scores a text: feeds ids[0 .. n) from position 0, as shp_llama_generate feeds a prompt, and says
+ * how likely each id was after those before it: logprob[i] of ids[i + 1] (n - 1 values), and for
+ * the distribution after ids[i] its entropy [n] and its n_top likeliest ids with their log
+ * probabilities [n][n_top], as shp_token_logprobs does (any of them may be NULL, the last two where
+ * n_top is 0).  Leaves the decoder as that prompt would: decoding can go on.  Synchronous. */
+int shp_llama_score(shp_llama* lm, const int32_t* ids, int32_t n, int32_t n_top, float* logprob,
+                    float* entropy, int32_t* top_ids, float* top_logprobs);
 int shp_llama_use_graph(shp_llama* lm, int enable);
 /* Decode engines.  All three compute the same math on the same device state, so they can be
  * switched between calls.

@@ -179,6 +179,9 @@ SIGNATURES = [
                                    C.POINTER(C.c_int32)]),
     ("shp_llama_generate", C.c_int, [C.c_void_p, C.POINTER(C.c_int32), C.c_int32, C.c_int32,
                                      C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
+    ("shp_llama_score", C.c_int, [C.c_void_p, C.POINTER(C.c_int32), C.c_int32, C.c_int32,
+                                  C.POINTER(C.c_float), C.POINTER(C.c_float),
+                                  C.POINTER(C.c_int32), C.POINTER(C.c_float)]),
     ("shp_llama_use_graph", C.c_int, [C.c_void_p, C.c_int]),
     ("shp_llama_set_engine", C.c_int, [C.c_void_p, C.c_int]),
     ("shp_llama_set_wait_limit", C.c_int, [C.c_void_p, C.c_int64]),

@@ -15,6 +15,7 @@
 #include <vector>
 
 #include "attention.h"
+#include "cache8.h"
 #include "decode.h"
 #include "gemm.h"
 #include "prefill.h"
@@ -260,6 +261,36 @@ struct Llama {
     float *pf_sum = nullptr;     // product results or K-split partials
     float *pf_act = nullptr, *pf_logits = nullptr;
 
+    // ---- scoring: what the distributions after each id of a text say (device, [max_seq]) -------
+    struct Score {
+        int32_t *targets = nullptr, *top_ids = nullptr;  // top_ids, top [max_seq][kMaxTop]
+        float *logprob = nullptr, *entropy = nullptr, *top = nullptr;
+        int n_top = -1;  // alternatives of the call at hand; -1: none is
+    } score;
+
+    int setup_score() {
+        if (score.top) return SHP_OK;
+        const uint64_t n = cfg.max_seq;
+        int rc = alloc((float**)&score.targets, n);
+        if (!rc) rc = alloc(&score.logprob, n);
+        if (!rc) rc = alloc(&score.entropy, n);
+        if (!rc) rc = alloc((float**)&score.top_ids, n * kMaxTop);
+        if (!rc) rc = alloc(&score.top, n * kMaxTop);
+        return rc;
+    }
+
+    // The logits of the positions pos .. pos + rows - 1.
+    int score_rows(const float* x, int rows, int pos) {
+        const LogprobArgs a = {x, cfg.vocab, rows, cfg.vocab, score.n_top, score.targets + pos,
+                               score.logprob + pos, score.entropy + pos,
+                               score.top_ids + (int64_t)pos * score.n_top,
+                               score.top + (int64_t)pos * score.n_top};
+        float* scratch = nullptr;
+        const size_t need = logprobs_scratch(rows, cfg.vocab);
+        int rc = need ? ctx->scratch(need, &scratch) : SHP_OK;
+        return rc ? rc : logprobs_launch(ctx->stream, a, scratch);
+    }
+
     GemmParams product(int rows, const float* a, const float* w, int N, int K, float* c,
                        const float* residual) const {
         GemmParams p;
@@ -380,6 +411,7 @@ struct Llama {
                 rc = prefill_argmax_launch(s, pf_logits, m, cfg.vocab, st->out_tokens + host_pos + r,
                                            r + m == n ? logits : nullptr, &st->token, &st->pos,
                                            &st->step, host_pos + n);
+            if (!rc && score.n_top >= 0) rc = score_rows(pf_logits, m, host_pos + r);
         }
         if (!rc) host_pos += n;
         return rc;
@@ -577,6 +609,53 @@ int shp_llama_generate(shp_llama* p, const int32_t* prompt, int32_t n_prompt, in
         ++w;
     }
     *n_out = w;
+    return SHP_OK;
+}
+
+int shp_llama_score(shp_llama* p, const int32_t* ids, int32_t n, int32_t n_top, float* logprob,
+                    float* entropy, int32_t* top_ids, float* top_logprobs) {
+    if (!p || !ids || n <= 0 || (n_top && (!top_ids || !top_logprobs)))
+        return fail(SHP_ERR_INVALID, "shp_llama_score: bad arguments");
+    Llama* lm = reinterpret_cast<Llama*>(p);
+    {
+        int grc = shp::refuse_while_capturing(lm->ctx->stream, "shp_llama_score");
+        if (grc) return grc;
+    }
+    if (n_top < 0 || n_top > shp::kMaxTop || n_top > lm->cfg.vocab)
+        return fail(SHP_ERR_SHAPE, "shp_llama_score: n_top must be 0 to 64 and at most the vocabulary");
+    if (n > lm->cfg.max_seq) return fail(SHP_ERR_SHAPE, "shp_llama_score: text exceeds max_seq");
+    for (int i = 0; i < n; ++i)
+        if (ids[i] < 0 || ids[i] >= lm->cfg.vocab)
+            return fail(SHP_ERR_SHAPE, "shp_llama_score: token id");
+    SHP_HIP_CHECK(hipSetDevice(lm->ctx->device));
+    hipStream_t s = lm->ctx->stream;
+    int rc = lm->setup_score();
+    if (!rc) rc = lm->reset();
+    if (rc) return rc;
+    std::vector<int32_t> next(ids + 1, ids + n);
+    next.push_back(-1);  // nothing is known to follow the last id
+    SHP_HIP_CHECK(hipMemcpyAsync(lm->score.targets, next.data(), n * sizeof(int32_t),
+                                 hipMemcpyHostToDevice, s));
+    SHP_HIP_CHECK(hipStreamSynchronize(s));
+    lm->score.n_top = n_top;
+    if (n > 2 && lm->pf_rows) {  // as shp_llama_generate feeds a prompt
+        rc = lm->prefill(ids, n);
+    } else {
+        for (int i = 0; i < n && !rc; ++i) {
+            rc = shp_llama_step(p, ids[i]);
+            if (!rc) rc = lm->score_rows(lm->logits, 1, i);
+        }
+    }
+    lm->score.n_top = -1;
+    if (rc) return rc;
+    auto fetch = [&](void* dst, const void* src, size_t count) {
+        return dst && count ? hipMemcpyAsync(dst, src, count * 4, hipMemcpyDeviceToHost, s) : hipSuccess;
+    };
+    SHP_HIP_CHECK(fetch(logprob, lm->score.logprob, n - 1));
+    SHP_HIP_CHECK(fetch(entropy, lm->score.entropy, n));
+    SHP_HIP_CHECK(fetch(top_ids, lm->score.top_ids, (size_t)n * n_top));
+    SHP_HIP_CHECK(fetch(top_logprobs, lm->score.top, (size_t)n * n_top));
+    SHP_HIP_CHECK(hipStreamSynchronize(s));
     return SHP_OK;
 }
 

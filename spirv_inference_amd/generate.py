@@ -11,7 +11,8 @@ so the token ids are only meaningful for parity and timing.
 prints the generated ids and the decode time per token of each repetition.  Real weights
 supplied locally replace the seeded ones: `--reference-fixture DIR` (export_llama.py's
 raw-f32 parameter files) or `--safetensors FILE` (a Hugging Face checkpoint).  With
-`--profile-phases N` it also decodes N tokens in one persistent launch with the in-kernel phase
+`--score` it also says how likely the prompt's ids are: their mean log probability, and for the
+last position the entropy and the `--top` likeliest ids.  With `--profile-phases N` it also decodes N tokens in one persistent launch with the in-kernel phase
 stamps on and prints, for the last of them, the time each workgroup spends in the phases of a
 layer and at the grid barriers between them (means over workgroups, summed over layers).
 """
@@ -76,6 +77,9 @@ def main() -> int:
                     help="load export_llama.py raw-f32 parameters from DIR")
     ap.add_argument("--safetensors", metavar="FILE", nargs="+",
                     help="load a Hugging Face safetensors checkpoint (one file or shards)")
+    ap.add_argument("--score", action="store_true",
+                    help="also print the log probability of the prompt's ids")
+    ap.add_argument("--top", type=int, default=5, help="with --score: alternatives to print")
     ap.add_argument("--profile-phases", type=int, default=0, metavar="N",
                     help="after the timed runs, stamp-profile N tokens of the persistent engine")
     ap.add_argument("--copy-calibration-mb", type=int, default=0, metavar="MB",
@@ -106,6 +110,13 @@ def main() -> int:
             dt = time.perf_counter() - t0
             toks = lm.tokens()[len(prompt) - 1:len(prompt) - 1 + args.tokens]
             print(f"{dt / args.tokens * 1e3:.3f} ms/token  tokens {toks}", flush=True)
+        if args.score:
+            lp, ent, top, tlp = lm.score(prompt, args.top)
+            if len(lp):
+                print(f"prompt log probability {lp.sum():.4f}, mean {lp.mean():.4f} "
+                      f"(perplexity {np.exp(-lp.mean()):.2f})", flush=True)
+            print(f"after it: entropy {ent[-1]:.4f}, likeliest "
+                  + ", ".join(f"{t} {p:.4f}" for t, p in zip(top[-1], tlp[-1])), flush=True)
         if args.profile_phases > 0:
             lm.reset()
             for t in prompt:

@@ -185,6 +185,23 @@ class Llama:
               "shp_llama_generate")
         return list(out[:n.value])
 
+    def score(self, ids, n_top: int = 0):
+        """How likely each id is after those before it (shp_llama_score): log probabilities of
+        ids[1:], and of the distribution after each id the entropy, the n_top likeliest ids and
+        their log probabilities.  Decoding can go on from there."""
+        n = len(ids)
+        p = (C.c_int32 * n)(*[int(t) for t in ids])
+        lp, ent = np.empty(max(n - 1, 0), np.float32), np.empty(n, np.float32)
+        k = max(int(n_top), 0)
+        top, tlp = np.empty((n, k), np.int32), np.empty((n, k), np.float32)
+
+        def at(a, t):
+            return a.ctypes.data_as(C.POINTER(t))
+        check(lib().shp_llama_score(self.handle, p, n, int(n_top), at(lp, C.c_float),
+                                    at(ent, C.c_float), at(top, C.c_int32), at(tlp, C.c_float)),
+              "shp_llama_score")
+        return lp, ent, top, tlp
+
     def logits(self) -> np.ndarray:
         p, n = C.c_void_p(), C.c_uint64()
         check(lib().shp_llama_logits(self.handle, C.byref(p), C.byref(n)), "shp_llama_logits")

@@ -7,7 +7,9 @@ import numpy as np
 import pytest
 
 import cache8_ref as R
+from conftest import assert_close
 from spirv_inference_amd import Context, DeviceTensor, ShpError
+from spirv_inference_amd.models import Llama
 
 pytestmark = pytest.mark.gpu
 
@@ -185,3 +187,50 @@ def test_captured_calls(ctx):
             check((lp.download(), ent.download(), ids.download().reshape(rows, top),
                    tops.download().reshape(rows, top)), v, [3, 4], top)
         g.destroy()
+
+
+# ---- the decoder scores a text -----------------------------------------------------------------
+
+SMALL = dict(n_layers=2, hidden=256, n_heads=4, n_kv_heads=2, head_dim=64, ffn=512, vocab=1000,
+             max_seq=200)
+
+
+@pytest.mark.parametrize("engine", ["persistent", "graph", "kernels"])
+@pytest.mark.parametrize("n,top", [(1, 3), (2, 0), (3, 64), (40, 5), (150, 1)])
+def test_scores_are_those_of_the_token_steps(ctx, engine, n, top):
+    """The prompt pass adds up its products in another order than the token steps, so the two are
+    held to each other by the gate of the decoder's own tests (1e-4 + 1e-4 of the value)."""
+    ids = [int(t) for t in np.random.default_rng(n).integers(3, SMALL["vocab"], n)]
+    with Llama(ctx, seed=5, **SMALL) as lm:
+        lm.set_engine(engine)
+        lp, ent, tid, tlp = lm.score(ids, top)
+        on = lm.decode(4) or lm.tokens()[n - 1:n + 4]
+        lm.reset()
+        x = []
+        for t in ids:
+            lm.step(t)
+            ctx.sync()
+            x.append(lm.logits())
+        lm.decode(4)
+        assert lm.tokens()[n - 1:n + 4] == on
+    x = np.array(x)
+    want = R.logprobs(x, ids[1:] + [0], 0)
+    assert lp.shape == (n - 1,) and tid.shape == tlp.shape == (n, top)
+    assert_close(lp, want[0][:-1], what="logprob")
+    assert_close(ent, want[1], what="entropy")
+    full = x.astype(np.float64) - x.max(1, keepdims=True)
+    full -= np.log(np.exp(full).sum(1, keepdims=True))
+    for i in range(n):
+        assert_close(tlp[i], full[i, tid[i]], what="top")
+        assert len(set(tid[i])) == top and (np.diff(tlp[i]) <= 0).all()
+        if top:
+            rest = np.delete(full[i], tid[i]).max()
+            assert rest <= tlp[i, -1] + 1e-4 + 1e-4 * abs(rest)
+
+
+def test_scores_refuse_bad_texts(ctx):
+    with Llama(ctx, seed=5, **SMALL) as lm:
+        for ids, top in (([], 0), ([3, 1000], 0), ([3, -1], 0), ([3] * 201, 0), ([3], 65), ([3], -1)):
+            with pytest.raises(ShpError, match="shp_llama_score"):
+                lm.score(ids, top)
+        lm.score([3] * 200, 1)
