@@ -168,7 +168,10 @@ int shp_run_kernel(shp_ctx* ctx, const char* kernel, const float* in0, size_t n0
  * rows (_row) and heads (_head); the head_dim floats of a row lie next to each other; rows and
  * strides are multiples of 16 bytes.  n = 0 does nothing.
  *
- * All calls are asynchronous on the context stream and can be captured. */
+ * All calls are asynchronous on the context stream and can be captured.  attend and weights use the
+ * context's workspace, as the dense kernels' K splits do: calls of one context that could run at the
+ * same time (replays of its graphs on different streams, calls after shp_set_stream while the old
+ * stream still works) have to be ordered by the caller. */
 enum {
     SHP_CACHE8_I8 = 0,  /* -127 .. 127 */
     SHP_CACHE8_E4M3 = 1 /* 8-bit floats, 4 bits of exponent and 3 of mantissa, up to 448 */
@@ -260,11 +263,12 @@ int shp_cache8_evict(shp_ctx* ctx, const shp_cache8* src, const shp_cache8* dst,
  * targets[r] (minus infinity for an id outside the vocabulary), entropy = -sum p log p, both in
  * natural logarithms, and the n_top likeliest ids with their log probabilities, [rows][n_top], the
  * likeliest first and of equal ones the lowest id first.  targets with logprob, entropy, and
- * top_ids with top_logprobs may be NULL.  0 <= n_top <= 64 and at most vocab.  A logit of minus
+ * top_ids with top_logprobs may be NULL.  0 <= n_top <= 64 and at most vocab; up to 16,000,000 rows
+ * and 2^30 logits a row.  A logit of minus
  * infinity is a token that cannot be; a row that holds a NaN or plus infinity, or nothing but minus
- * infinity, has NaN in place of logarithms, and its ids go by the logits with NaN last.  Rows of
- * more than 32,768 logits use the context's workspace, as shp_cache8_attend does, and are refused
- * in a capture that finds it too small. */
+ * infinity, has NaN in place of logarithms, and its ids go by the logits with NaN last.  Fewer than
+ * 256 rows of more than 32,768 logits use the context's workspace, as shp_cache8_attend does, and are
+ * refused in a capture that finds it too small. */
 typedef struct shp_logprobs_args {
     const float* logits;
     int64_t row_stride;

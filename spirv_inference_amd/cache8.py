@@ -38,6 +38,10 @@ class Cache8:
                  v: Optional[DeviceTensor] = None, k_scale: Optional[DeviceTensor] = None,
                  v_scale: Optional[DeviceTensor] = None,
                  lengths: Optional[DeviceTensor] = None):
+        if fmt not in FORMATS:
+            raise ValueError(f"format {fmt!r}: one of {', '.join(FORMATS)} is needed")
+        if block not in (16, 32, 64, 128):
+            raise ValueError(f"blocks of {block} tokens: 16, 32, 64 or 128 are needed")
         self.ctx = ctx
         self.n_seqs, self.n_kv_heads, self.head_dim = n_seqs, n_kv_heads, head_dim
         self.capacity, self.block, self.fmt = capacity, block, fmt

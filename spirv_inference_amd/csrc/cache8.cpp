@@ -211,8 +211,8 @@ int shp_token_logprobs(shp_ctx* ctx, const shp_logprobs_args* a) {
     if (!a->targets != !a->logprob) return bad(me, "targets and logprob go together");
     if (a->n_top && (!a->top_ids || !a->top_logprobs))
         return bad(me, "n_top without top_ids or top_logprobs");
-    if ((int64_t)a->rows * ((a->vocab + 4095) / 4096) > 0x7fffffff)
-        return bad(me, "too many logits", SHP_ERR_UNSUPPORTED);
+    if (a->rows > 16000000 || a->vocab > (1 << 30))
+        return bad(me, "more than 16000000 rows or 2^30 logits a row", SHP_ERR_UNSUPPORTED);
     if (!ctx) return bad(me, "null ctx");
     if (a->rows == 0) return SHP_OK;
     Ctx* x = reinterpret_cast<Ctx*>(ctx);

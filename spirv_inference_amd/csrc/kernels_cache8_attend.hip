@@ -176,6 +176,20 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
     if ((int)blockIdx.z >= splits) return;
     const int tile0 = (int)blockIdx.z * share, tile1 = min(tiles, tile0 + share);
 
+    const uint8_t* kp = c.k + (int64_t)sh * c.cap * D;
+    const uint8_t* vp = c.v + (int64_t)sh * c.cap * D;
+    const int64_t sbase = (int64_t)sh * (c.cap >> c.block_log2);
+    const int last_block = max(p.len - 1, 0) >> c.block_log2;
+    u4 kr[4][D / 64], vr[NO];
+    float ks = 0.0f, vs = 0.0f;
+    auto fetch = [&](int tile) __attribute__((always_inline)) {
+        load_k<D>(kp + (int64_t)tile * kCacheTile * D, kr);
+        load_v<D>(vp + (int64_t)tile * kCacheTile * D, vr);
+        const int64_t b = sbase + min((tile * kCacheTile + 16 * g) >> c.block_log2, last_block);
+        ks = c.k_scale[b];
+        vs = c.v_scale[b];
+    };
+
     float m[MT], l[MT], back[MT];
     int limit[MT];
     f4 o[MT][NO];
@@ -191,20 +205,10 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
     // tokens that every row sees
     const int open = max(p.len - p.count + r0 / q.group + 1, 0);
 
-    const uint8_t* kp = c.k + (int64_t)sh * c.cap * D;
-    const uint8_t* vp = c.v + (int64_t)sh * c.cap * D;
-    const int64_t sbase = (int64_t)sh * (c.cap >> c.block_log2);
-    const int last_block = max(p.len - 1, 0) >> c.block_log2;
-
     for (int tile = tile0 + wave; tile < tile1; tile += WAVES) {
         const int t0 = tile * kCacheTile;
-        u4 kr[4][D / 64], vr[NO];
-        load_k<D>(kp + (int64_t)t0 * D, kr);
-        load_v<D>(vp + (int64_t)t0 * D, vr);
-        const int64_t b = sbase + min((t0 + 16 * g) >> c.block_log2, last_block);
-        const float ks = c.k_scale[b];
-        float vs = c.v_scale[b];
-        vs = vs < kScaleFloor ? kScaleFloor : vs;
+        // (the next tile's loads ahead of their use cost a wavefront of occupancy and 5 %)
+        fetch(tile);
         const bool edge = t0 + kCacheTile > open;
         f4 sc[MT][4];
 #pragma unroll
@@ -223,11 +227,12 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
             }
         }
         // sc[t][j][i]: token t0 + 16 g + 4 j + i, row r0 + 16 t + li
-        const float lv = __builtin_amdgcn_logf(vs);
+        const float kscale = ks, vscale = vs < kScaleFloor ? kScaleFloor : vs;
+        const float lv = __builtin_amdgcn_logf(vscale);
         h8 wh[MT][2], wl[MT][2];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const float f = ks * back[t];
+            const float f = kscale * back[t];
             float mx = -__builtin_inff();
             if (edge) {
 #pragma unroll
@@ -286,7 +291,7 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
                     wl[t][j >> 1][e + 1] = pl.y;
                 }
             }
-            if (sum != 0.0f) l[t] += sum / vs;  // of a block nobody sees, the scale may be NaN
+            if (sum != 0.0f) l[t] += sum / vscale;  // of a block nobody sees, the scale may be NaN
         }
         if (FMT == kE4M3 && t0 + kCacheTile > p.len) {
             // bytes behind the last token may be NaN codes, which a weight of zero does not cancel

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import cache8_ref as R
-from spirv_inference_amd import _lib
+from spirv_inference_amd import Cache8, _lib
 from spirv_inference_amd._lib import (Cache8AppendArgs, Cache8AttendArgs, Cache8EvictArgs,
                                       Cache8Struct, Cache8WeightsArgs, LogprobsArgs)
 
@@ -161,10 +161,19 @@ def test_bad_reads_and_evictions_are_refused():
     (dict(logits=P + 2), "logits"), (dict(row_stride=63), "row_stride"),
     (dict(n_top=-1), "n_top"), (dict(n_top=65, vocab=100, row_stride=100), "n_top"),
     (dict(n_top=9, vocab=8), "n_top"), (dict(targets=0), "targets"), (dict(logprob=0), "targets"),
-    (dict(top_ids=0), "top_ids"), (dict(top_logprobs=0), "top_ids")])
+    (dict(top_ids=0), "top_ids"), (dict(top_logprobs=0), "top_ids"),
+    (dict(rows=16000001), "16000000"), (dict(vocab=(1 << 30) + 1, row_stride=1 << 31), "2^30")])
 def test_bad_logprobs_are_refused(over, what):
     rc, msg = call("shp_token_logprobs", args(LogprobsArgs, **over))
     assert rc != 0 and what in msg and "ctx" not in msg, msg
+
+
+def test_the_mirror_refuses_unknown_formats_and_blocks():
+    with pytest.raises(ValueError, match="i8, e4m3"):
+        Cache8(None, 1, 1, 64, 64, fmt="int8")
+    for block in (0, 8, 48, 256):
+        with pytest.raises(ValueError, match="16, 32, 64 or 128"):
+            Cache8(None, 1, 1, 64, 64, block=block)
 
 
 # ---- the reference itself -------------------------------------------------------------------

@@ -498,6 +498,19 @@ def test_eviction_orders_weights(ctx, kind):
             q.ref = R.RefCache(1, 2, 64, 1536, 64, "i8")
 
 
+@pytest.mark.parametrize("n", [1000, 1030, 8200, 8230, 20000, 32800, 40000])
+def test_eviction_from_long_sequences(ctx, n):
+    """Weights by the thousand: those a workgroup holds one, 8 or 32 a thread, and those it reads
+    again for each digit; with plateaus, so that a digit's count decides."""
+    rng = np.random.default_rng(n)
+    cap = -(-n // 64) * 64
+    w = np.round(rng.exponential(size=(1, 1, cap)) * 40).astype(np.float32) / 40
+    keep = 500
+    with filled(ctx, rng, 1, 1, 64, cap, 64, "i8", [n]) as p, \
+            Pair(ctx, 1, 1, 64, 512, 64, "i8") as q:
+        evict_both(p, q, w, keep, 7)
+
+
 def test_eviction_of_a_spoiled_block_spoils_where_its_tokens_go(ctx):
     rng = np.random.default_rng(41)
     k, v = rows(rng, 1, 100, 1, 64), rows(rng, 1, 100, 1, 64)
@@ -623,6 +636,33 @@ def test_a_capture_without_workspace_runs_unsplit(ctx):
             own.sync()
             assert (np.abs(out.download().reshape(q.shape) - want) <= tol).all()
             out.upload(np.zeros(4 * 64, np.float32))
+        g.destroy()
+
+
+def test_accounts_captured_without_workspace(ctx):
+    """Row groups cannot leave their sums anywhere: one wavefront after the other adds its rows."""
+    rng = np.random.default_rng(56)
+    n, heads, cap, lens = 60, 8, 384, [300, 61]
+    with Context("any") as own, filled(own, rng, 2, 1, 64, cap, 32, "e4m3", lens) as p:
+        q = rows(rng, 2, n, heads, 64)
+        tq, out, lse = p.up(q), p.new(q.size), p.new(2 * heads * n)
+        start = rng.uniform(0, 2, (2, 1, cap)).astype(np.float32)
+        acc, res = p.up(start), p.new(start.size, fill=-3)
+        own.capture_begin()
+        p.dev.attend(tq, out, heads, n, lse=lse)
+        p.dev.weights(tq, lse, acc, res, heads, n)
+        g = own.capture_end()
+        for _ in range(3):
+            g.launch()
+            own.sync()
+            l64 = lse.download().reshape(2, heads, n).astype(np.float64)
+            want, tol = R.attend(p.ref, q, [n, n], 0.125, lse_in=l64)
+            got = res.download().reshape(start.shape)
+            for s, ln in enumerate(lens):
+                t = tol[s, :, :ln] + (want[s, :, :ln] + start[s, :, :ln]) * (n * heads + 2) * 2.0 ** -24
+                assert (np.abs(got[s, :, :ln] - want[s, :, :ln] - start[s, :, :ln]) <= t).all()
+                assert (got[s, :, ln:] == -3).all()
+            res.upload(np.full(start.size, -3))
         g.destroy()
 
 
