@@ -68,6 +68,8 @@ class Cache8:
                                     self.lengths.ptr, n_seqs, n_kv_heads, head_dim, capacity,
                                     block, FORMATS[fmt])
         self._ref = C.byref(self._struct)
+        self._lib = lib()
+        self._plain = {}  # (rows, heads) -> strides of a tensor without gaps
 
     def close(self) -> None:
         for t in self._own:
@@ -84,34 +86,42 @@ class Cache8:
         """Uploads how many tokens each sequence holds (synchronous)."""
         self.lengths.upload(np.asarray(lengths, np.int32))
 
-    def _strides(self, strides, n: int, heads: int):
-        d = self.head_dim
-        return (n * heads * d, heads * d, d) if strides is None else strides
+    def _strides(self, n: int, heads: int):
+        s = self._plain.get((n, heads))
+        if s is None:
+            d = self.head_dim
+            s = self._plain[n, heads] = (n * heads * d, heads * d, d)
+        return s
 
     def append(self, k: DeviceTensor, v: DeviceTensor, n: int,
                counts: Optional[DeviceTensor] = None, k_strides=None, v_strides=None) -> None:
         """Quantises the new rows k and v into the cache (shp_cache8_append)."""
-        args = Cache8AppendArgs(k.ptr, v.ptr, *self._strides(k_strides, n, self.n_kv_heads),
-                                *self._strides(v_strides, n, self.n_kv_heads), _ptr(counts), n)
-        check(lib().shp_cache8_append(self.ctx.handle, self._ref, C.byref(args)),
-              "shp_cache8_append")
+        plain = self._strides(n, self.n_kv_heads)
+        args = Cache8AppendArgs(k.ptr, v.ptr, *(k_strides or plain), *(v_strides or plain),
+                                _ptr(counts), n)
+        rc = self._lib.shp_cache8_append(self.ctx.handle, self._ref, args)
+        if rc:
+            check(rc, "shp_cache8_append")
 
     def read(self, n: int, k: Optional[DeviceTensor], v: Optional[DeviceTensor]) -> None:
         """The values of every sequence's newest n tokens, [n_seqs][n_kv_heads][n][head_dim]
         (shp_cache8_read)."""
-        check(lib().shp_cache8_read(self.ctx.handle, self._ref, n, _ptr(k), _ptr(v)),
-              "shp_cache8_read")
+        rc = self._lib.shp_cache8_read(self.ctx.handle, self._ref, n, _ptr(k), _ptr(v))
+        if rc:
+            check(rc, "shp_cache8_read")
 
     def attend(self, q: DeviceTensor, out: DeviceTensor, n_heads: int, n: int,
                counts: Optional[DeviceTensor] = None, lse: Optional[DeviceTensor] = None,
                scale: Optional[float] = None, q_strides=None, o_strides=None) -> None:
         """Attention of n rows a sequence over the cached tokens (shp_cache8_attend); scale is
         head_dim ** -0.5 unless given, lse [n_seqs][n_heads][n] gets the log sums."""
-        args = Cache8AttendArgs(q.ptr, out.ptr, *self._strides(q_strides, n, n_heads),
-                                *self._strides(o_strides, n, n_heads), _ptr(counts), _ptr(lse),
-                                n, n_heads, self.head_dim ** -0.5 if scale is None else scale)
-        check(lib().shp_cache8_attend(self.ctx.handle, self._ref, C.byref(args)),
-              "shp_cache8_attend")
+        plain = self._strides(n, n_heads)
+        args = Cache8AttendArgs(q.ptr, out.ptr, *(q_strides or plain), *(o_strides or plain),
+                                _ptr(counts), _ptr(lse), n, n_heads,
+                                self.head_dim ** -0.5 if scale is None else scale)
+        rc = self._lib.shp_cache8_attend(self.ctx.handle, self._ref, args)
+        if rc:
+            check(rc, "shp_cache8_attend")
 
     def weights(self, q: DeviceTensor, lse: DeviceTensor, acc_in: Optional[DeviceTensor],
                 acc_out: DeviceTensor, n_heads: int, n: int,
@@ -119,16 +129,18 @@ class Cache8:
                 q_strides=None) -> None:
         """Adds the attention weight that the rows of an attend() gave each token to its account,
         [n_seqs][n_kv_heads][capacity] (shp_cache8_weights)."""
-        args = Cache8WeightsArgs(q.ptr, *self._strides(q_strides, n, n_heads), _ptr(counts),
+        args = Cache8WeightsArgs(q.ptr, *(q_strides or self._strides(n, n_heads)), _ptr(counts),
                                  lse.ptr, _ptr(acc_in), acc_out.ptr, n, n_heads,
                                  self.head_dim ** -0.5 if scale is None else scale)
-        check(lib().shp_cache8_weights(self.ctx.handle, self._ref, C.byref(args)),
-              "shp_cache8_weights")
+        rc = self._lib.shp_cache8_weights(self.ctx.handle, self._ref, args)
+        if rc:
+            check(rc, "shp_cache8_weights")
 
     def evict(self, dst: "Cache8", weights: DeviceTensor, keep: int, recent: int,
               kept: DeviceTensor, dst_weights: Optional[DeviceTensor] = None) -> None:
         """Copies each sequence's newest `recent` tokens and the heaviest others, `keep` in all, to
         the cache dst (shp_cache8_evict); kept [n_seqs][n_kv_heads][keep] gets their places."""
         args = Cache8EvictArgs(weights.ptr, kept.ptr, _ptr(dst_weights), keep, recent)
-        check(lib().shp_cache8_evict(self.ctx.handle, self._ref, dst._ref, C.byref(args)),
-              "shp_cache8_evict")
+        rc = self._lib.shp_cache8_evict(self.ctx.handle, self._ref, dst._ref, args)
+        if rc:
+            check(rc, "shp_cache8_evict")
