@@ -1,9 +1,11 @@
 // Attention over the 8-bit cache, and the accounts of the weight each cached token gets.
 //
-// A wavefront owns 16 * MT query rows (the rows of all query heads of a KV head, row r = new token
+// A wavefront holds 16 * MT query rows (the rows of all query heads of a KV head, row r = new token
 // r / group, head r % group) and walks the sequence's tokens 64 at a time, with the running maximum
 // and sum of a softmax.  Codes are exact as fp16, q and the weights are cut into two fp16 pieces of
-// 11 bits, so the products run on v_mfma_f32_16x16x32_f16 and keep fp32's accuracy.
+// 11 bits (both rounded to nearest, so an operand is off by 2^-23 of itself), and the products run on
+// v_mfma_f32_16x16x32_f16 with fp32 sums: twice the products of one fp16 pass at 8 times the rate of
+// fp32's own matrix instructions, and errors against 64 bits no larger than those of fp32 products.
 //
 // Scores are computed transposed, S^T = K Q^T.  Row m of token tile j is given to token
 // (m / 4) * 16 + 4 j + m % 4 of the 64: the lane (query l % 16, group g = l / 16) then holds the
@@ -32,7 +34,7 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kLift = 12.0f;  // weights reach 2^12: the low piece stays a normal fp16 number longer
-constexpr float kLargeScore = 262144.0f;
+constexpr float kLargeScore = 262144.0f;  // |m| past which the rounding of m matters to a weight
 constexpr int kQBits = 14;      // a row of q is scaled to reach 2^13 .. 2^14
 
 // Four codes as fp16 numbers.
@@ -146,6 +148,18 @@ __device__ __forceinline__ float log_sum(float m, float l) {
     return l == 0.0f ? -__builtin_inff() : (m - kLift + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
+// A workgroup's four wavefronts hold the same rows and take a tile each in turn; their parts meet in LDS
+// at the end.  (Side by side over rows they would share tiles, but then few rows have to be cut into
+// many shares of the tokens, whose parts go through memory: 512 rows x 4 heads on 8,190 tokens 171 us
+// that way, 147 so, measured in one run.)  32 rows are what registers allow with two workgroups on a CU:
+// 64 rows of 64 dimensions spilled and took 147 us where 32 take 92.  The tokens of a sequence are shared
+// out over workgroups while that fills the GPU.
+//
+// With up to 16 rows reading the cache bounds it: 16 x 128,001-131,072 tokens x 8 heads x 128 (4.2 GB)
+// 722 us, 5.9 TB/s, 24 sequences of 0-8,100 tokens 54 us, 3.7 TB/s (46 us where they are all as long as
+// the average); a single sequence of 300 tokens takes 5.8 us, which is latency.  With more rows the matrix
+// and vector units do, which take about as long: 512 rows x 4 heads on 8,190 tokens x 8 heads x 128
+// (66.6 GFLOP, twice that as products of pieces) 150 us, 890 TFLOP/s of products.
 template <int D, int FMT, int MT>
 __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Query q, int least,
                                                                float* part, int* counters) {
@@ -467,8 +481,10 @@ __device__ __forceinline__ void halve(float* v) {
 // lane l ends up with token l's.  Where a KV head has more rows than that, row groups leave their sums
 // in `part` [group][head][capacity] and cache8_weights_join_kernel adds them in order; a group of
 // several chunks of rows adds to what its own chunks before left there.  groups == 1 writes the
-// accounts themselves.  One query row in 16 lanes' worth of columns costs as much as 16, so a decode
-// step is bound by reading K; a prompt's chunk by the vector unit (exp2 and the conversions of K).
+// accounts themselves.  A decode step is bound by reading K: 24 sequences of 500-8,100 tokens x 8 heads x
+// 128 (113 MB) 30 us, 3.8 TB/s.  A prompt's chunk is bound by the vector unit (exp2, the conversion of K,
+// q's pieces): 512 rows x 8 heads on 8,190 tokens x 4 heads x 64 (16.6 GFLOP) 50.5 us, of
+// which 5 are the join.
 template <int D, int FMT, int MT>
 __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(Cache8 c, Cache8Query q, int row_waves,
                                                              int groups, int chunks, float* part) {
@@ -586,20 +602,26 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(Cache8 c, Cache8
     }
 }
 
-// acc_out = acc_in + the row groups' sums, in order.
+// acc_out = acc_in + the row groups' sums: a lane a token, a wavefront every fourth group, in order.
 __global__ __launch_bounds__(256) void cache8_weights_join_kernel(Cache8 c, Cache8Query q, int groups,
                                                                   int rows_of_group, const float* part) {
-    const int sh = blockIdx.y, s = sh / c.kv, t = (int)blockIdx.x * 256 + threadIdx.x;
+    __shared__ float sums[4][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int sh = blockIdx.y, s = sh / c.kv, t = (int)blockIdx.x * 64 + lane;
     const int len = seq_length(c, s), count = seq_count(q.counts, q.n, s);
-    if (t >= len) return;
+    if ((int)blockIdx.x * 64 >= len) return;
+    const int64_t at = (int64_t)sh * c.cap + t, stride = (int64_t)gridDim.y * c.cap;
     // the groups with a row that sees token t
     const int first = max(t - (len - count), 0) * q.group / rows_of_group;
-    const int end = (count * q.group + rows_of_group - 1) / rows_of_group;
-    const int64_t at = (int64_t)sh * c.cap + t, stride = (int64_t)gridDim.y * c.cap;
+    const int end = t < len ? (count * q.group + rows_of_group - 1) / rows_of_group : 0;
     float sum = 0.0f;
 #pragma unroll 8
-    for (int i = first; i < end; ++i) sum += part[i * stride + at];
-    q.acc_out[at] = (q.acc_in ? q.acc_in[at] : 0.0f) + sum;
+    for (int i = first + wave; i < end; i += 4) sum += part[i * stride + at];
+    sums[wave][lane] = sum;
+    __syncthreads();
+    if (wave || t >= len) return;
+    q.acc_out[at] = (q.acc_in ? q.acc_in[at] : 0.0f) +
+                    ((sums[0][lane] + sums[1][lane]) + (sums[2][lane] + sums[3][lane]));
 }
 
 }  // namespace
@@ -612,8 +634,12 @@ Cache8Plan cache8_attend_plan(const Cache8& c, int head_dim, int64_t rows, int c
     p.row_tiles = rows <= 16 ? 1 : 2;
     const int64_t per = 16 * p.row_tiles;
     p.row_blocks = (int)((rows + per - 1) / per);
-    // Workgroups for 8 on every CU with 16 rows, which evens out sequences of different length, and
-    // for the two that it holds at once with 32; a workgroup takes two tiles a wavefront or more.
+    // Workgroups for 8 on every CU with 16 rows, which evens out sequences of different length (64 x
+    // 3,000-6,000 tokens: 123 us, 134 with 4 and 127 with 16 a CU), and for the two that it holds at
+    // once with 32 (64 rows x 4 heads: 35 us, 44 with 4 a CU, 42 with one).  A workgroup takes two
+    // tiles a wavefront or more (300 tokens 5.8 us, 7.0 from one tile; 4 rows of 8 sequences 18.4, 25.8),
+    // a sequence 32 shares at most, whose parts one workgroup joins (32,000 tokens 24.6 us with 32, 29.9
+    // with 16).
     const int64_t units = (int64_t)c.n_seqs * c.kv * p.row_blocks;
     const int64_t want = ((p.row_tiles == 2 ? 2 : 8) * (int64_t)std::max(cu_count, 1) + units - 1) / units;
     p.least = 8;
@@ -670,7 +696,7 @@ int cache8_weights_launch(hipStream_t s, const Cache8& c, int head_dim, int form
                        dim3(256), 0, s, c, q, p.row_waves, p.groups, p.chunks, scratch);
     SHP_HIP_CHECK(hipGetLastError());
     if (p.groups > 1) {
-        hipLaunchKernelGGL(cache8_weights_join_kernel, dim3((c.cap + 255) / 256, c.n_seqs * c.kv),
+        hipLaunchKernelGGL(cache8_weights_join_kernel, dim3(c.cap / kCacheTile, c.n_seqs * c.kv),
                            dim3(256), 0, s, c, q, p.groups, 16 * p.row_tiles * p.chunks, scratch);
         SHP_HIP_CHECK(hipGetLastError());
     }

@@ -3,8 +3,13 @@
 //
 // A workgroup holds 32 logits a thread in registers: their maximum m, Z = sum exp(x - m) and X = sum
 // exp(x - m) (x - m) give log p = x - m - log Z and the entropy log Z - X / Z, a sum of two numbers
-// that are not negative.  Where there are rows enough, a workgroup of 512 takes a row, chunk after
-// chunk; few rows are cut into parts of 32,768 logits for workgroups of 1,024, and joined.
+// that are not negative.
+//
+// From 256 rows on a workgroup takes a row, chunk after chunk, and reading bounds it: 1,500 x
+// 131,071 with 20 alternatives (786 MB) 160 us, 4.9 TB/s, 146 without alternatives.  It has 256 threads,
+// from 1,024 rows on 128 (4,000 x 40,000 133 us, 148 with 256; 600 x 32,000 40, 30).  Fewer rows are cut
+// into parts of 32,768 logits for workgroups of 1,024, and joined: 1 x 32,000 9.4 us (17 the other
+// way), 128 x 32,000 12.2 (26); 300 x 131,071 take 69 and 72, 600 x 32,000 28 and 35.
 #include "cache8.h"
 
 namespace {
@@ -15,7 +20,7 @@ typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kHeld = 32;
 constexpr int kFewThreads = 1024, kFewSpan = kFewThreads * kHeld, kManyThreads = 256;
-constexpr int kManyRows = 256;
+constexpr int kManyRows = 256, kMostRows = 1024, kMostThreads = 128;
 constexpr int kCandidates = 448;  // logits of a chunk that are put in order by counting
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -434,7 +439,10 @@ size_t logprobs_scratch(int rows, int vocab) {
 int logprobs_launch(hipStream_t s, const LogprobArgs& a, float* scratch) {
     const int p = parts_of(a.rows, a.vocab);
     Part* out = reinterpret_cast<Part*>(scratch);
-    if (a.rows >= kManyRows)
+    if (a.rows >= kMostRows)
+        hipLaunchKernelGGL((logprobs_kernel<kMostThreads, true>), dim3(a.rows), dim3(kMostThreads), 0, s, a, 1,
+                           a.vocab, out);
+    else if (a.rows >= kManyRows)
         hipLaunchKernelGGL((logprobs_kernel<kManyThreads, true>), dim3(a.rows), dim3(kManyThreads), 0, s, a, 1,
                            a.vocab, out);
     else
