@@ -8,7 +8,7 @@
 // From 256 rows on a workgroup takes a row, chunk after chunk, and reading bounds it: 1,500 x
 // 131,071 with 20 alternatives (786 MB) 160 us, 4.9 TB/s, 146 without alternatives.  It has 256 threads,
 // from 1,024 rows on 128 (4,000 x 40,000 133 us, 148 with 256; 600 x 32,000 40, 30).  Fewer rows are cut
-// into parts of 32,768 logits for workgroups of 1,024, and joined: 1 x 32,000 9.4 us (17 the other
+// into parts of 32,768 logits for workgroups of 1,024, and joined: 1 x 32,000 8.2 us (17 the other
 // way), 128 x 32,000 12.2 (26); 300 x 131,071 take 69 and 72, 600 x 32,000 28 and 35.
 #include "cache8.h"
 
@@ -116,20 +116,27 @@ __device__ __forceinline__ int id_at(int i0, int e) {
     return i0 + ((e >> 2) * T + (int)threadIdx.x) * 4 + (e & 3);
 }
 
-// A logit that `top` threads reach with the best they hold, so that `top` logits or more do (if that
-// many threads hold one): one wavefront halves the range of the threads' best until no more than
-// twice as many pass.  For everybody behind the next barrier.
+// A logit that `top` groups of threads reach with the best they hold, so that `top` logits or more do
+// (if that many groups hold one): one wavefront halves the range of the groups' best until no more
+// than twice as many pass.  Up to 24 alternatives take 64 groups, one a lane, at a ballot a turn (a row
+// of 32,000, 5 alternatives: 9.5 us by threads, 8.2 by groups; 24: 11.3 and 10.5).  More would let
+// through many logits too many, which all have to be put in order (32: 11.3 and 13.9; 64: 13.7 and
+// 22.9), and take the threads one by one.  For everybody behind the next barrier.
 template <int T>
 __device__ __forceinline__ void find_threshold(int top, Shared<T>& sm) {
     const int tid = threadIdx.x;
     if (tid >= 64) return;
-    unsigned b[T / 64], lo = ~0u, hi = 0;
+    unsigned b[T / 64], best = 0;
 #pragma unroll
     for (int i = 0; i < T / 64; ++i) {
         b[i] = sm.bests[i * 64 + tid];
-        lo = min(lo, b[i]);
-        hi = max(hi, b[i]);
+        best = max(best, b[i]);
     }
+    const bool groups = top <= 24;
+    unsigned lo = best, hi = best;
+    if (!groups)
+#pragma unroll
+        for (int i = 0; i < T / 64; ++i) lo = min(lo, b[i]);
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) {
         lo = min(lo, (unsigned)__shfl_xor((int)lo, o));
@@ -138,8 +145,12 @@ __device__ __forceinline__ void find_threshold(int top, Shared<T>& sm) {
     while (hi - lo > 1) {
         const unsigned next = lo + (hi - lo) / 2;
         int n = 0;
+        if (groups) {
+            n = __popcll(__ballot(best >= next));
+        } else {
 #pragma unroll
-        for (int i = 0; i < T / 64; ++i) n += __popcll(__ballot(b[i] >= next));
+            for (int i = 0; i < T / 64; ++i) n += __popcll(__ballot(b[i] >= next));
+        }
         if (n < top) {
             hi = next;
         } else {
@@ -147,7 +158,7 @@ __device__ __forceinline__ void find_threshold(int top, Shared<T>& sm) {
             if (n <= 2 * top) break;
         }
     }
-    // as a float of that order; 0: some threads hold nothing, and the others pass all they have
+    // as a float of that order; 0: some groups hold nothing, and the others pass all they have
     if (tid == 0)
         sm.threshold = lo & 0x80000000u ? __uint_as_float(lo ^ 0x80000000u)
                        : lo             ? __uint_as_float(~lo) : -__builtin_inff();
