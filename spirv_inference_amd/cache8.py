@@ -75,6 +75,9 @@ class Cache8:
         for t in self._own:
             t.free()
         self._own = []
+        # calls on a closed cache are refused
+        st = self._struct
+        st.k = st.v = st.k_scale = st.v_scale = st.lengths = None
 
     def __enter__(self):
         return self

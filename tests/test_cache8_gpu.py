@@ -733,3 +733,17 @@ def test_refusals_name_the_call(ctx):
         with pytest.raises(ValueError, match="bytes where the cache needs"):
             Cache8(ctx, 1, 1, 64, 128, k=ctx.empty(4, np.uint8))
         t.free()
+
+
+def test_a_closed_cache_refuses_calls(ctx):
+    c, open_one = Cache8(ctx, 1, 1, 64, 64), Cache8(ctx, 1, 1, 64, 64)
+    c.close()
+    t = ctx.empty(4096)
+    for call in (lambda: c.append(t, t, 1), lambda: c.read(1, t, t), lambda: c.attend(t, t, 1, 1),
+                 lambda: c.weights(t, t, None, t, 1, 1), lambda: c.evict(open_one, t, 1, 0, t),
+                 lambda: open_one.evict(c, t, 1, 0, t)):
+        with pytest.raises(ShpError, match="null array in the cache"):
+            call()
+    c.close()
+    open_one.close()
+    t.free()
