@@ -11,7 +11,7 @@
 // (m / 4) * 16 + 4 j + m % 4 of the 64: the lane (query l % 16, group g = l / 16) then holds the
 // scores of tokens 16 g .. 16 g + 15, all of one block (one scale), and these are the k slots that
 // the lane's 16 bytes of a dimension of V stand for in O^T = V^T P^T.  So K and V go from memory to
-// the matrix cores without LDS, in 16-byte loads, and P never leaves its registers.
+// the matrix cores without LDS, in 16-byte loads (but see stage_k), and P never leaves its registers.
 //
 // With u_t = log2 of (weight * scale of V), the running maximum m is taken over u, and
 // w_t = 2^(u_t - m + 12) is what multiplies V's codes: it spans fp16's range whatever the scales
@@ -128,6 +128,37 @@ __device__ __forceinline__ void load_k(const uint8_t* tile, u4 raw[4][D / 64]) {
         for (int a = 0; a < D / 64; ++a)
             raw[j][a] = *reinterpret_cast<const u4*>(p + 4 * j * D + 64 * a);
 }
+// K's tiles of 128 dimensions go through LDS where 32 rows share one: lanes 0 to 15 of load_k read 16
+// bytes each of 16 rows, 16 cache lines, and tiles that many rows want come from L2, where that is
+// what costs (512 rows on 8,190 tokens: attention 141 us so, 150 without, accounts 88 and 97; rows of 64
+// dimensions are half as many lines and attention takes 94 and 91, and 16 query rows, which memory
+// bounds, 727 and 720).
+template <int D, int MT>
+constexpr bool kStaged = D == 128 && MT == 2;
+typedef const __attribute__((address_space(1))) void* GlobalPtr;
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+// A wavefront's tile to LDS in whole rows, 1 KB a load, without passing its registers.  Piece p (16 bytes)
+// of token t's row goes to place p ^ turn(t), turn(t) = t % 4 + 4 * (t / 16 % 2), so that the eight
+// lanes that staged() serves at once take different banks.
+__device__ __forceinline__ void stage_k(const uint8_t* tile, uint8_t* lds) {
+    const int lane = threadIdx.x & 63, t = lane >> 3, at = t * 128 + 16 * ((lane & 7) ^ (t & 3));
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        __builtin_amdgcn_global_load_lds((GlobalPtr)(tile + i * 1024 + (at ^ (i & 2 ? 64 : 0))),
+                                         (LdsPtr)(lds + i * 1024), 16, 0, 0);
+}
+// Until the wavefront's tile is there: the compiler does not promise to wait for these loads.
+__device__ __forceinline__ void wait_staged() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+// raw[j][a] of load_k.
+__device__ __forceinline__ u4 staged(const uint8_t* lds, int j, int a) {
+    const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+    const int t = (m >> 2) * 16 + 4 * j + (m & 3);
+    return *reinterpret_cast<const u4*>(lds + t * 128 + 16 * ((4 * a + g) ^ (m & 7)));
+}
 // V of a 64-token tile: raw[d] = tokens 16 g .. 16 g + 15 of dimension 16 d + m.
 template <int D>
 __device__ __forceinline__ void load_v(const uint8_t* tile, u4 raw[D / 16]) {
@@ -159,13 +190,17 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 // 722 us, 5.9 TB/s, 24 sequences of 0-8,100 tokens 54 us, 3.7 TB/s (46 us where they are all as long as
 // the average); a single sequence of 300 tokens takes 5.8 us, which is latency.  With more rows the matrix
 // and vector units do, which take about as long: 512 rows x 4 heads on 8,190 tokens x 8 heads x 128
-// (66.6 GFLOP, twice that as products of pieces) 150 us, 890 TFLOP/s of products.
+// (66.6 GFLOP, twice that as products of pieces) 141 us, 945 TFLOP/s of products.
 template <int D, int FMT, int MT>
 __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Query q, int least,
                                                                float* part, int* counters) {
     constexpr int NO = D / 16;   // accumulators of 16 rows
     constexpr int PW = D + 4;    // floats of a row's part: sums, maximum, weight, two of padding
-    __shared__ __attribute__((aligned(16))) float ex[2][MT * (NO * 4 + 2) * 64];
+    // staged tiles of K, then parts of rows
+    constexpr bool STAGED = kStaged<D, MT>;
+    constexpr int EX = MT * (NO * 4 + 2) * 64, KB = STAGED ? 64 * D : 0;
+    __shared__ __attribute__((aligned(16))) float ex[2][EX];
+    static_assert(4 * KB <= 2 * EX * 4);
     __shared__ int arrived;
     constexpr int ROWS = 16 * MT, WAVES = 4;
     const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
@@ -194,10 +229,15 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
     const uint8_t* vp = c.v + (int64_t)sh * c.cap * D;
     const int64_t sbase = (int64_t)sh * (c.cap >> c.block_log2);
     const int last_block = max(p.len - 1, 0) >> c.block_log2;
+    uint8_t* const kl = reinterpret_cast<uint8_t*>(&ex[0][0]) + wave * KB;
     u4 kr[4][D / 64], vr[NO];
     float ks = 0.0f, vs = 0.0f;
     auto fetch = [&](int tile) __attribute__((always_inline)) {
-        load_k<D>(kp + (int64_t)tile * kCacheTile * D, kr);
+        if constexpr (STAGED) {
+            stage_k(kp + (int64_t)tile * kCacheTile * D, kl);
+        } else {
+            load_k<D>(kp + (int64_t)tile * kCacheTile * D, kr);
+        }
         load_v<D>(vp + (int64_t)tile * kCacheTile * D, vr);
         const int64_t b = sbase + min((tile * kCacheTile + 16 * g) >> c.block_log2, last_block);
         ks = c.k_scale[b];
@@ -223,6 +263,7 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
         const int t0 = tile * kCacheTile;
         // (the next tile's loads ahead of their use cost a wavefront of occupancy and 5 %)
         fetch(tile);
+        if constexpr (STAGED) wait_staged();
         const bool edge = t0 + kCacheTile > open;
         f4 sc[MT][4];
 #pragma unroll
@@ -231,7 +272,9 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
             for (int t = 0; t < MT; ++t) sc[t][j] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int a = 0; a < D / 32; ++a) {
-                const u4 w = kr[j][a >> 1];
+                u4 w;
+                if constexpr (STAGED) w = staged(kl, j, a >> 1);
+                else w = kr[j][a >> 1];
                 const h8 kf = a & 1 ? codes8<FMT>(w.z, w.w) : codes8<FMT>(w.x, w.y);
 #pragma unroll
                 for (int t = 0; t < MT; ++t) {
@@ -337,6 +380,7 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
     }
 
     // the wavefronts' parts, in pairs: the upper one's goes through LDS
+    if constexpr (STAGED) __syncthreads();
 #pragma unroll
     for (int step = WAVES / 2; step > 0; step >>= 1) {
         float* x = ex[wave & (step - 1)];
@@ -488,6 +532,8 @@ __device__ __forceinline__ void halve(float* v) {
 template <int D, int FMT, int MT>
 __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(Cache8 c, Cache8Query q, int row_waves,
                                                              int groups, int chunks, float* part) {
+    constexpr bool STAGED = kStaged<D, MT>;
+    __shared__ __attribute__((aligned(16))) uint8_t tiles_k[STAGED ? 4 : 1][STAGED ? 64 * D : 16];
     const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int sh = blockIdx.x, tok_waves = 4 / row_waves;
@@ -536,13 +582,16 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(Cache8 c, Cache8
         }
         const bool gaps = !__all(whole);
         int tile = worker;
+        uint8_t* const kl = tiles_k[STAGED ? wave : 0];
         u4 kr[4][D / 64];
         float ks = 0.0f;
         auto fetch = [&](int t) __attribute__((always_inline)) {
-            load_k<D>(kp + (int64_t)t * kCacheTile * D, kr);
+            if constexpr (STAGED) stage_k(kp + (int64_t)t * kCacheTile * D, kl);
+            else load_k<D>(kp + (int64_t)t * kCacheTile * D, kr);
             ks = ksp[min((t * kCacheTile + 16 * g) >> c.block_log2, last_block)];
         };
         if (tile < tiles) fetch(tile);
+        if constexpr (STAGED) wait_staged();
         for (; tile < tiles; tile += workers) {
             const int t0 = tile * kCacheTile;
             float v[16], f[MT];
@@ -558,7 +607,9 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(Cache8 c, Cache8
                 for (int t = 0; t < MT; ++t) sc[t][j] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int a = 0; a < D / 32; ++a) {
-                    const u4 w = kr[j][a >> 1];
+                    u4 w;
+                    if constexpr (STAGED) w = staged(kl, j, a >> 1);
+                    else w = kr[j][a >> 1];
                     const h8 kf = a & 1 ? codes8<FMT>(w.z, w.w) : codes8<FMT>(w.x, w.y);
 #pragma unroll
                     for (int t = 0; t < MT; ++t) {
@@ -590,6 +641,7 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(Cache8 c, Cache8
             halve<4>(v);
             halve<2>(v);
             halve<1>(v);
+            if constexpr (STAGED) wait_staged();  // before the store, which would be waited for too
             const int t = t0 + lane;
             if (t < p.len) {
                 float sum = v[0];
