@@ -128,13 +128,13 @@ __device__ __forceinline__ void load_k(const uint8_t* tile, u4 raw[4][D / 64]) {
         for (int a = 0; a < D / 64; ++a)
             raw[j][a] = *reinterpret_cast<const u4*>(p + 4 * j * D + 64 * a);
 }
-// K's tiles of 128 dimensions go through LDS where 32 rows share one: lanes 0 to 15 of load_k read 16
+// K's tiles of 128 dimensions go through LDS where 32 rows or more share one: lanes 0 to 15 of load_k read 16
 // bytes each of 16 rows, 16 cache lines, and tiles that many rows want come from L2, where that is
-// what costs (512 rows on 8,190 tokens: attention 141 us so, 150 without, accounts 88 and 97; rows of 64
-// dimensions are half as many lines and attention takes 94 and 91, and 16 query rows, which memory
-// bounds, 727 and 720).
+// what costs (512 rows on 8,190 tokens: attention 141 us so, 150 without, accounts 88 and 97 with 32 rows a
+// wavefront; rows of 64 dimensions are half as many lines and attention takes 94 and 91, and 16 query
+// rows, which memory bounds, 727 and 720).
 template <int D, int MT>
-constexpr bool kStaged = D == 128 && MT == 2;
+constexpr bool kStaged = D == 128 && MT >= 2;
 typedef const __attribute__((address_space(1))) void* GlobalPtr;
 typedef __attribute__((address_space(3))) void* LdsPtr;
 
@@ -528,7 +528,7 @@ __device__ __forceinline__ void halve(float* v) {
 // accounts themselves.  A decode step is bound by reading K: 24 sequences of 500-8,100 tokens x 8 heads x
 // 128 (113 MB) 30 us, 3.8 TB/s.  A prompt's chunk is bound by the vector unit (exp2, the conversion of K,
 // q's pieces): 512 rows x 8 heads on 8,190 tokens x 4 heads x 64 (16.6 GFLOP) 50.5 us, of
-// which 5 are the join.
+// which 5 are the join; 512 rows x 4 heads on 8 heads x 128 (33.3 GFLOP) 76 us.
 template <int D, int FMT, int MT>
 __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(Cache8 c, Cache8Query q, int row_waves,
                                                              int groups, int chunks, float* part) {
@@ -718,10 +718,16 @@ int cache8_attend_launch(hipStream_t s, const Cache8& c, int head_dim, int forma
 
 // A row group a wavefront, as long as their sums fit 64 MiB.  With 16 rows about 8,192 wavefronts;
 // with more, which take longer to load (their q is cut into pieces), no more than the 2,048 that are
-// held at once (512 rows on 8,190 tokens 62 -> 51 us).  Each has four tiles or more.
+// held at once (512 rows on 8,190 tokens 62 -> 51 us).  Each has four tiles or more.  64 rows a wavefront
+// read K half as often as 32 and begin half as many times, which pays where there is work for all: from
+// 8 pairs of 64 rows and 64 tokens for each wavefront that is held with 128 dimensions (8 heads of 1,024
+// rows on 8,190 tokens 47.0 us, 51.3 with 32 rows; of 800: 57.4, 52.3) and from 4 with 64 (4 heads of
+// 1,024 rows 20.4, 22.3; of 256: 13.7, 10.6; a last group of 32 rows costs more so: 16 heads of 800 rows
+// on 4,000 tokens 37.7, 36.3).
 Cache8WeightsPlan cache8_weights_plan(const Cache8& c, int head_dim, int64_t rows, bool may_group) {
     Cache8WeightsPlan p;
-    p.row_tiles = rows <= 16 ? 1 : rows <= 32 || head_dim == 128 ? 2 : 4;
+    const int64_t pairs = (int64_t)c.n_seqs * c.kv * ((rows + 63) / 64) * (c.cap / kCacheTile);
+    p.row_tiles = rows <= 16 ? 1 : rows <= 32 || pairs < (head_dim == 128 ? 8 : 4) * 2048 ? 2 : 4;
     const int64_t per = 16 * p.row_tiles, all = std::max<int64_t>((rows + per - 1) / per, 1);
     const int64_t heads = (int64_t)c.n_seqs * c.kv, one = heads * c.cap;
     int64_t groups = may_group ? std::min(all, std::max<int64_t>((16ll << 20) / one, 1)) : 1;
@@ -743,7 +749,8 @@ int cache8_weights_launch(hipStream_t s, const Cache8& c, int head_dim, int form
            : p.row_tiles == 2 ? (i8 ? cache8_weights_kernel<64, kI8, 2> : cache8_weights_kernel<64, kE4M3, 2>)
                               : (i8 ? cache8_weights_kernel<64, kI8, 4> : cache8_weights_kernel<64, kE4M3, 4>))
         : (p.row_tiles == 1   ? (i8 ? cache8_weights_kernel<128, kI8, 1> : cache8_weights_kernel<128, kE4M3, 1>)
-                              : (i8 ? cache8_weights_kernel<128, kI8, 2> : cache8_weights_kernel<128, kE4M3, 2>));
+           : p.row_tiles == 2 ? (i8 ? cache8_weights_kernel<128, kI8, 2> : cache8_weights_kernel<128, kE4M3, 2>)
+                              : (i8 ? cache8_weights_kernel<128, kI8, 4> : cache8_weights_kernel<128, kE4M3, 4>));
     hipLaunchKernelGGL(kern, dim3(c.n_seqs * c.kv, (p.groups + p.row_waves - 1) / p.row_waves, p.workers),
                        dim3(256), 0, s, c, q, p.row_waves, p.groups, p.chunks, scratch);
     SHP_HIP_CHECK(hipGetLastError());

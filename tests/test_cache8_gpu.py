@@ -413,15 +413,8 @@ def test_results_do_not_change_from_call_to_call(ctx):
 
 # ---- accounts and eviction ------------------------------------------------------------------
 
-@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
-@pytest.mark.parametrize("d,kv,group,n,counts,lens", [
-    (64, 2, 8, 1, None, [300, 64]),
-    (64, 1, 3, 50, [50, 11], [130, 11]),
-    (128, 2, 4, 9, [0, 9], [77, 5]),
-    (128, 1, 1, 1, None, [1, 0])])
-def test_accounts(ctx, fmt, d, kv, group, n, counts, lens):
+def check_accounts(ctx, fmt, d, kv, group, n, counts, lens, cap):
     rng = np.random.default_rng(30 + n)
-    cap = 320
     with filled(ctx, rng, 2, kv, d, cap, 16, fmt, lens) as p:
         q = rows(rng, 2, n, kv * group, d)
         tq, tc = p.up(q), None if counts is None else p.up(counts, np.int32)
@@ -446,6 +439,24 @@ def test_accounts(ctx, fmt, d, kv, group, n, counts, lens):
             assert (got[s, :, ln:] == -3).all() and (bare[s, :, ln:] == -3).all()
             np.testing.assert_array_equal(place[s, :, ln:], start[s, :, ln:])
             np.testing.assert_array_equal(place[s, :, :ln], got[s, :, :ln])
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("d,kv,group,n,counts,lens", [
+    (64, 2, 8, 1, None, [300, 64]),
+    (64, 1, 3, 50, [50, 11], [130, 11]),
+    (128, 2, 4, 9, [0, 9], [77, 5]),
+    (128, 1, 1, 1, None, [1, 0])])
+def test_accounts(ctx, fmt, d, kv, group, n, counts, lens):
+    check_accounts(ctx, fmt, d, kv, group, n, counts, lens, 320)
+
+
+# a capacity of which so many tiles could be held that a wavefront takes 64 rows
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("d,n,counts,lens", [
+    (64, 67, [67, 30], [300, 65]), (128, 67, [67, 30], [300, 65]), (128, 100, None, [64, 129])])
+def test_accounts_of_many_rows_in_a_long_cache(ctx, fmt, d, n, counts, lens):
+    check_accounts(ctx, fmt, d, 2, 3, n, counts, lens, 65536)
 
 
 def evict_both(p, q, weights, keep, recent):
