@@ -187,12 +187,13 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 // out over workgroups while that fills the GPU.
 //
 // With up to 16 rows reading the cache bounds it: 16 x 128,001-131,072 tokens x 8 heads x 128 (4.2 GB)
-// 722 us, 5.9 TB/s, 24 sequences of 0-8,100 tokens 54 us, 3.7 TB/s (46 us where they are all as long as
+// 720 us, 5.9 TB/s, 24 sequences of 0-8,100 tokens 53 us, 3.8 TB/s (46 us where they are all as long as
 // the average); a single sequence of 300 tokens takes 5.8 us, which is latency.  With more rows the matrix
 // and vector units do, which take about as long: 512 rows x 4 heads on 8,190 tokens x 8 heads x 128
 // (66.6 GFLOP, twice that as products of pieces) 141 us, 945 TFLOP/s of products.
+// (Launch bounds: the wavefronts a SIMD that each variant reaches without spills.)
 template <int D, int FMT, int MT>
-__global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Query q, int least,
+__global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_attend_kernel(Cache8 c, Cache8Query q, int least,
                                                                float* part, int* counters) {
     constexpr int NO = D / 16;   // accumulators of 16 rows
     constexpr int PW = D + 4;    // floats of a row's part: sums, maximum, weight, two of padding
@@ -462,49 +463,72 @@ __global__ __launch_bounds__(256, 2) void cache8_attend_kernel(Cache8 c, Cache8Q
     if (threadIdx.x == 0)
         __hip_atomic_store((SHP_GLOBAL int*)(counters + unit), 0, __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
-    // factors 2^(m_i - m) of every share and row [splits][rows], then the rows' m and l
-    float* const factor = &ex[0][0];
-    float* const weight = factor + splits * rows;
-    float* const rm = weight + splits * rows;
-    for (int e = threadIdx.x; e < splits * rows; e += 256) {
-        const int i = e / rows, r = e - i * rows;
-        const float4 x = ld_coh16(pr, (unsigned)((i * ROWS + r) * PW + D) * 4u, 0);
-        factor[e] = x.x;
-        weight[e] = x.y;
+    // What the shares hold of the rows is on its way (B loads an output at a time) while their maxima and
+    // weights, a share to one of 32 lanes, give the factors 2^(m_i - m) and the rows' m and l.  The join is
+    // latency (64 rows x 4 heads of 8,190 tokens: 34.5 us in all with a row's shares one after the other and
+    // 8 loads on their way, 32.6 so; 4 rows of 8 sequences 18.4, 17.2).
+    constexpr int T = D / 4, NE = ROWS * T / 256, B = NE == 1 ? 16 : 8, NR = ROWS / 8;
+    float* const factor = &ex[0][0];        // [ROWS][32]
+    float* const total = factor + ROWS * 32;  // [ROWS][2]
+    const int tid = threadIdx.x, share_i = tid & 31;
+    float4 ml[NR], x[NE][B];
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+        const int r = (tid >> 5) + 8 * k;
+        ml[k] = make_float4(-__builtin_inff(), 0.f, 0.f, 0.f);
+        if (share_i < splits && r < rows)
+            ml[k] = ld_coh16(pr, (unsigned)((share_i * ROWS + r) * PW + D) * 4u, 0);
+    }
+    auto load = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+            if (i0 + i < splits)
+#pragma unroll
+                for (int n = 0; n < NE; ++n) {
+                    const int e = tid + 256 * n, r = min(e / T, rows - 1);
+                    x[n][i] = ld_coh16(pr, (unsigned)(((i0 + i) * ROWS + r) * PW + e % T * 4) * 4u, 0);
+                }
+    };
+    load(0);
+#pragma unroll
+    for (int k = 0; k < NR; ++k) {
+        float top = ml[k].x;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+        const float f = factor_of(ml[k].x, top);
+        float sum = ml[k].y * f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+        const int r = (tid >> 5) + 8 * k;
+        factor[r * 32 + share_i] = f;
+        if (share_i == 0) {
+            total[2 * r] = top;
+            total[2 * r + 1] = sum;
+        }
     }
     __syncthreads();
-    if ((int)threadIdx.x < rows) {
-        const int r = threadIdx.x;
-        float top = -__builtin_inff(), sum = 0.0f;
-        for (int i = 0; i < splits; ++i) top = fmaxf(top, factor[i * rows + r]);
-        for (int i = 0; i < splits; ++i) {
-            const float f = factor_of(factor[i * rows + r], top);
-            factor[i * rows + r] = f;
-            sum += weight[i * rows + r] * f;
-        }
-        rm[r] = top;
-        rm[rows + r] = sum;
+    f4 sum[NE];
+#pragma unroll
+    for (int n = 0; n < NE; ++n) sum[n] = f4{0.f, 0.f, 0.f, 0.f};
+    for (int i0 = 0; i0 < splits; i0 += B) {
+        if (i0) load(i0);
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+            if (i0 + i < splits)
+#pragma unroll
+                for (int n = 0; n < NE; ++n)
+                    sum[n] += f4{x[n][i].x, x[n][i].y, x[n][i].z, x[n][i].w} *
+                              factor[(tid + 256 * n) / T * 32 + i0 + i];
     }
-    __syncthreads();
-    constexpr int T = D / 4;
-    for (int e = threadIdx.x; e < rows * T; e += 256) {
-        const int r = e / T, d = e % T * 4;
-        f4 sum = {0.f, 0.f, 0.f, 0.f};
-        for (int i0 = 0; i0 < splits; i0 += 8) {  // eight loads in flight
-            float4 x[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                x[i] = ld_coh16(pr, (unsigned)((min(i0 + i, splits - 1) * ROWS + r) * PW + d) * 4u, 0);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (i0 + i < splits)
-                    sum += f4{x[i].x, x[i].y, x[i].z, x[i].w} * factor[(i0 + i) * rows + r];
-        }
+    for (int n = 0; n < NE; ++n) {
+        const int e = tid + 256 * n, r = e / T, d = e % T * 4;
+        if (r >= rows) continue;
         int64_t at, at_lse;
         place(r0 + r, at, at_lse);
-        const float total = rm[rows + r];
-        *reinterpret_cast<f4*>(q.out + at + d) = sum * (total == 0.0f ? 0.0f : 1.0f / total);
-        if (q.lse && d == 0) q.lse[at_lse] = log_sum(rm[r], total);
+        const float all = total[2 * r + 1];
+        *reinterpret_cast<f4*>(q.out + at + d) = sum[n] * (all == 0.0f ? 0.0f : 1.0f / all);
+        if (q.lse && d == 0) q.lse[at_lse] = log_sum(total[2 * r], all);
     }
 }
 
@@ -683,17 +707,28 @@ namespace shp {
 Cache8Plan cache8_attend_plan(const Cache8& c, int head_dim, int64_t rows, int cu_count,
                               bool may_split) {
     Cache8Plan p;
-    p.row_tiles = rows <= 16 ? 1 : 2;
+    // 32 rows a workgroup use each tile for twice the work, 16 leave room for more workgroups on a CU.
+    // 32 pay where there is much of both, from 32 pairs of 32 rows and 64 tokens a CU with 128 dimensions
+    // (64 rows x 4 heads on 8,190 tokens x 8 heads 32.6 us, 36.5 with 16 rows; 40: 36.8, 34.5; 16: 23.7,
+    // 19.7) and 128 with 64, whose tiles cost half (512 rows x 8 heads on 8,190 tokens x 4 heads 90 us, 102;
+    // 192: 55, 47; 128: 32, 34; 32 on 600 tokens 11.7, 8.7); and with 128 where blocks of 16 do not find
+    // room at once, three on a CU (prompts of 500 x 4 x 8 heads 16.9 us, 21.4; of 350: 16.0, 12.7).
+    const int64_t cu = std::max(cu_count, 1), heads = (int64_t)c.n_seqs * c.kv;
+    const int64_t pairs = heads * ((rows + 31) / 32) * (c.cap / kCacheTile);
+    const bool many = head_dim == 64 ? pairs >= 128 * cu
+                                     : pairs >= 32 * cu || heads * ((rows + 15) / 16) > 3 * cu;
+    p.row_tiles = rows > 16 && many ? 2 : 1;
     const int64_t per = 16 * p.row_tiles;
     p.row_blocks = (int)((rows + per - 1) / per);
-    // Workgroups for 8 on every CU with 16 rows, which evens out sequences of different length (64 x
-    // 3,000-6,000 tokens: 123 us, 134 with 4 and 127 with 16 a CU), and for the two that it holds at
-    // once with 32 (64 rows x 4 heads: 35 us, 44 with 4 a CU, 42 with one).  A workgroup takes two
-    // tiles a wavefront or more (300 tokens 5.8 us, 7.0 from one tile; 4 rows of 8 sequences 18.4, 25.8),
-    // a sequence 32 shares at most, whose parts one workgroup joins (32,000 tokens 24.6 us with 32, 29.9
-    // with 16).
-    const int64_t units = (int64_t)c.n_seqs * c.kv * p.row_blocks;
-    const int64_t want = ((p.row_tiles == 2 ? 2 : 8) * (int64_t)std::max(cu_count, 1) + units - 1) / units;
+    // Workgroups for 8 on every CU where a head has no more than 16 rows, which evens out sequences of
+    // different length (64 x 3,000-6,000 tokens: 123 us, 134 with 4 and 127 with 16 a CU); for 3 with
+    // more blocks of 16 (8 rows x 4 heads of 8 sequences on 4,000 tokens 25.6, 28.6 with 5), and for the
+    // two that a CU holds at once with 32 (64 rows x 4 heads: 44 us with 4 a CU, 42 with one, where two
+    // took 35).  A workgroup takes two tiles a wavefront or more (300 tokens 5.8 us, 7.1 from one tile; 4
+    // rows of 8 sequences 17.2, 23.8; 1,000 tokens 8.3, 7.3), a sequence 32 shares at most, whose parts one
+    // workgroup joins (32,000 tokens 24.6 us with 32, 29.9 with 16).
+    const int64_t units = heads * p.row_blocks;
+    const int64_t want = ((p.row_tiles == 2 ? 2 : p.row_blocks > 1 ? 3 : 8) * cu + units - 1) / units;
     p.least = 8;
     const int64_t most = (c.cap / kCacheTile + p.least - 1) / p.least;
     p.splits = (int)std::max<int64_t>(std::min<int64_t>(std::min(want, most), 32), 1);

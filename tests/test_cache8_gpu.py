@@ -272,6 +272,27 @@ def test_attention(ctx, fmt, d, kv, group, n, block, lens):
         p.check_attend(rows(rng, 2, n, kv * group, d))
 
 
+# So many pairs of rows and tiles, by the capacity, that a workgroup takes 32 rows; their tokens in one
+# share or several.
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("d,kv,group,n,counts,lens", [
+    (64, 4, 4, 64, None, [70]),
+    (64, 4, 4, 61, [59], [1500]),
+    (128, 2, 4, 33, [33], [1234]),
+    (128, 2, 3, 43, None, [40])])
+def test_attention_of_many_rows_in_a_long_cache(ctx, fmt, d, kv, group, n, counts, lens):
+    rng = np.random.default_rng(17 + n)
+    with filled(ctx, rng, 1, kv, d, 65536, 32, fmt, lens, spread=0.3) as p:
+        p.check_attend(rows(rng, 1, n, kv * group, d), counts=counts)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+def test_attention_of_prompts_that_fill_the_gpu(ctx, fmt):
+    rng = np.random.default_rng(16)
+    with filled(ctx, rng, 5, 8, 128, 128, 64, fmt, [90, 128, 3, 85, 0]) as p:
+        p.check_attend(rows(rng, 5, 90, 32, 128), counts=[90, 88, 90, 1, 7])
+
+
 def test_attention_of_padded_rows(ctx):
     rng = np.random.default_rng(12)
     with filled(ctx, rng, 4, 2, 64, 256, 32, "e4m3", [100, 256, 5, 0]) as p:
