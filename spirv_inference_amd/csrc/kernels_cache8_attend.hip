@@ -128,11 +128,11 @@ __device__ __forceinline__ void load_k(const uint8_t* tile, u4 raw[4][D / 64]) {
         for (int a = 0; a < D / 64; ++a)
             raw[j][a] = *reinterpret_cast<const u4*>(p + 4 * j * D + 64 * a);
 }
-// K's tiles of 128 dimensions go through LDS where 32 rows or more share one: lanes 0 to 15 of load_k read 16
-// bytes each of 16 rows, 16 cache lines, and tiles that many rows want come from L2, where that is
-// what costs (512 rows on 8,190 tokens: attention 141 us so, 150 without, accounts 88 and 97 with 32 rows a
-// wavefront; rows of 64 dimensions are half as many lines and attention takes 94 and 91, and 16 query
-// rows, which memory bounds, 727 and 720).
+// K's tiles of 128 dimensions go through LDS where 32 rows or more share one: lanes 0 to 15 of load_k
+// read 16 bytes each of 16 rows, 16 cache lines, and tiles that many rows want come from L2, where that
+// is what costs (512 rows on 8,190 tokens: attention 141 us so, 150 without, accounts 88 and 97 with 32
+// rows a wavefront; rows of 64 dimensions are half as many lines and attention takes 94 and 91, and 16
+// query rows, which memory bounds, 727 and 720).
 template <int D, int MT>
 constexpr bool kStaged = D == 128 && MT >= 2;
 typedef const __attribute__((address_space(1))) void* GlobalPtr;
