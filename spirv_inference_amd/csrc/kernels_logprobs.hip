@@ -44,10 +44,12 @@ struct Sums {
     float m, z, x;
 };
 
-// Adds a part to sums whose maximum is t.m already.
+// Adds a part to sums whose maximum is t.m already.  Of a part that holds nothing but the type's lowest
+// numbers d * z would be minus infinity and f zero: d stays where their product is finite for every
+// length of a row, which also leaves alone what holds nothing but minus infinity (z is 0, and d may be
+// a NaN).  Logits that are plus infinity or NaN are in z and x.
 __device__ __forceinline__ void add_part(Sums& t, float m, float z, float x) {
-    if (z == 0.0f) return;  // nothing but minus infinity
-    const float d = m - t.m, f = __builtin_amdgcn_exp2f(d * kLog2e);
+    const float d = fmaxf(m - t.m, -1e28f), f = __builtin_amdgcn_exp2f(d * kLog2e);
     t.z += z * f;
     t.x += (x + d * z) * f;
 }

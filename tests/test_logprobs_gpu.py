@@ -108,6 +108,39 @@ def test_infinities_and_nan(ctx, vocab):
     check(run(ctx, x, t, 10), x, t, 10)
 
 
+# What is masked: a part of its own for the join, whole chunks at either end, the logits of one
+# wavefront of a chunk, all but one logit.
+MASKED = [(1, 40000, lambda i: i >= 32768), (3, 100000, lambda i: i < 70000),
+          (1, 32000, lambda i: i // 4 % 1024 // 64 == 5), (300, 20000, lambda i: i >= 9000),
+          (300, 20000, lambda i: i < 9000), (300, 20000, lambda i: i // 4 % 256 // 64 == 2),
+          (1030, 9000, lambda i: i >= 4100), (1030, 9000, lambda i: i < 4100),
+          (2, 50, lambda i: i != 17), (2, 40000, lambda i: i != 35000)]
+
+
+@pytest.mark.parametrize("case", range(len(MASKED)))
+@pytest.mark.parametrize("fill", [-3.4028235e38, -1e38, -2e9])
+def test_masks_of_very_negative_numbers(ctx, case, fill):
+    """Finite logits whose weight is zero: parts of a row that hold nothing else add nothing."""
+    rows, vocab, masked = MASKED[case]
+    rng = np.random.default_rng(case)
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    x[:, masked(np.arange(vocab))] = fill
+    t = rng.integers(0, vocab, rows)
+    for top in (0, 5):
+        check(run(ctx, x, t, top), x, t, top)
+
+
+@pytest.mark.parametrize("rows,vocab", [(2, 40000), (300, 20000)])
+def test_a_nan_among_very_negative_numbers_shows(ctx, rows, vocab):
+    rng = np.random.default_rng(13)
+    x = rng.standard_normal((rows, vocab)).astype(np.float32)
+    x[:, 9000:] = -3.4028235e38
+    x[::2, vocab - 5] = np.nan
+    x[1, 9000:] = -np.inf
+    t = rng.integers(0, vocab, rows)
+    check(run(ctx, x, t, 3), x, t, 3)
+
+
 def test_large_common_offsets_cancel(ctx):
     rng = np.random.default_rng(7)
     x = (rng.integers(-40, 40, (4, 5000)) * 0.25 + np.array([[1e5], [-1e5], [0], [3e6]])).astype(np.float32)
