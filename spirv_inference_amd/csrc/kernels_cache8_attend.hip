@@ -13,9 +13,14 @@
 // the lane's 16 bytes of a dimension of V stand for in O^T = V^T P^T.  So K and V go from memory to
 // the matrix cores without LDS, in 16-byte loads (but see stage_k), and P never leaves its registers.
 //
-// With u_t = log2 of (weight * scale of V), the running maximum m is taken over u, and
-// w_t = 2^(u_t - m + 12) is what multiplies V's codes: it spans fp16's range whatever the scales
-// are, and the row's sum is that of w_t / scale.
+// A row keeps the maximum m of its scores (in units of log2, rounded up to a whole number) and the sum
+// of the weights e_t = 2^(score - m), in which V has no part.  What multiplies V's codes is w_t = e_t *
+// (scale of V) * 2^(12 - k), k being the running maximum, rounded up, of log2(e_t * scale of V): the
+// largest w_t of a row fill fp16's range whatever the scales are.  A token whose e_t * scale is 2^15
+// times smaller than the row's largest has fewer bits of w_t, and one 2^37 times smaller none.
+// (A single maximum, over log2(weight * scale), with the row's sum made of w_t / scale, is wrong where
+// scales lie more than about 2^130 apart: the weight of the tokens with small values is lost.)  Scaling
+// is by powers of two, which rounds nothing, and seldom: a maximum has to pass a whole number.
 #include "cache8.h"
 #include "coherent.h"
 #include "gemm.h"
@@ -33,8 +38,12 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kLift = 12.0f;  // weights reach 2^12: the low piece stays a normal fp16 number longer
-constexpr float kLargeScore = 262144.0f;  // |m| past which the rounding of m matters to a weight
+constexpr int kLift = 12;  // w reaches 2^12: the low piece stays a normal fp16 number longer
+constexpr int kRoom = 24;  // log2 of the room for sums of V over tokens
+constexpr float kLargeScore = 262144.0f;  // |m| past which the rounding of a score shows in a weight
+constexpr float kNoWeight = -126.0f;  // log2 of the smallest weight that counts: normal fp32 numbers
+constexpr float kLeastLift = -114.0f;  // ... and that k follows, so that 2^(12 - k) * scale stays finite
+constexpr float kNoValues = -1000.0f;  // k before the first token: below all that it can be
 constexpr int kQBits = 14;      // a row of q is scaled to reach 2^13 .. 2^14
 
 // Four codes as fp16 numbers.
@@ -65,9 +74,19 @@ __device__ __forceinline__ void pieces(float x, float y, h2& hi, h2& lo) {
     lo = __builtin_convertvector(f2{x - (float)hi.x, y - (float)hi.y}, h2);
 }
 
+// f over the lane groups of 16, for every lane: two exchanges of rows of 16 and of 32 lanes.
+template <class F>
+__device__ __forceinline__ float over_groups(float x, F f) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
 __device__ __forceinline__ float max_over_groups(float x) {
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
+    return over_groups(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float sum_over_groups(float x) {
+    return over_groups(x, [](float a, float b) { return a + b; });
 }
 
 // A KV head of a sequence and its query rows.
@@ -174,9 +193,14 @@ __device__ __forceinline__ float factor_of(float m, float top) {
     return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
 }
 
-// The log of a row's sum from its maximum and weight as the wavefronts keep them.
+// What sums of weights times V are to be multiplied by, from the sum of the weights.
+__device__ __forceinline__ float inverse(float l) {
+    return l == 0.0f ? 0.0f : (float)(1 << kRoom) / l;
+}
+
+// The log of a row's sum from its maximum and sum of weights as the wavefronts keep them.
 __device__ __forceinline__ float log_sum(float m, float l) {
-    return l == 0.0f ? -__builtin_inff() : (m - kLift + __builtin_amdgcn_logf(l)) * kLn2;
+    return l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
 // A workgroup's four wavefronts hold the same rows and take a tile each in turn; their parts meet in LDS
@@ -245,7 +269,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
         vs = c.v_scale[b];
     };
 
-    float m[MT], l[MT], back[MT];
+    float m[MT], l[MT], k[MT], back[MT];
     int limit[MT];
     f4 o[MT][NO];
     h8 qh[MT][D / 32], ql[MT][D / 32];
@@ -254,6 +278,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
         load_q<D>(q, p, r0 + 16 * t + li, qh[t], ql[t], back[t], limit[t]);
         m[t] = -__builtin_inff();
         l[t] = 0.0f;
+        k[t] = kNoValues;
 #pragma unroll
         for (int d = 0; d < NO; ++d) o[t][d] = f4{0.f, 0.f, 0.f, 0.f};
     }
@@ -285,12 +310,11 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
             }
         }
         // sc[t][j][i]: token t0 + 16 g + 4 j + i, row r0 + 16 t + li
-        const float kscale = ks, vscale = vs < kScaleFloor ? kScaleFloor : vs;
-        const float lv = __builtin_amdgcn_logf(vscale);
+        const float ve = (float)__builtin_amdgcn_frexp_expf(vs);  // V's scale is under 2^ve
         h8 wh[MT][2], wl[MT][2];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const float f = kscale * back[t];
+            const float f = ks * back[t];
             float mx = -__builtin_inff();
             if (edge) {
 #pragma unroll
@@ -303,17 +327,28 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) mx = fmaxf(mx, sc[t][j][i]);
-            const float top = fmaxf(m[t], max_over_groups(__builtin_fmaf(mx, f, lv)));
-            if (__any(top > m[t])) {
-                const float down = factor_of(m[t], top);
-                l[t] *= down;
-#pragma unroll
-                for (int d = 0; d < NO; ++d) o[t][d] *= down;
+            // the best of the lane's 16 tokens (rounded: not to be fused with what it is compared with)
+            const float best = __builtin_fmaf(mx, f, 0.0f);
+            if (__any(best > m[t])) {
+                const float top = fmaxf(m[t], __builtin_ceilf(max_over_groups(best)));
+                const float step = m[t] == top ? 0.0f : m[t] - top;
+                l[t] *= __builtin_amdgcn_exp2f(step);
+                k[t] = fmaxf(k[t] + step, kNoValues);
                 m[t] = top;
             }
-            // u - m as one fused step; where u is so large that the rounding of m would show (a
-            // weight of more than 2^12, or none), u is rounded as m was
-            const float at = lv + kLift - m[t];
+            const float e = best - m[t];
+            const bool on = e >= kNoWeight;  // not where the row sees none of the 16
+            const float u = on ? fmaxf(e, kLeastLift) + ve : kNoValues;
+            if (__any(u > k[t])) {
+                const float top = fmaxf(k[t], __builtin_ceilf(max_over_groups(u)));
+                const float down = __builtin_amdgcn_exp2f(k[t] - top);
+#pragma unroll
+                for (int d = 0; d < NO; ++d) o[t][d] *= down;
+                k[t] = top;
+            }
+            const float lift = on ? __builtin_amdgcn_ldexpf(vs, kLift - (int)k[t]) : 0.0f;
+            // score - m as one fused step; where scores are so large that their rounding would show
+            // (a weight of 2^12, or none), rounded as the maximum was
             const bool large = fabsf(m[t]) > kLargeScore;
             float sum = 0.0f;
             if (edge || __any(large)) {
@@ -322,17 +357,17 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float x = sc[t][j][i];
-                        const float u = large ? __builtin_fmaf(x, f, lv) - m[t] + kLift
-                                              : __builtin_fmaf(x, f, at);
+                        const float y = large ? __builtin_fmaf(x, f, 0.0f) - m[t]
+                                              : __builtin_fmaf(x, f, -m[t]);
                         sc[t][j][i] = t0 + 16 * g + 4 * j + i < limit[t]
-                                          ? __builtin_amdgcn_exp2f(u) : 0.0f;
+                                          ? __builtin_amdgcn_exp2f(y) : 0.0f;
                     }
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        sc[t][j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j][i], f, at));
+                        sc[t][j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][j][i], f, -m[t]));
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -341,7 +376,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     h2 ph, pl;
-                    pieces(sc[t][j][2 * i], sc[t][j][2 * i + 1], ph, pl);
+                    pieces(sc[t][j][2 * i] * lift, sc[t][j][2 * i + 1] * lift, ph, pl);
                     const int e = 4 * (j & 1) + 2 * i;
                     wh[t][j >> 1][e] = ph.x;
                     wh[t][j >> 1][e + 1] = ph.y;
@@ -349,7 +384,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
                     wl[t][j >> 1][e + 1] = pl.y;
                 }
             }
-            if (sum != 0.0f) l[t] += sum / vscale;  // of a block nobody sees, the scale may be NaN
+            l[t] += sum;
         }
         if (FMT == kE4M3 && t0 + kCacheTile > p.len) {
             // bytes behind the last token may be NaN codes, which a weight of zero does not cancel
@@ -372,12 +407,21 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
                     o[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, wh[t][e], o[t][d], 0, 0, 0);
                 }
             }
+            // a dimension after the other: what else is begun early does not find registers
+            if constexpr (STAGED) __builtin_amdgcn_sched_barrier(0);
         }
     }
+    // the lane's numbers once more, which the loop's registers need not hold so
+    const int ln = __lane_id(), row = ln & 15, quad = ln >> 4, tid = wave * 64 + ln;
+    // the sums of the tokens' weights times V, 2^24 times smaller: with 4,194,304 tokens they are finite
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
-        l[t] += __shfl_xor(l[t], 16);
-        l[t] += __shfl_xor(l[t], 32);
+        l[t] = sum_over_groups(l[t]);
+#pragma unroll
+        for (int d = 0; d < NO; ++d)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                o[t][d][i] = __builtin_amdgcn_ldexpf(o[t][d][i], (int)k[t] - kLift - kRoom);
     }
 
     // the wavefronts' parts, in pairs: the upper one's goes through LDS
@@ -390,16 +434,16 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
             for (int t = 0; t < MT; ++t) {
 #pragma unroll
                 for (int d = 0; d < NO; ++d)
-                    *reinterpret_cast<f4*>(&x[((t * NO + d) * 64 + lane) * 4]) = o[t][d];
-                x[(MT * NO * 4 + 2 * t) * 64 + lane] = m[t];
-                x[(MT * NO * 4 + 2 * t + 1) * 64 + lane] = l[t];
+                    *reinterpret_cast<f4*>(&x[((t * NO + d) * 64 + ln) * 4]) = o[t][d];
+                x[(MT * NO * 4 + 2 * t) * 64 + ln] = m[t];
+                x[(MT * NO * 4 + 2 * t + 1) * 64 + ln] = l[t];
             }
         __syncthreads();
         if (wave < step)
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                const float m1 = x[(MT * NO * 4 + 2 * t) * 64 + lane];
-                const float l1 = x[(MT * NO * 4 + 2 * t + 1) * 64 + lane];
+                const float m1 = x[(MT * NO * 4 + 2 * t) * 64 + ln];
+                const float l1 = x[(MT * NO * 4 + 2 * t + 1) * 64 + ln];
                 const float top = fmaxf(m[t], m1);
                 const float f0 = factor_of(m[t], top), f1 = factor_of(m1, top);
                 l[t] = l[t] * f0 + l1 * f1;
@@ -407,7 +451,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
 #pragma unroll
                 for (int d = 0; d < NO; ++d)
                     o[t][d] = o[t][d] * f0 +
-                              *reinterpret_cast<const f4*>(&x[((t * NO + d) * 64 + lane) * 4]) * f1;
+                              *reinterpret_cast<const f4*>(&x[((t * NO + d) * 64 + ln) * 4]) * f1;
             }
         __syncthreads();
     }
@@ -422,15 +466,15 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
         if (wave) return;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const int r = r0 + 16 * t + li;
+            const int r = r0 + 16 * t + row;
             if (r >= p.rows) continue;
             int64_t at, at_lse;
             place(r, at, at_lse);
-            const float inv = l[t] == 0.0f ? 0.0f : 1.0f / l[t];
+            const float inv = inverse(l[t]);
 #pragma unroll
             for (int d = 0; d < NO; ++d)
-                *reinterpret_cast<f4*>(q.out + at + 16 * d + 4 * g) = o[t][d] * inv;
-            if (q.lse && g == 0) q.lse[at_lse] = log_sum(m[t], l[t]);
+                *reinterpret_cast<f4*>(q.out + at + 16 * d + 4 * quad) = o[t][d] * inv;
+            if (q.lse && quad == 0) q.lse[at_lse] = log_sum(m[t], l[t]);
         }
         return;
     }
@@ -443,34 +487,34 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
     if (wave == 0) {
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const int r = 16 * t + li;
+            const int r = 16 * t + row;
             if (r >= rows) continue;
             const unsigned at = (unsigned)(((int)blockIdx.z * ROWS + r) * PW) * 4u;
 #pragma unroll
             for (int d = 0; d < NO; ++d)
-                st_coh16(pr, at + (16 * d + 4 * g) * 4u,
+                st_coh16(pr, at + (16 * d + 4 * quad) * 4u,
                          make_float4(o[t][d].x, o[t][d].y, o[t][d].z, o[t][d].w));
-            if (g == 0) st_coh16(pr, at + D * 4u, make_float4(m[t], l[t], 0.f, 0.f));
+            if (quad == 0) st_coh16(pr, at + D * 4u, make_float4(m[t], l[t], 0.f, 0.f));
         }
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's parts are stored
     __syncthreads();
-    if (threadIdx.x == 0)
+    if (tid == 0)
         arrived = __hip_atomic_fetch_add((SHP_GLOBAL int*)(counters + unit), 1, __ATOMIC_RELAXED,
                                          __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     if (arrived != splits - 1) return;
-    if (threadIdx.x == 0)
+    if (tid == 0)
         __hip_atomic_store((SHP_GLOBAL int*)(counters + unit), 0, __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
     // What the shares hold of the rows is on its way (B loads an output at a time) while their maxima and
-    // weights, a share to one of 32 lanes, give the factors 2^(m_i - m) and the rows' m and l.  The join is
+    // sums, a share to one of 32 lanes, give the factors 2^(m_i - m) and the rows' m and l.  The join is
     // latency (64 rows x 4 heads of 8,190 tokens: 34.5 us in all with a row's shares one after the other and
     // 8 loads on their way, 32.6 so; 4 rows of 8 sequences 18.4, 17.2).
     constexpr int T = D / 4, NE = ROWS * T / 256, B = NE == 1 ? 16 : 8, NR = ROWS / 8;
     float* const factor = &ex[0][0];        // [ROWS][32]
     float* const total = factor + ROWS * 32;  // [ROWS][2]
-    const int tid = threadIdx.x, share_i = tid & 31;
+    const int share_i = tid & 31;
     float4 ml[NR], x[NE][B];
 #pragma unroll
     for (int k = 0; k < NR; ++k) {
@@ -527,7 +571,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
         int64_t at, at_lse;
         place(r0 + r, at, at_lse);
         const float all = total[2 * r + 1];
-        *reinterpret_cast<f4*>(q.out + at + d) = sum[n] * (all == 0.0f ? 0.0f : 1.0f / all);
+        *reinterpret_cast<f4*>(q.out + at + d) = sum[n] * inverse(all);
         if (q.lse && d == 0) q.lse[at_lse] = log_sum(total[2 * r], all);
     }
 }

@@ -329,6 +329,44 @@ def test_attention_where_scales_differ_by_many_orders(ctx, fmt):
         p.check_attend(q, scale=0.5)
 
 
+# Blocks of 16 tokens whose V is all zeros (the smallest scale, 2^-60) or 1e-12 beside blocks of very
+# large V: in one tile, in the tiles of different wavefronts, in the shares of different workgroups.
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("huge", [1e24, 1e30, 3e38])
+@pytest.mark.parametrize("small", [0.0, 1e-12])
+@pytest.mark.parametrize("n,length,run", [(1, 32, 16), (1, 128, 64), (40, 320, 16), (1, 2000, 1024)])
+def test_attention_weighs_tokens_whatever_their_values(ctx, fmt, d, huge, small, n, length, run):
+    """Tokens of all magnitudes share the weight; how large a value is does not change its weight."""
+    rng = np.random.default_rng(21)
+    k, v = rows(rng, 1, length, 1, d), rng.uniform(-1, 1, (1, length, 1, d))
+    v = v * np.where(np.arange(length) // run % 2, huge, small)[None, :, None, None]
+    with Pair(ctx, 1, 1, d, -(-length // 128) * 128, 16, fmt) as p:
+        p.append(k, v.astype(np.float32), [length])
+        p.check_attend(rows(rng, 1, n, 2, d))
+        p.check_attend(np.zeros((1, n, 2, d), np.float32))
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("gap", [60.0, 80.0, 86.0])
+@pytest.mark.parametrize("length,run", [(32, 16), (128, 64), (2000, 1024)])
+def test_attention_of_large_values_with_little_weight(ctx, fmt, gap, length, run):
+    """Weights of e^-60 to e^-86 on values of 1e36 beside weights of one on values of 0.01 and zero."""
+    rng = np.random.default_rng(22)
+    big = np.arange(length) // run % 2 == 1
+    k = np.zeros((1, length, 1, 64), np.float32)
+    k[0, big, 0, 0] = -1.0
+    v = rng.uniform(0.5, 1, (1, length, 1, 64))
+    v[0, ~big] *= 0.01
+    v[0, big] *= 1e36
+    v[0, :8] = 0.0
+    with Pair(ctx, 1, 1, 64, -(-length // 128) * 128, 16, fmt) as p:
+        p.append(k, v.astype(np.float32), [length])
+        q = np.zeros((1, 1, 4, 64), np.float32)
+        q[..., 0] = gap
+        p.check_attend(q, scale=1.0)
+
+
 def test_attention_of_zero_tiny_and_huge_queries(ctx):
     rng = np.random.default_rng(15)
     with filled(ctx, rng, 1, 1, 64, 128, 32, "i8", [100]) as p:
