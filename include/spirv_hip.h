@@ -210,8 +210,9 @@ int shp_cache8_read(shp_ctx* ctx, const shp_cache8* cache, int32_t n, float* k, 
  * with V a token whose weight times V's scale is 2^15 times smaller than the row's largest has fewer,
  * and one 2^37 times smaller none (its weight counts in the sum and in lse all the same).
  * The tokens are split over workgroups whose partial results go through the context's workspace;
- * it grows on an eager call that needs more, and a captured call that finds it too small runs
- * without the split: run the call once before it is captured. */
+ * it grows on an eager call that needs more, to twice its size at least, which the host waits for, and
+ * a captured call that finds it too small runs without the split: run the call once before it is
+ * captured. */
 typedef struct shp_cache8_attend_args {
     const float* q;
     float* out;

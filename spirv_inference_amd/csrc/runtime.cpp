@@ -111,8 +111,17 @@ Ctx::~Ctx() {
 
 int Ctx::ensure_workspace(size_t bytes) {
     if (bytes <= workspace_bytes) return SHP_OK;
+    // Twice the old size at least: the buffers that are kept below then stay smaller together than the
+    // one in use, however slowly the calls of a program grow.
+    const size_t least = bytes;
+    bytes = std::max(bytes, 2 * workspace_bytes);
     float* grown = nullptr;
-    SHP_HIP_CHECK(hipMalloc((void**)&grown, bytes));
+    if (bytes > least && hipMalloc((void**)&grown, bytes) != hipSuccess) {
+        (void)hipGetLastError();
+        bytes = least;  // where only this much is left
+        grown = nullptr;
+    }
+    if (!grown) SHP_HIP_CHECK(hipMalloc((void**)&grown, bytes));
     // The old buffer may be baked into a captured hipGraph (a model's or the caller's):
     // keep it alive until the context goes away.
     if (workspace) retired.push_back(workspace);

@@ -3,12 +3,15 @@
 Bounds: x - m is rounded once (2^-24 of its size), the sums of exp(x - m) over a row are off by
 under 64 roundings relative to themselves plus 2^-23 of |x - m| per weight, which stays under 2^-23 *
 max over weights of exp(d) |d| < 2^-23; logf and the last differences add roundings of their own size."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
 import cache8_ref as R
 from conftest import assert_close
 from spirv_inference_amd import Context, DeviceTensor, ShpError
+from spirv_inference_amd._lib import lib
 from spirv_inference_amd.models import Llama
 
 pytestmark = pytest.mark.gpu
@@ -220,6 +223,23 @@ def test_captured_calls(ctx):
             check((lp.download(), ent.download(), ids.download().reshape(rows, top),
                    tops.download().reshape(rows, top)), v, [3, 4], top)
         g.destroy()
+
+
+def test_the_workspace_grows_seldom():
+    """Outgrown buffers live as long as their context (a graph may hold them): calls that grow one row
+    at a time leave few of them, smaller together than the one in use."""
+    vocab = 70001
+    with Context("any") as own:
+        x, tg, lp = own.empty(255 * vocab), own.tensor(np.zeros(255), np.int32), own.empty(255)
+        seen = {}
+        for rows in range(1, 256):
+            own.token_logprobs(x, tg, lp, None, None, None, rows, vocab)
+            ptr, size = C.c_void_p(), C.c_uint64()
+            assert lib().shp_workspace_info(own.handle, C.byref(ptr), C.byref(size)) == 0
+            seen[ptr.value] = size.value
+        own.sync()
+        sizes = sorted(seen.values())
+        assert sum(sizes[:-1]) <= sizes[-1] and len(sizes) < 10, sizes
 
 
 # ---- the decoder scores a text -----------------------------------------------------------------
