@@ -42,28 +42,39 @@ class Cache8:
             raise ValueError(f"format {fmt!r}: one of {', '.join(FORMATS)} is needed")
         if block not in (16, 32, 64, 128):
             raise ValueError(f"blocks of {block} tokens: 16, 32, 64 or 128 are needed")
+        if head_dim not in (64, 128):
+            raise ValueError(f"head_dim {head_dim}: 64 or 128 is needed")
+        if n_seqs < 1 or n_kv_heads < 1 or n_seqs * n_kv_heads > 65535:
+            raise ValueError(f"{n_seqs} sequences of {n_kv_heads} heads: 1 to 65535 heads of all "
+                             "sequences together are needed")
+        if not 0 < capacity <= 1 << 22 or capacity % 64 or capacity % block:
+            raise ValueError(f"capacity {capacity}: a multiple of 64 and of block is needed, "
+                             "4194304 at most")
         self.ctx = ctx
         self.n_seqs, self.n_kv_heads, self.head_dim = n_seqs, n_kv_heads, head_dim
         self.capacity, self.block, self.fmt = capacity, block, fmt
-        n, scales = n_seqs * n_kv_heads * capacity, n_seqs * n_kv_heads * capacity // block
-        self._own = []
-
-        def have(t, size, dtype):
-            if t is None:
-                t = DeviceTensor(ctx, size, dtype)
-                self._own.append(t)
-            elif t.nbytes < size * np.dtype(dtype).itemsize:
+        n = n_seqs * n_kv_heads * capacity
+        # the arrays that are given are looked at before any is allocated
+        arrays = {"k": (k, n * head_dim, np.uint8), "v": (v, n * head_dim, np.uint8),
+                  "k_scale": (k_scale, n // block, np.float32),
+                  "v_scale": (v_scale, n // block, np.float32), "lengths": (lengths, n_seqs, np.int32)}
+        for t, size, dtype in arrays.values():
+            if t is not None and t.nbytes < size * np.dtype(dtype).itemsize:
                 raise ValueError(f"an array of {t.nbytes} bytes where the cache needs "
                                  f"{size * np.dtype(dtype).itemsize}")
-            return t
-
-        self.k, self.v = have(k, n * head_dim, np.uint8), have(v, n * head_dim, np.uint8)
-        self.k_scale = have(k_scale, scales, np.float32)
-        self.v_scale = have(v_scale, scales, np.float32)
-        given = lengths is not None
-        self.lengths = have(lengths, n_seqs, np.int32)
-        if not given:
-            self.lengths.upload(np.zeros(n_seqs, np.int32))
+        self._own = []
+        try:
+            for name, (t, size, dtype) in arrays.items():
+                if t is None:
+                    t = DeviceTensor(ctx, size, dtype)
+                    self._own.append(t)
+                setattr(self, name, t)
+            if lengths is None:
+                self.lengths.upload(np.zeros(n_seqs, np.int32))
+        except BaseException:  # nobody gets an object to close
+            for t in self._own:
+                t.free()
+            raise
         self._struct = Cache8Struct(self.k.ptr, self.v.ptr, self.k_scale.ptr, self.v_scale.ptr,
                                     self.lengths.ptr, n_seqs, n_kv_heads, head_dim, capacity,
                                     block, FORMATS[fmt])

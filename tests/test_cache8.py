@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import cache8_ref as R
-from spirv_inference_amd import Cache8, _lib
+from spirv_inference_amd import Cache8, _lib, cache8
 from spirv_inference_amd._lib import (Cache8AppendArgs, Cache8AttendArgs, Cache8EvictArgs,
                                       Cache8Struct, Cache8WeightsArgs, LogprobsArgs)
 
@@ -174,6 +174,42 @@ def test_the_mirror_refuses_unknown_formats_and_blocks():
     for block in (0, 8, 48, 256):
         with pytest.raises(ValueError, match="16, 32, 64 or 128"):
             Cache8(None, 1, 1, 64, 64, block=block)
+
+
+@pytest.mark.parametrize("over,what", [
+    (dict(head_dim=96), "head_dim"), (dict(n_seqs=0), "heads"), (dict(n_kv_heads=-1), "heads"),
+    (dict(n_seqs=40000, n_kv_heads=2), "heads"), (dict(capacity=0), "capacity"),
+    (dict(capacity=96), "capacity"), (dict(capacity=192, block=128), "capacity"),
+    (dict(capacity=(1 << 22) + 64), "capacity"), (dict(given="k_scale"), "array of 4 bytes"),
+    (dict(given="v_scale"), "array of 4 bytes"), (dict(given="lengths"), "array of 4 bytes"),
+    (dict(fails_at=1), "no memory"), (dict(fails_at=5), "no memory"), (dict(fails_at=6), "no copy")])
+def test_a_cache_that_cannot_be_made_holds_no_memory(monkeypatch, over, what):
+    """Geometry and given arrays are looked at first, and what was allocated before a failure is
+    freed: the caller gets no object to close."""
+    made, freed = [], []
+
+    class Tensor:
+        nbytes = 4
+
+        def __init__(self, ctx, n, dtype):
+            if len(made) + 1 == fails_at:
+                raise MemoryError("no memory")
+            made.append(self)
+
+        def upload(self, a):
+            raise MemoryError("no copy")
+
+        def free(self):
+            freed.append(self)
+
+    dims = dict(n_seqs=2, n_kv_heads=2, head_dim=64, capacity=128, block=64)
+    fails_at, given = over.get("fails_at"), over.get("given")
+    dims.update({k: v for k, v in over.items() if k in dims})
+    small = object.__new__(Tensor)
+    monkeypatch.setattr(cache8, "DeviceTensor", Tensor)
+    with pytest.raises(MemoryError if fails_at else ValueError, match=what):
+        Cache8(None, **dims, **({given: small} if given else {}))
+    assert made == freed and len(made) == (fails_at - 1 if fails_at else 0)
 
 
 # ---- the reference itself -------------------------------------------------------------------
