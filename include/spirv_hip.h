@@ -158,9 +158,9 @@ int shp_run_kernel(shp_ctx* ctx, const char* kernel, const float* in0, size_t n0
  *            outside 0 .. capacity count as the nearest of the two)
  * Nothing needs to be cleared first: what lies behind a sequence's length is never used.
  * head_dim 64 or 128; block 16, 32, 64 or 128; capacity a multiple of 64 and of block, up to
- * 4,194,304; at most 65,535 heads of all sequences together; k and v 16-byte aligned; scales
- * positive.  No counterpart in the reference, which caches
- * nothing (run_llama_spirv.py:194-295 recomputes every position).
+ * 4,194,304; at most 65,535 heads of all sequences together; k and v 16-byte aligned, all other
+ * arrays of these calls 4-byte aligned; scales positive.  No counterpart in the reference, which
+ * caches nothing (run_llama_spirv.py:194-295 recomputes every position).
  *
  * Where a call takes n rows a sequence, counts[s] (device, may be NULL: all) says how many of
  * them are real, and row i < counts[s] belongs to token lengths[s] - counts[s] + i.  Rows from
@@ -267,9 +267,9 @@ int shp_cache8_evict(shp_ctx* ctx, const shp_cache8* src, const shp_cache8* dst,
  * natural logarithms, and the n_top likeliest ids with their log probabilities, [rows][n_top], the
  * likeliest first and of equal ones the lowest id first.  targets with logprob, entropy, and
  * top_ids with top_logprobs may be NULL.  0 <= n_top <= 64 and at most vocab; up to 16,000,000 rows
- * and 2^30 logits a row.  A logit of minus
- * infinity is a token that cannot be; a row that holds a NaN or plus infinity, or nothing but minus
- * infinity, has NaN in place of logarithms, and its ids go by the logits with NaN last.  Fewer than
+ * and 2^30 logits a row; all arrays 4-byte aligned.  A logit of minus infinity is a token that cannot
+ * be; a row that holds a NaN or plus infinity, or nothing but minus infinity, has NaN in place of
+ * logarithms, and its ids go by the logits with NaN last.  Fewer than
  * 256 rows of more than 32,768 logits use the context's workspace, as shp_cache8_attend does, and are
  * refused in a capture that finds it too small. */
 typedef struct shp_logprobs_args {

@@ -11,6 +11,8 @@ namespace {
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 bool aligned4(const void* p) { return ((uintptr_t)p & 3) == 0; }
+template <class... P>
+bool aligned4(const void* p, P... rest) { return aligned4(p) && aligned4(rest...); }
 
 int bad(const char* where, const char* what, int code = SHP_ERR_INVALID) {
     return fail(code, std::string(where) + ": " + what);
@@ -79,6 +81,7 @@ int shp_cache8_append(shp_ctx* ctx, const shp_cache8* cache, const shp_cache8_ap
     rc = shp::check_rows(me, "k", a->k, a->k_seq, a->k_row, a->k_head);
     if (!rc) rc = shp::check_rows(me, "v", a->v, a->v_seq, a->v_row, a->v_head);
     if (rc) return rc;
+    if (!shp::aligned4(a->counts)) return bad(me, "counts must be 4-byte aligned");
     if (!ctx) return bad(me, "null ctx");
     if (a->n == 0) return SHP_OK;
     Ctx* x = reinterpret_cast<Ctx*>(ctx);
@@ -115,6 +118,7 @@ int shp_cache8_attend(shp_ctx* ctx, const shp_cache8* cache, const shp_cache8_at
     rc = shp::check_query(me, c, a->q, a->q_seq, a->q_row, a->q_head, a->n, a->n_heads, a->scale);
     if (!rc) rc = shp::check_rows(me, "out", a->out, a->o_seq, a->o_row, a->o_head);
     if (rc) return rc;
+    if (!shp::aligned4(a->counts, a->lse)) return bad(me, "counts and lse must be 4-byte aligned");
     if (!ctx) return bad(me, "null ctx");
     if (a->n == 0) return SHP_OK;
     Ctx* x = reinterpret_cast<Ctx*>(ctx);
@@ -150,6 +154,8 @@ int shp_cache8_weights(shp_ctx* ctx, const shp_cache8* cache, const shp_cache8_w
     rc = shp::check_query(me, c, a->q, a->q_seq, a->q_row, a->q_head, a->n, a->n_heads, a->scale);
     if (rc) return rc;
     if (!a->lse || !a->acc_out) return bad(me, "null lse or acc_out");
+    if (!shp::aligned4(a->counts, a->lse, a->acc_in, a->acc_out))
+        return bad(me, "counts, lse, acc_in and acc_out must be 4-byte aligned");
     if (!ctx) return bad(me, "null ctx");
     Ctx* x = reinterpret_cast<Ctx*>(ctx);
     SHP_HIP_CHECK(hipSetDevice(x->device));
@@ -189,6 +195,8 @@ int shp_cache8_evict(shp_ctx* ctx, const shp_cache8* src, const shp_cache8* dst,
     if (a->keep < 1 || a->keep > d.cap || a->recent < 0 || a->recent > a->keep)
         return bad(me, "needs 1 <= keep <= dst capacity and 0 <= recent <= keep", SHP_ERR_SHAPE);
     if (!a->weights || !a->kept) return bad(me, "null weights or kept");
+    if (!shp::aligned4(a->weights, a->kept, a->dst_weights))
+        return bad(me, "weights, kept and dst_weights must be 4-byte aligned");
     if (a->dst_weights == a->weights) return bad(me, "dst_weights is weights");
     if (!ctx) return bad(me, "null ctx");
     Ctx* x = reinterpret_cast<Ctx*>(ctx);
@@ -211,6 +219,8 @@ int shp_token_logprobs(shp_ctx* ctx, const shp_logprobs_args* a) {
     if (!a->targets != !a->logprob) return bad(me, "targets and logprob go together");
     if (a->n_top && (!a->top_ids || !a->top_logprobs))
         return bad(me, "n_top without top_ids or top_logprobs");
+    if (!shp::aligned4(a->targets, a->logprob, a->entropy, a->top_ids, a->top_logprobs))
+        return bad(me, "targets and outputs must be 4-byte aligned");
     if (a->rows > 16000000 || a->vocab > (1 << 30))
         return bad(me, "more than 16000000 rows or 2^30 logits a row", SHP_ERR_UNSUPPORTED);
     if (!ctx) return bad(me, "null ctx");

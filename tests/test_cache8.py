@@ -124,6 +124,24 @@ def test_bad_arguments_are_refused(name, over, what):
     assert rc != 0 and what in msg and "ctx" not in msg, (rc, msg)
 
 
+@pytest.mark.parametrize("name,cls,fields", [
+    ("shp_cache8_append", Cache8AppendArgs, ["counts"]),
+    ("shp_cache8_attend", Cache8AttendArgs, ["counts", "lse"]),
+    ("shp_cache8_weights", Cache8WeightsArgs, ["counts", "lse", "acc_in", "acc_out"]),
+    ("shp_cache8_evict", Cache8EvictArgs, ["weights", "kept", "dst_weights"]),
+    ("shp_token_logprobs", LogprobsArgs, ["targets", "logprob", "entropy", "top_ids", "top_logprobs"])])
+def test_arrays_of_numbers_that_are_not_aligned_are_refused(name, cls, fields):
+    far = cache(k=P + 0x50000, v=P + 0x60000, k_scale=P + 0x70000, v_scale=P + 0x80000,
+                lengths=P + 0x90000)
+    first = () if cls is LogprobsArgs else (cache(), far) if cls is Cache8EvictArgs else (cache(),)
+    for f in fields:
+        for off in (1, 2, 3):
+            rc, msg = call(name, *first, args(cls, **{f: 0x100000 + off}))
+            assert rc == _lib.SHP_ERR_INVALID and "4-byte aligned" in msg, (f, msg)
+        rc, msg = call(name, *first, args(cls, **{f: 0x100004}))
+        assert msg == f"{name}: null ctx"
+
+
 def test_null_structures_are_refused():
     for name in (*CALLS, "shp_cache8_evict"):
         rest = (cache(k=P + 64),) if name == "shp_cache8_evict" else ()
