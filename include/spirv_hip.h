@@ -250,8 +250,9 @@ int shp_cache8_weights(shp_ctx* ctx, const shp_cache8* cache,
  * their old order, each KV head its own.  Blocks are made anew from the values of src.  Writes
  * dst->lengths, kept [n_seqs][n_kv_heads][keep] (the tokens' places in src, -1 behind the last)
  * and dst_weights [n_seqs][n_kv_heads][dst->capacity] (may be NULL: their weights, zero behind the
- * last).  weights is [n_seqs][n_kv_heads][src->capacity].  src and dst agree in all but capacity and
- * share no memory; 1 <= keep <= dst->capacity and 0 <= recent <= keep. */
+ * last).  weights is [n_seqs][n_kv_heads][src->capacity].  src and dst agree in all but capacity;
+ * none of the arrays that are written shares memory with another array of the call (refused, by
+ * their sizes); 1 <= keep <= dst->capacity and 0 <= recent <= keep. */
 typedef struct shp_cache8_evict_args {
     const float* weights;
     int32_t* kept;

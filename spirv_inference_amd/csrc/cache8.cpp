@@ -1,7 +1,9 @@
 // The C ABI of the 8-bit cache and of token log probabilities: argument checks, scratch and
 // timing around the launchers.  Arguments are checked before the context, so a refusal needs no
 // device.
+#include <array>
 #include <cmath>
+#include <vector>
 
 #include "cache8.h"
 #include "runtime.h"
@@ -49,6 +51,34 @@ int check_rows(const char* where, const char* what, const float* p, int64_t seq,
     if (!aligned16(p) || (seq | row | head) & 3)
         return bad(where, (std::string(what) + " rows must be 16-byte aligned").c_str());
     return SHP_OK;
+}
+
+struct Range {
+    uintptr_t from, bytes;
+    Range(const void* p, int64_t n) : from((uintptr_t)p), bytes(p ? (uintptr_t)n : 0) {}
+    bool meets(const Range& o) const {
+        return bytes && o.bytes && from < o.from + o.bytes && o.from < from + bytes;
+    }
+};
+std::array<Range, 5> ranges(const Cache8& c, int head_dim) {
+    const int64_t n = (int64_t)c.n_seqs * c.kv * c.cap, scales = (n >> c.block_log2) * 4;
+    return {Range(c.k, n * head_dim), Range(c.v, n * head_dim), Range(c.k_scale, scales),
+            Range(c.v_scale, scales), Range(c.lengths, c.n_seqs * 4ll)};
+}
+// Whether what an eviction writes overlaps what it reads, or something else that it writes.
+bool evict_overlaps(const Cache8& s, const Cache8& d, int head_dim, const shp_cache8_evict_args& a) {
+    const int64_t heads = (int64_t)s.n_seqs * s.kv;
+    std::vector<Range> in(1, Range(a.weights, heads * s.cap * 4));
+    std::vector<Range> out = {Range(a.kept, heads * a.keep * 4), Range(a.dst_weights, heads * d.cap * 4)};
+    for (const Range& r : ranges(s, head_dim)) in.push_back(r);
+    for (const Range& r : ranges(d, head_dim)) out.push_back(r);
+    for (size_t i = 0; i < out.size(); ++i) {
+        for (const Range& r : in)
+            if (out[i].meets(r)) return true;
+        for (size_t j = 0; j < i; ++j)
+            if (out[i].meets(out[j])) return true;
+    }
+    return false;
 }
 
 // What attention and its accounts have in common.
@@ -199,6 +229,8 @@ int shp_cache8_evict(shp_ctx* ctx, const shp_cache8* src, const shp_cache8* dst,
         return bad(me, "weights, kept and dst_weights must be 4-byte aligned");
     if (a->dst_weights == a->weights) return bad(me, "dst_weights is weights");
     if (!ctx) return bad(me, "null ctx");
+    if (shp::evict_overlaps(s, d, src->head_dim, *a))
+        return bad(me, "what is written shares memory with what is read or written");
     Ctx* x = reinterpret_cast<Ctx*>(ctx);
     SHP_HIP_CHECK(hipSetDevice(x->device));
     return x->timed("cache8_evict", [&] {

@@ -174,6 +174,42 @@ def test_bad_reads_and_evictions_are_refused():
         assert rc != 0 and what in msg, (dst, over, msg)
 
 
+def test_evictions_into_their_own_arrays_are_refused():
+    """By the arrays' sizes, not only where they begin.  The context is memory that a refused call
+    does not touch: calls without an overlap get as far as asking for its device."""
+    ctx = C.create_string_buffer(1 << 16)
+    # 2 x 2 heads of 128 (src) and 64 (dst) tokens x 64, blocks of 64, 64 kept
+    size = dict(k=32768, v=32768, k_scale=32, v_scale=32, lengths=8, weights=2048)
+    dsize = dict(k=16384, v=16384, k_scale=16, v_scale=16, lengths=8, kept=1024, dst_weights=1024)
+    at, where = 1 << 20, {}
+    for n, b in (*(("s." + n, b) for n, b in size.items()), *(("d." + n, b) for n, b in dsize.items())):
+        where[n] = at
+        at += -(-b // 16) * 16
+
+    def evict(**moved):
+        w = {**where, **{n.replace("_", ".", 1): p for n, p in moved.items()}}
+        names = ("k", "v", "k_scale", "v_scale", "lengths")
+        s, d = (cache(capacity=c, **{n: w[f"{o}.{n}"] for n in names}) for o, c in (("s", 128), ("d", 64)))
+        rc = _lib.lib().shp_cache8_evict(ctx, C.byref(s), C.byref(d), C.byref(args(
+            Cache8EvictArgs, weights=w["s.weights"], kept=w["d.kept"], dst_weights=w["d.dst_weights"])))
+        return "shares memory" in _lib.lib().shp_last_error().decode(), rc
+
+    for n, b in dsize.items():
+        for o, ob in (*(("s." + m, x) for m, x in size.items()), *(("d." + m, x) for m, x in dsize.items())):
+            if o == "d." + n:
+                continue
+            step = 16 if n in "kv" else 4
+            for p in (where[o] + ob - step, where[o] - b + step):  # the last bytes, the first bytes
+                p = p // step * step
+                overlap, rc = evict(**{"d_" + n: p})
+                assert overlap and rc == _lib.SHP_ERR_INVALID, (n, o)
+    far = 1 << 22
+    for n in dsize:
+        # next to each other is not an overlap
+        assert not evict(**{"d_" + n: far})[0] and not evict(**{"d_" + n: at})[0], n
+    assert not evict(d_dst_weights=0)[0]
+
+
 @pytest.mark.parametrize("over,what", [
     (dict(rows=-1), "rows"), (dict(vocab=0), "vocab"), (dict(logits=0), "logits"),
     (dict(logits=P + 2), "logits"), (dict(row_stride=63), "row_stride"),
