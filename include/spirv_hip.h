@@ -166,7 +166,7 @@ int shp_run_kernel(shp_ctx* ctx, const char* kernel, const float* in0, size_t n0
  * them are real, and row i < counts[s] belongs to token lengths[s] - counts[s] + i.  Rows from
  * counts[s] on are neither read nor written.  Strides are in floats, between sequences (_seq),
  * rows (_row) and heads (_head); the head_dim floats of a row lie next to each other; rows and
- * strides are multiples of 16 bytes.  n = 0 does nothing.
+ * strides are multiples of 16 bytes.  n = 0 adds nothing: accounts are copied, other calls do nothing.
  *
  * All calls are asynchronous on the context stream and can be captured.  attend and weights use the
  * context's workspace, as the dense kernels' K splits do: calls of one context that could run at the

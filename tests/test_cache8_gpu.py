@@ -518,6 +518,21 @@ def test_accounts_of_many_rows_in_a_long_cache(ctx, fmt, d, n, counts, lens):
     check_accounts(ctx, fmt, d, 2, 3, n, counts, lens, 65536)
 
 
+def test_accounts_of_no_rows_are_copied(ctx):
+    rng = np.random.default_rng(31)
+    with filled(ctx, rng, 2, 1, 64, 128, 32, "i8", [100, 0]) as p:
+        start = rng.uniform(0, 2, (2, 1, 128)).astype(np.float32)
+        acc, res, bare, t = p.up(start), p.new(256, fill=-3), p.new(256, fill=-3), p.new(64)
+        p.dev.weights(t, t, acc, res, 2, 0)
+        p.dev.weights(t, t, acc, acc, 2, 0)
+        p.dev.weights(t, t, None, bare, 2, 0)
+        ctx.sync()
+        np.testing.assert_array_equal(acc.download(), start.reshape(-1))
+        for got, want in ((res, start), (bare, 0 * start)):
+            want[0, :, 100:], want[1] = -3, -3
+            np.testing.assert_array_equal(got.download().reshape(start.shape), want)
+
+
 def evict_both(p, q, weights, keep, recent):
     s_, kv, d, cap = q.dims
     kept, acc = p.new(s_ * kv * keep, np.int32, 99), p.new(s_ * kv * cap, fill=-3)
