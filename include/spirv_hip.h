@@ -229,8 +229,9 @@ int shp_cache8_attend(shp_ctx* ctx, const shp_cache8* cache, const shp_cache8_at
  * rows of all query heads of a KV head give a token, [n_seqs][n_kv_heads][capacity]; lse is what
  * shp_cache8_attend wrote for the same rows.  acc_in may be acc_out, or NULL for zeros.  What
  * lies behind a sequence's length is left as it was: clear it once before the first call, so that
- * tokens appended later start from zero.  Uses the context's workspace as shp_cache8_attend does; for
- * the same arguments the order of the sums is the same. */
+ * tokens appended later start from zero.  Uses the context's workspace as shp_cache8_attend does; the
+ * order of the sums is the same for the same arguments, but another one in a captured call that finds
+ * the workspace too small (a KV head's rows are then added one chunk after the other). */
 typedef struct shp_cache8_weights_args {
     const float* q;
     int64_t q_seq, q_row, q_head;

@@ -173,8 +173,7 @@ __device__ __forceinline__ float code_value(unsigned w, int i) {
     else return __builtin_amdgcn_cvt_f32_fp8((int)b, 0);
 }
 
-// Tokens sequence s holds, and the index of its first new row (negative where fewer tokens are
-// held than rows are given).
+// Tokens sequence s holds, and how many of the n rows given for it are real, both within what can be.
 __device__ __forceinline__ int seq_length(const shp::Cache8& c, int s) {
     return min(max(c.lengths[s], 0), c.cap);
 }
