@@ -2,6 +2,8 @@
 
 Codes, scales and what eviction keeps are compared bit for bit; attention and accounts within the
 bounds that cache8_ref.bound derives from the operations' roundings."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -518,6 +520,13 @@ def test_accounts_of_many_rows_in_a_long_cache(ctx, fmt, d, n, counts, lens):
     check_accounts(ctx, fmt, d, 2, 3, n, counts, lens, 65536)
 
 
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("counts", [[0, 1], [1, 0], [0, 0]])
+def test_accounts_of_a_decode_step_with_idle_slots(ctx, fmt, counts):
+    """One row group a head: where a sequence has no row, its accounts are copied."""
+    check_accounts(ctx, fmt, 64, 2, 4, 1, counts, [200, 77], 320)
+
+
 def test_accounts_of_no_rows_are_copied(ctx):
     rng = np.random.default_rng(31)
     with filled(ctx, rng, 2, 1, 64, 128, 32, "i8", [100, 0]) as p:
@@ -531,6 +540,20 @@ def test_accounts_of_no_rows_are_copied(ctx):
         for got, want in ((res, start), (bare, 0 * start)):
             want[0, :, 100:], want[1] = -3, -3
             np.testing.assert_array_equal(got.download().reshape(start.shape), want)
+
+
+@pytest.mark.parametrize("d,fmt", [(64, "i8"), (128, "e4m3")])
+def test_accounts_of_row_groups_of_several_chunks(d, fmt):
+    """So many rows over so large a cache that the row groups whose sums find room each take several
+    chunks of 64 rows, the later ones adding to what the earlier left."""
+    kv, group, n, cap, counts, lens = 4, 3, 350, 131072, [350, 30], [400, 65]
+    one = 2 * kv * cap * 4  # bytes of a group's sums
+    with Context("any") as own:
+        check_accounts(own, fmt, d, kv, group, n, counts, lens, cap)
+        ptr, size = C.c_void_p(), C.c_uint64()
+        check(lib().shp_workspace_info(own.handle, C.byref(ptr), C.byref(size)), "workspace_info")
+        # several groups, but fewer than there are chunks
+        assert 2 * one <= size.value < n * group // 64 * one
 
 
 def evict_both(p, q, weights, keep, recent):

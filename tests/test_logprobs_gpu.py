@@ -62,6 +62,26 @@ def test_logprobs(ctx, rows, vocab, top, std):
     check(run(ctx, x, targets, top), x, targets, top)
 
 
+# so many rows that each takes a workgroup of 128, with one chunk of logits or several
+@pytest.mark.parametrize("rows,vocab,top", [
+    (1024, 4096, 64), (1025, 4097, 5), (1100, 300, 64), (1030, 12345, 20), (1500, 1, 1)])
+def test_logprobs_of_many_rows(ctx, rows, vocab, top):
+    rng = np.random.default_rng(rows)
+    x = (rng.standard_normal((rows, vocab)) * 3).astype(np.float32)
+    targets = rng.integers(0, vocab, rows)
+    check(run(ctx, x, targets, top), x, targets, top)
+
+
+# so many parts of a row that the best of all do not fit into the memory of the workgroup that joins them
+@pytest.mark.parametrize("kind", ["normal", "few", "equal"])
+def test_logprobs_of_more_than_a_million_logits(ctx, kind):
+    rng = np.random.default_rng(14)
+    shape = (2, 1_100_003)
+    x = {"normal": rng.standard_normal(shape), "few": rng.integers(0, 50000, shape) * 1e-4,
+         "equal": np.full(shape, -2.5)}[kind].astype(np.float32)
+    check(run(ctx, x, [7, 1_100_002], 64), x, [7, 1_100_002], 64)
+
+
 @pytest.mark.parametrize("vocab", [200, 32000, 70001])
 @pytest.mark.parametrize("kind", ["equal", "few", "ascending", "descending", "zeros"])
 def test_ties_go_to_the_lowest_id(ctx, vocab, kind):
@@ -71,6 +91,10 @@ def test_ties_go_to_the_lowest_id(ctx, vocab, kind):
          "descending": np.tile(np.arange(vocab)[::-1] * 1e-3, (2, 1)),
          "zeros": rng.choice([0.0, -0.0], (2, vocab))}[kind].astype(np.float32)
     check(run(ctx, x, [0, vocab - 1], 64), x, [0, vocab - 1], 64)
+
+
+def test_plateaus_of_many_rows(ctx):
+    test_plateaus_and_chunks_of_one_kind(ctx, 1026, 13000)
 
 
 @pytest.mark.parametrize("rows,vocab", [(2, 40000), (300, 20000)])
