@@ -49,7 +49,7 @@ struct Scales {
 
 // ---- append ----------------------------------------------------------------------------------
 // The new rows of one span, of K or V of one head.  Rows are read once, into registers; V's codes
-// turn through LDS.  Prompts of 4 x up to 2,000 rows x 8 heads x 128 (41 MB): 11.4 us; a kernel
+// turn through LDS.  Prompts of 4 x up to 2,000 rows x 8 heads x 128 (2,316 rows, 24 MB): 11.4 us; a kernel
 // that read rows twice, wrote single bytes and divided for every code took 18.8.
 template <int D, int FMT, int SPAN, bool V>
 __device__ __forceinline__ void append_span(const Cache8& c, const Cache8Rows& r, Scales& sc,
@@ -568,8 +568,8 @@ __device__ __forceinline__ void gather_k(const Cache8& src, const Cache8& dst, c
 // One span of V: a lane makes words of four tokens of a dimension, whose bytes it reads one by one.
 // The 64 tokens of a span come from few tiles (their places rise), so a wavefront's loads share
 // lines, and lines are all that reading whole tiles would fetch too.  128 heads, 1,900-8,190 tokens of
-// 128 to 2,048, K and V: 64 us for 182 MB; with a lane a token, which then writes single bytes, 79; with
-// whole tiles read and their bytes sorted out in LDS 76.
+// 128 to 2,048, K and V: 64 us for 216 MB, of which the kept tokens are 134; with a lane a token, which
+// then writes single bytes, 79; with whole tiles read and their bytes sorted out in LDS 76.
 template <int D, int FMT, int SPAN>
 __device__ __forceinline__ void gather_v(const Cache8& src, const Cache8& dst, const int32_t* id,
                                          int t0, int t1, Scales& sc) {

@@ -5,7 +5,8 @@
 // and sum of a softmax.  Codes are exact as fp16, q and the weights are cut into two fp16 pieces of
 // 11 bits (both rounded to nearest, so an operand is off by 2^-23 of itself), and the products run on
 // v_mfma_f32_16x16x32_f16 with fp32 sums: twice the products of one fp16 pass at 8 times the rate of
-// fp32's own matrix instructions, and errors against 64 bits no larger than those of fp32 products.
+// fp32's own matrix instructions.  Against 64 bits (norms) outputs are off by 1.6e-7 on 300 tokens, 4.3e-7
+// for 512 rows on 8,190 and 4.9e-7 on 131,072; those of fp32 products by 2.6e-7, 1.6e-6 and 3.2e-6.
 //
 // Scores are computed transposed, S^T = K Q^T.  Row m of token tile j is given to token
 // (m / 4) * 16 + 4 j + m % 4 of the 64: the lane (query l % 16, group g = l / 16) then holds the
@@ -149,7 +150,7 @@ __device__ __forceinline__ void load_k(const uint8_t* tile, u4 raw[4][D / 64]) {
 }
 // K's tiles of 128 dimensions go through LDS where 32 rows or more share one: lanes 0 to 15 of load_k
 // read 16 bytes each of 16 rows, 16 cache lines, and tiles that many rows want come from L2, where that
-// is what costs (512 rows on 8,190 tokens: attention 141 us so, 150 without, accounts 88 and 97 with 32
+// is what costs (512 rows on 8,190 tokens: attention 143 us so, 150 without, accounts 88 and 97 with 32
 // rows a wavefront; rows of 64 dimensions are half as many lines and attention takes 94 and 91, and 16
 // query rows, which memory bounds, 727 and 720).
 template <int D, int MT>
@@ -207,14 +208,15 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 // at the end.  (Side by side over rows they would share tiles, but then few rows have to be cut into
 // many shares of the tokens, whose parts go through memory: 512 rows x 4 heads on 8,190 tokens 171 us
 // that way, 147 so, measured in one run.)  32 rows are what registers allow with two workgroups on a CU:
-// 64 rows of 64 dimensions spilled and took 147 us where 32 take 92.  The tokens of a sequence are shared
+// 64 rows of 64 dimensions spilled and took 147 us where 32 take 88.  The tokens of a sequence are shared
 // out over workgroups while that fills the GPU.
 //
 // With up to 16 rows reading the cache bounds it: 16 x 128,001-131,072 tokens x 8 heads x 128 (4.2 GB)
 // 720 us, 5.9 TB/s, 24 sequences of 0-8,100 tokens 53 us, 3.8 TB/s (46 us where they are all as long as
-// the average); a single sequence of 300 tokens takes 5.8 us, which is latency.  With more rows the matrix
-// and vector units do, which take about as long: 512 rows x 4 heads on 8,190 tokens x 8 heads x 128
-// (66.6 GFLOP, twice that as products of pieces) 141 us, 945 TFLOP/s of products.
+// the average); a single sequence of 300 tokens takes 5.7 us, which is latency.  With more rows the vector
+// unit, busy in 61 % of the cycles, and the matrix unit, busy in 37 %, do between them: 512 rows x 4 heads
+// on 8,190 tokens x 8 heads x 128 (66.6 GFLOP, twice that as products of pieces) 143 us, 931 TFLOP/s of
+// products.
 // (Launch bounds: the wavefronts a SIMD that each variant reaches without spills.)
 template <int D, int FMT, int MT>
 __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_attend_kernel(Cache8 c, Cache8Query q, int least,
@@ -594,9 +596,12 @@ __device__ __forceinline__ void halve(float* v) {
 // in `part` [group][head][capacity] and cache8_weights_join_kernel adds them in order; a group of
 // several chunks of rows adds to what its own chunks before left there.  groups == 1 writes the
 // accounts themselves.  A decode step is bound by reading K: 24 sequences of 500-8,100 tokens x 8 heads x
-// 128 (113 MB) 30 us, 3.8 TB/s.  A prompt's chunk is bound by the vector unit (exp2, the conversion of K,
-// q's pieces): 512 rows x 8 heads on 8,190 tokens x 4 heads x 64 (16.6 GFLOP) 50.5 us, of
-// which 5 are the join; 512 rows x 4 heads on 8 heads x 128 (33.3 GFLOP) 76 us.
+// 128 (113 MB) 30 us, 3.8 TB/s.  A prompt's chunk keeps the vector unit busy in 50 % of the cycles (exp2,
+// the conversion of K, q's pieces) and the matrix unit in 25 %, and a quarter of the time no wavefront is
+// there (the groups do not end together): 512 rows x 8 heads on 8,190 tokens x 4 heads x 64 (16.6
+// GFLOP) 50.5 us, of which 5 are the join; 512 rows x 4 heads on 8 heads x 128 (33.3 GFLOP) 76 us.  The log
+// sum enters in units of log2, rounded to fp32: against 64 bits the accounts of the chunk are off by
+// 4.9e-8 (norms), fp32 torch's by 3.3e-8, those of the decode step by 2.5e-8 both.
 template <int D, int FMT, int MT>
 __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(Cache8 c, Cache8Query q, int row_waves,
                                                              int groups, int chunks, float* part) {
@@ -753,10 +758,10 @@ Cache8Plan cache8_attend_plan(const Cache8& c, int head_dim, int64_t rows, int c
     Cache8Plan p;
     // 32 rows a workgroup use each tile for twice the work, 16 leave room for more workgroups on a CU.
     // 32 pay where there is much of both, from 32 pairs of 32 rows and 64 tokens a CU with 128 dimensions
-    // (64 rows x 4 heads on 8,190 tokens x 8 heads 32.6 us, 36.5 with 16 rows; 40: 36.8, 34.5; 16: 23.7,
-    // 19.7) and 128 with 64, whose tiles cost half (512 rows x 8 heads on 8,190 tokens x 4 heads 90 us, 102;
-    // 192: 55, 47; 128: 32, 34; 32 on 600 tokens 11.7, 8.7); and with 128 where blocks of 16 do not find
-    // room at once, three on a CU (prompts of 500 x 4 x 8 heads 16.9 us, 21.4; of 350: 16.0, 12.7).
+    // (64 rows x 4 heads on 8,190 tokens x 8 heads 33.0 us, 35.5 with 16 rows; 40: 36.6, 33.5; 16: 24.0,
+    // 18.9) and 128 with 64, whose tiles cost half (512 rows x 8 heads on 8,190 tokens x 4 heads 88 us, 102;
+    // 192: 52, 46; 128: 32, 34; 32 on 600 tokens 11.8, 8.5); and with 128 where blocks of 16 do not find
+    // room at once, three on a CU (prompts of 500 x 4 x 8 heads 16.7 us, 21.2; of 350: 15.9, 12.5).
     const int64_t cu = std::max(cu_count, 1), heads = (int64_t)c.n_seqs * c.kv;
     const int64_t pairs = heads * ((rows + 31) / 32) * (c.cap / kCacheTile);
     const bool many = head_dim == 64 ? pairs >= 128 * cu

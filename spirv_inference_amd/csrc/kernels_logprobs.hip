@@ -3,12 +3,14 @@
 //
 // A workgroup holds 32 logits a thread in registers: their maximum m, Z = sum exp(x - m) and X = sum
 // exp(x - m) (x - m) give log p = x - m - log Z and the entropy log Z - X / Z, a sum of two numbers
-// that are not negative.
+// that are not negative.  exp(d) is exp2(d * log2 e) with a rounded product, off by 2^-24 of d log2 e; |d| e^d
+// is under 0.37, so that costs a sum less than its own rounding.  Against 64 bits results are off by 6.7e-8
+// (1 x 32,000) and 9.5e-8 (1,500 x 131,071), norms; those of fp32 torch by 4.5e-8 and 5.0e-8.
 //
 // From 256 rows on a workgroup takes a row, chunk after chunk, and reading bounds it: 1,500 x
 // 131,071 with 20 alternatives (786 MB) 160 us, 4.9 TB/s, 146 without alternatives.  It has 256 threads,
 // from 1,024 rows on 128 (4,000 x 40,000 133 us, 148 with 256; 600 x 32,000 40, 30).  Fewer rows are cut
-// into parts of 32,768 logits for workgroups of 1,024, and joined: 1 x 32,000 8.2 us (17 the other
+// into parts of 32,768 logits for workgroups of 1,024, and joined: 1 x 32,000 8.1 us (17 the other
 // way), 128 x 32,000 12.2 (26); 300 x 131,071 take 69 and 72, 600 x 32,000 28 and 35.
 #include "cache8.h"
 
