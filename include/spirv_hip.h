@@ -203,7 +203,8 @@ int shp_cache8_append(shp_ctx* ctx, const shp_cache8* cache, const shp_cache8_ap
 int shp_cache8_read(shp_ctx* ctx, const shp_cache8* cache, int32_t n, float* k, float* v);
 
 /* Attention: out = softmax(scale * q . K) V over the tokens up to the row's own.  n_heads query
- * heads share the n_kv_heads KV heads in order, n_heads / n_kv_heads each.  A row that sees no
+ * heads share the n_kv_heads KV heads in order, n_heads / n_kv_heads each; a KV head has at most
+ * 500,000 rows of a sequence (n of each of its query heads).  A row that sees no
  * token (its sequence is empty, or holds fewer tokens than rows) gets zeros.  lse (may be NULL)
  * [n_seqs][n_heads][n]: log of the sum of exp(scale * q . k), minus infinity for such a row.
  * Statistics and sums are fp32, and q and the weights enter the products with 22 bits; in the product
