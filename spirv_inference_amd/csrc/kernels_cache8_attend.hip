@@ -189,6 +189,12 @@ __device__ __forceinline__ void load_v(const uint8_t* tile, u4 raw[D / 16]) {
         raw[d] = *reinterpret_cast<const u4*>(p + d * 16 * kCacheTile);
 }
 
+// What a product of codes and pieces of q is multiplied by: finite where K's scale is, so that a product
+// of zero is a score of zero however large q and K are.
+__device__ __forceinline__ float score_factor(float kscale, float back) {
+    return __builtin_elementwise_minimum(kscale * back, 3.4028234663852886e+38f);  // a NaN stays
+}
+
 // 2^(m - top), also where both are minus infinity or infinity.
 __device__ __forceinline__ float factor_of(float m, float top) {
     return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
@@ -316,7 +322,7 @@ __global__ __launch_bounds__(256, MT == 2 ? 2 : D == 64 ? 4 : 3) void cache8_att
         h8 wh[MT][2], wl[MT][2];
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
-            const float f = ks * back[t];
+            const float f = score_factor(ks, back[t]);
             float mx = -__builtin_inff();
             if (edge) {
 #pragma unroll
@@ -671,7 +677,7 @@ __global__ __launch_bounds__(256, 2) void cache8_weights_kernel(Cache8 c, Cache8
 #pragma unroll
             for (int e = 0; e < 16; ++e) v[e] = 0.0f;
 #pragma unroll
-            for (int t = 0; t < MT; ++t) f[t] = ks * back[t];
+            for (int t = 0; t < MT; ++t) f[t] = score_factor(ks, back[t]);
             const bool edge = gaps || t0 + kCacheTile > open;
             f4 sc[MT][4];
 #pragma unroll

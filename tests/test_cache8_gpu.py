@@ -387,6 +387,26 @@ def test_attention_of_zero_tiny_and_huge_queries(ctx):
         np.testing.assert_allclose(out[0, 2, 0], p.ref.values("v", 0, 0)[best], rtol=1e-6)
 
 
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [1, 40])
+def test_attention_of_huge_queries_to_huge_keys_across_them(ctx, fmt, d, n):
+    """q and K whose products would overflow, but of which none meets another: scores of zero."""
+    rng = np.random.default_rng(24)
+    k, q = np.zeros((1, 100, 1, d), np.float32), np.zeros((1, n, 2, d), np.float32)
+    k[..., ::2], q[..., 1::2] = 1e30, 1e32
+    with Pair(ctx, 1, 1, d, 128, 32, fmt) as p:
+        p.append(k, rows(rng, 1, 100, 1, d), [100])
+        _, lse = p.check_attend(q)
+        t = p.up(lse)
+        acc = p.new(128)
+        p.dev.weights(p.up(q), t, None, acc, 2, n)
+        ctx.sync()
+        got = acc.download()[:100]
+        want, tol = R.attend(p.ref, q, [n], d ** -0.5, lse_in=lse.astype(np.float64))
+        assert (np.abs(got - want[0, 0, :100]) <= tol[0, 0, :100] + want[0, 0, :100] * (2 * n + 2) * 2.0 ** -24).all()
+
+
 def test_a_row_that_is_not_finite_spoils_only_itself(ctx):
     rng = np.random.default_rng(16)
     with filled(ctx, rng, 1, 1, 64, 128, 32, "i8", [100]) as p:
