@@ -207,9 +207,10 @@ int shp_cache8_read(shp_ctx* ctx, const shp_cache8* cache, int32_t n, float* k, 
  * 500,000 rows of a sequence (n of each of its query heads).  A row that sees no
  * token (its sequence is empty, or holds fewer tokens than rows) gets zeros.  lse (may be NULL)
  * [n_seqs][n_heads][n]: log of the sum of exp(scale * q . k), minus infinity for such a row.
- * Statistics and sums are fp32, and q and the weights enter the products with 22 bits; in the product
- * with V a token whose weight times V's scale is 2^15 times smaller than the row's largest has fewer,
- * and one 2^37 times smaller none (its weight counts in the sum and in lse all the same).
+ * Statistics and sums are fp32, and q and the weights enter the products with 22 bits.  An element of
+ * q that is 2^15 times smaller than the largest of its row has fewer, and one 2^39 times smaller none;
+ * so, in the product with V, does a token whose weight times V's scale is 2^15 and 2^37 times smaller
+ * than the row's largest (its weight counts in the sum and in lse all the same).
  * The tokens are split over workgroups whose partial results go through the context's workspace;
  * it grows on an eager call that needs more, to twice its size at least, which the host waits for, and
  * a captured call that finds it too small runs without the split: run the call once before it is

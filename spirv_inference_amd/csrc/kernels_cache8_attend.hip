@@ -3,7 +3,8 @@
 // A wavefront holds 16 * MT query rows (the rows of all query heads of a KV head, row r = new token
 // r / group, head r % group) and walks the sequence's tokens 64 at a time, with the running maximum
 // and sum of a softmax.  Codes are exact as fp16, q and the weights are cut into two fp16 pieces of
-// 11 bits (both rounded to nearest, so an operand is off by 2^-23 of itself), and the products run on
+// 11 bits (both rounded to nearest, so an operand is off by 2^-23 of itself, or of 2^-15 of its row's
+// largest where that is more), and the products run on
 // v_mfma_f32_16x16x32_f16 with fp32 sums: twice the products of one fp16 pass at 8 times the rate of
 // fp32's own matrix instructions.  Against 64 bits (norms) outputs are off by 1.6e-7 on 300 tokens, 4.3e-7
 // for 512 rows on 8,190 and 4.9e-7 on 131,072; those of fp32 products by 2.6e-7, 1.6e-6 and 3.2e-6.
