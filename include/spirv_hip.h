@@ -265,6 +265,104 @@ typedef struct shp_cache8_evict_args {
 int shp_cache8_evict(shp_ctx* ctx, const shp_cache8* src, const shp_cache8* dst,
                      const shp_cache8_evict_args* args);
 
+/* ---- paged key/value cache -------------------------------------------------------------
+ * Keys and values of n_seqs sequences in pages of page_size tokens, which a table hands out:
+ *   k, v     [n_pages][n_kv_heads][page_size][head_dim], in fp32, fp16 or bf16
+ *   table    [n_seqs][max_pages]: the page that holds tokens p * page_size .. of the sequence.  An
+ *            entry outside 0 .. n_pages - 1 is a page that is not there: no row sees its tokens,
+ *            and what is written to them is dropped
+ *   lengths  [n_seqs]: tokens each sequence holds, the call's own new rows included (values
+ *            outside 0 .. max_pages * page_size count as the nearest of the two)
+ * All arrays are the caller's, on the context's device.  Nothing needs to be cleared first: what lies
+ * behind a sequence's length is never used.  Sequences may share pages that no call writes to; a
+ * page that is written belongs to one sequence.
+ * head_dim 64 or 128; page_size 16, 32, 64, 128 or 256; max_pages * page_size up to 4,194,304; at most
+ * 65,535 heads of all sequences together; k and v 16-byte aligned, all other arrays of these calls
+ * 4-byte aligned.  Rows, counts and strides are as for shp_cache8: row i < counts[s] is token
+ * lengths[s] - counts[s] + i, its place.  Values that fp16 cannot hold become infinities.
+ * All calls are asynchronous on the context stream and can be captured.  No counterpart in the
+ * reference, which caches nothing (run_llama_spirv.py:194-295 recomputes every position).
+ *
+ * A tree of drafted tokens: parents[s][i] is the row that row i follows, an earlier one; any other
+ * value: row i follows the context (the tokens before the sequence's new rows).  Trees have at most
+ * 256 rows.  A row's depth is the number of rows above it, and its position lengths[s] - counts[s] +
+ * depth; without a tree a row's position is its place. */
+enum { SHP_PAGED_F32 = 0, SHP_PAGED_F16 = 1, SHP_PAGED_BF16 = 2 };
+typedef struct shp_paged {
+    void *k, *v;
+    const int32_t* table;
+    int32_t* lengths;
+    int32_t n_seqs, n_kv_heads, head_dim, n_pages, page_size, max_pages, format;
+} shp_paged;
+
+/* Writes new rows, turned by their positions: the first `rot` dimensions of a row of k (and of q) are
+ * rot / 2 pairs (x0, x1), dimensions j and j + rot / 2 or, interleaved, 2 j and 2 j + 1, and become
+ * (x0 cos a - x1 sin a, x1 cos a + x0 sin a) with a = position * inv_freq[j], the product of the two
+ * exact.  The position is lengths[s] - counts[s] + offsets[s][i], i where offsets is NULL (a tree's
+ * offsets are its depths).  inv_freq [rot / 2] on the device; rot a multiple of 8 up to head_dim, or 0
+ * (nothing is turned, inv_freq is not read).  v and the other dimensions are stored as they are.  q
+ * [n_heads heads a row] goes to q_out turned, and may be q_out with the same strides; both NULL: no
+ * queries.  Rows of tokens before the first (lengths[s] < counts[s]) are not stored, their queries
+ * are turned all the same. */
+typedef struct shp_paged_append_args {
+    const float *k, *v;
+    int64_t k_seq, k_row, k_head;
+    int64_t v_seq, v_row, v_head;
+    const float* q;
+    float* q_out;
+    int64_t q_seq, q_row, q_head;
+    int64_t o_seq, o_row, o_head;
+    const int32_t* counts;
+    const int32_t* offsets;
+    const float* inv_freq;
+    int32_t n, n_heads, rot, interleaved;
+} shp_paged_append_args;
+int shp_paged_append(shp_ctx* ctx, const shp_paged* cache, const shp_paged_append_args* args);
+
+/* Attention: out = softmax(x) V over the tokens a row sees, x = scale * q . k, where cap > 0 then cap *
+ * tanh(x / cap), and with slopes [n_heads] less slopes[head] * |difference of the positions|.  Row i of
+ * a sequence sees a token at place t if
+ *   - t >= first[s][i] (NULL: 0): where the row's document begins; and
+ *   - it is no later: t <= the row's place, or in a tree (parents not NULL) the context, the rows above
+ *     it and itself; and with window > 0 their positions differ by less than window;
+ *   - or, window or not, t < prefix[s] (NULL: 0), of a tree's own rows only those above it and itself.
+ * n_heads query heads share the n_kv_heads KV heads in order; a KV head has at most 500,000 rows of a
+ * sequence.  A row that sees no token, or lies before the first token itself, gets zeros.  lse (may be
+ * NULL) [n_seqs][n_heads][n]: log of the sum of exp(x), minus infinity for such a row.  What a row does
+ * not see has no part in its result, whatever it holds.  Statistics and sums are fp32.  */
+typedef struct shp_paged_attend_args {
+    const float* q;
+    float* out;
+    int64_t q_seq, q_row, q_head;
+    int64_t o_seq, o_row, o_head;
+    const int32_t* counts;
+    float* lse;
+    const float* slopes;
+    const int32_t* prefix;
+    const int32_t* first;
+    const int32_t* parents;
+    int32_t n, n_heads, window;
+    float scale, cap;
+} shp_paged_attend_args;
+int shp_paged_attend(shp_ctx* ctx, const shp_paged* cache, const shp_paged_attend_args* args);
+
+/* Keeps what the model agrees with of a drafted tree whose rows were appended.  Row 0 is the token that is
+ * settled already and is kept; behind a kept row, the first row j with it as its parent and tokens[j]
+ * == choices[its parent] (the id the model chose there) is kept, until there is none.  Writes path
+ * [n_seqs][n] (the rows kept, in order, -1 behind them), accepted [n_seqs] (how many), next [n_seqs]
+ * (choices of the last row kept) and lengths_out [n_seqs] (may be the cache's lengths): lengths - counts
+ * + accepted.  The kept rows of K and V move to the places behind the context; those of the others are
+ * undefined.  A sequence without rows, or with more than it holds tokens, keeps none: next is -1 and
+ * the length stays.  parents, tokens and choices [n_seqs][n], n up to 256.  Arrays that are written
+ * share no memory with others of the call. */
+typedef struct shp_paged_accept_args {
+    const int32_t* counts;
+    const int32_t *parents, *tokens, *choices;
+    int32_t *path, *accepted, *next, *lengths_out;
+    int32_t n;
+} shp_paged_accept_args;
+int shp_paged_accept(shp_ctx* ctx, const shp_paged* cache, const shp_paged_accept_args* args);
+
 /* ---- how likely a token is -----------------------------------------------------------
  * For each of `rows` rows of vocab logits (row_stride floats apart): logprob = log softmax at
  * targets[r] (minus infinity for an id outside the vocabulary), entropy = -sum p log p, both in

@@ -93,6 +93,40 @@ class Cache8EvictArgs(C.Structure):
                 ("keep", C.c_int32), ("recent", C.c_int32)]
 
 
+class PagedStruct(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p),
+                ("lengths", C.c_void_p), ("n_seqs", C.c_int32), ("n_kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+                ("max_pages", C.c_int32), ("format", C.c_int32)]
+
+
+class PagedAppendArgs(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_seq", C.c_int64), ("k_row", C.c_int64),
+                ("k_head", C.c_int64), ("v_seq", C.c_int64), ("v_row", C.c_int64),
+                ("v_head", C.c_int64), ("q", C.c_void_p), ("q_out", C.c_void_p),
+                ("q_seq", C.c_int64), ("q_row", C.c_int64), ("q_head", C.c_int64),
+                ("o_seq", C.c_int64), ("o_row", C.c_int64), ("o_head", C.c_int64),
+                ("counts", C.c_void_p), ("offsets", C.c_void_p), ("inv_freq", C.c_void_p),
+                ("n", C.c_int32), ("n_heads", C.c_int32), ("rot", C.c_int32),
+                ("interleaved", C.c_int32)]
+
+
+class PagedAttendArgs(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_seq", C.c_int64),
+                ("q_row", C.c_int64), ("q_head", C.c_int64), ("o_seq", C.c_int64),
+                ("o_row", C.c_int64), ("o_head", C.c_int64), ("counts", C.c_void_p),
+                ("lse", C.c_void_p), ("slopes", C.c_void_p), ("prefix", C.c_void_p),
+                ("first", C.c_void_p), ("parents", C.c_void_p), ("n", C.c_int32),
+                ("n_heads", C.c_int32), ("window", C.c_int32), ("scale", C.c_float),
+                ("cap", C.c_float)]
+
+
+class PagedAcceptArgs(C.Structure):
+    _fields_ = [("counts", C.c_void_p), ("parents", C.c_void_p), ("tokens", C.c_void_p),
+                ("choices", C.c_void_p), ("path", C.c_void_p), ("accepted", C.c_void_p),
+                ("next", C.c_void_p), ("lengths_out", C.c_void_p), ("n", C.c_int32)]
+
+
 class LogprobsArgs(C.Structure):
     _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_int64), ("targets", C.c_void_p),
                 ("logprob", C.c_void_p), ("entropy", C.c_void_p), ("top_ids", C.c_void_p),
@@ -140,6 +174,12 @@ SIGNATURES = [
                                      C.POINTER(Cache8WeightsArgs)]),
     ("shp_cache8_evict", C.c_int, [C.c_void_p, C.POINTER(Cache8Struct), C.POINTER(Cache8Struct),
                                    C.POINTER(Cache8EvictArgs)]),
+    ("shp_paged_append", C.c_int, [C.c_void_p, C.POINTER(PagedStruct),
+                                   C.POINTER(PagedAppendArgs)]),
+    ("shp_paged_attend", C.c_int, [C.c_void_p, C.POINTER(PagedStruct),
+                                   C.POINTER(PagedAttendArgs)]),
+    ("shp_paged_accept", C.c_int, [C.c_void_p, C.POINTER(PagedStruct),
+                                   C.POINTER(PagedAcceptArgs)]),
     ("shp_token_logprobs", C.c_int, [C.c_void_p, C.POINTER(LogprobsArgs)]),
     ("shp_capture_begin", C.c_int, [C.c_void_p]),
     ("shp_capture_end", C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
