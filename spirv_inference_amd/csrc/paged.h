@@ -38,7 +38,17 @@ struct PagedQuery {
     int n, heads, group, window;
     float scale, cap;
 };
-int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format, const PagedQuery& q);
+// How attention splits the tokens of a sequence, and the floats of scratch that takes (0: none).
+struct PagedPlan {
+    int row_tiles;   // 16-row tiles a workgroup owns
+    int row_blocks;  // workgroups over the rows of one KV head
+    int splits;      // workgroups over the tokens of a sequence at most
+    int least;       // tiles a workgroup takes at least
+    size_t scratch;
+};
+PagedPlan paged_attend_plan(const Paged& c, int head_dim, int64_t rows, int cu_count, bool may_split);
+int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format, const PagedQuery& q,
+                        const PagedPlan& p, float* scratch, int* counters);
 
 struct PagedTree {
     const int32_t *counts, *parents, *tokens, *choices;
