@@ -34,6 +34,7 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned short us2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef bf16 b8 __attribute__((ext_vector_type(8)));
@@ -65,17 +66,6 @@ __device__ __forceinline__ float max_over_groups(float x) {
 __device__ __forceinline__ float sum_over_groups(float x) {
     return over_groups(x, [](float a, float b) { return a + b; });
 }
-__device__ __forceinline__ int min_over_rows(int x) {
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) x = min(x, __shfl_xor(x, o));
-    return __builtin_amdgcn_readfirstlane(x);
-}
-__device__ __forceinline__ int max_over_rows(int x) {
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) x = max(x, __shfl_xor(x, o));
-    return __builtin_amdgcn_readfirstlane(x);
-}
-
 // Two numbers as pieces, next to each other in a word of each.
 template <class E>
 __device__ __forceinline__ void cut(float x, float y, unsigned* piece) {
@@ -108,16 +98,8 @@ __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// The bits of an infinity, and of 1 (16-bit types).
+// The bits of an infinity.
 template <class E> constexpr unsigned kInf = kF32<E> ? 0x7f800000u : kPieces<E> == 2 ? 0x7c00u : 0x7f80u;
-template <class E> constexpr unsigned kOne = kPieces<E> == 2 ? 0x3c00u : 0x3f80u;
-// Whether the value with these bits is a NaN or the infinity of this sign.
-template <class E>
-__device__ __forceinline__ bool not_finite(unsigned x, int minus) {
-    constexpr unsigned kSign = kF32<E> ? 0x80000000u : 0x8000u;
-    const unsigned a = x & (kSign - 1);
-    return a > kInf<E> || x == (minus ? kSign | kInf<E> : kInf<E>);
-}
 // Dimension d (of two in a word) of two tokens' words, side by side.
 __device__ __forceinline__ unsigned dims_of(unsigned first, unsigned second, int d) {
     return __builtin_amdgcn_perm(second, first, d & 1 ? 0x07060302u : 0x05040100u);
@@ -137,10 +119,17 @@ __device__ __forceinline__ uint64_t below(int n) {
     return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1;
 }
 
+// All ones where bit n is set: selects by it need no scalar registers.
+__device__ __forceinline__ unsigned mask_of(uint64_t bits, int n) {
+    return (unsigned)__builtin_amdgcn_sbfe((int)(unsigned)(n < 32 ? bits : bits >> 32), n & 31, 1);
+}
+
 // 2^(m - top), also where both are minus infinity or infinity.
 __device__ __forceinline__ float factor_of(float m, float top) {
     return m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
 }
+// What sums of weights times V are to be multiplied by, from the sum of the weights.
+__device__ __forceinline__ float inverse(float l) { return l == 0.0f ? 0.0f : 1.0f / l; }
 // The log of a row's sum from its shifted maximum and sum of weights.
 __device__ __forceinline__ float log_sum(float m, float l) {
     return l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
@@ -153,208 +142,327 @@ struct Tree {
     uint16_t parent[kTreeRows], depth[kTreeRows];
 };
 
-// Which tokens a row sees: [first, len) of those in [lo, hi), before `prefix` or among its tree's.
+// A KV head of a sequence and its rows.
+struct Unit {
+    int s, h, len, count, begin, nrows;
+    int window, prefix_all, prefix;  // prefix: of it what is no tree's
+    bool drafted;
+};
+__device__ __forceinline__ Unit unit_of(const Paged& c, const PagedQuery& q, int s, int h) {
+    Unit u;
+    u.s = s;
+    u.h = h;
+    u.len = paged_length(c, u.s);
+    u.count = paged_count(q.counts, q.n, u.s);
+    u.begin = u.len - u.count;
+    u.nrows = u.count * q.group;
+    u.drafted = q.parents != nullptr;
+    u.window = q.window ? min(q.window, 1 << 30) : 1 << 30;
+    u.prefix_all = q.prefix ? min(max(q.prefix[u.s], 0), u.len) : 0;
+    u.prefix = u.drafted ? min(u.prefix_all, max(u.begin, 0)) : u.prefix_all;
+    return u;
+}
+
+// What a workgroup does: a block of rows of a KV head, and of the tiles that they see the shares
+// z * share .. of `shares`.  With target = 0 it is a place in the grid, and all tiles.  Else the blocks and the tiles
+// of all sequences are counted and cut into shares of one size, about `target` of them, which evens out
+// sequences of different lengths; a workgroup finds its own in their running sum, or that there is none for it.
+struct Task {
+    int s, h, block, z, share, shares, first;  // first: the place of its rows' first part and of their counter
+    bool any;
+};
+template <int T, int ROWS>
+__device__ __forceinline__ Task task_of(const Paged& c, const PagedQuery& q, int target, int least) {
+    Task k;
+    if (target == 0) {
+        const int id = (int)blockIdx.x;
+        k.s = (int)fdiv((unsigned)id, q.by_kv);
+        k.h = id - k.s * c.kv;
+        k.block = (int)(gridDim.y - 1 - blockIdx.y);  // those that see most begin first
+        k.z = 0;
+        k.share = 1 << 30;
+        k.shares = 1;
+        k.first = 0;
+        k.any = true;
+        return k;
+    }
+    const int lane = threadIdx.x & 63;
+    // blocks of sequence s, and the tiles that a block sees of it, no more than those that a window touches
+    const int most = q.window && !q.prefix ? (min(q.window, 1 << 22) + q.n) / T + 2 : 1 << 22;
+    auto size = [&](int s, int& blocks, int& tiles) __attribute__((always_inline)) {
+        const bool real = s < c.n_seqs;
+        const int len = real ? paged_length(c, s) : 0, count = real ? paged_count(q.counts, q.n, s) : 0;
+        blocks = (count * q.group + ROWS - 1) / ROWS;
+        tiles = max(min((len + T - 1) / T, most), 1);
+    };
+    int blocks, tiles, top = 1;
+    float all = 0.0f;
+    for (int s0 = 0; s0 < c.n_seqs; s0 += 64) {
+        size(s0 + lane, blocks, tiles);
+        all += (float)blocks * (float)tiles;
+        top = max(top, tiles);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        all += __shfl_xor(all, o);
+        top = max(top, __shfl_xor(top, o));
+    }
+    // (32 shares of a block at most, whose parts one workgroup joins)
+    k.share = max(max((int)(all * (float)c.kv / (float)target) + 1, (top + 31) / 32), least);
+    k.share = __builtin_amdgcn_readfirstlane(k.share);
+    // running sums of the sequences' workgroups, 64 sequences at a time
+    int mine, to;
+    auto count_up = [&](int s0) __attribute__((always_inline)) {
+        if (c.n_seqs > 64) size(s0 + lane, blocks, tiles);
+        to = mine = c.kv * blocks * ((tiles + k.share - 1) / k.share);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_up(to, o);
+            if (lane >= o) to += x;
+        }
+        return __builtin_amdgcn_readlane(to, 63);
+    };
+    int n = 0;
+    for (int s0 = 0; s0 < c.n_seqs; s0 += 64) n += count_up(s0);
+    // Workgroups with numbers 8 apart run on one XCD, one after the other: each XCD gets a run of the tasks, in which
+    // blocks of rows that read the same tokens are neighbours.
+    const int run = (n + 7) / 8, id = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
+    k.any = (int)(blockIdx.x >> 3) < run && id < n;
+    for (int s0 = 0, sum = 0; k.any; s0 += 64) {
+        const int all_here = c.n_seqs > 64 ? count_up(s0) : n;
+        const uint64_t behind = __ballot(sum + to > id);
+        if (behind) {
+            const int at = __builtin_ctzll(behind);
+            k.s = s0 + at;
+            const int nb = __builtin_amdgcn_readlane(blocks, at);
+            const int start = sum + __builtin_amdgcn_readlane(to, at) - __builtin_amdgcn_readlane(mine, at);
+            k.shares = (__builtin_amdgcn_readlane(tiles, at) + k.share - 1) / k.share;
+            const int off = id - start, rest = off / nb;
+            k.block = off - rest * nb;
+            k.h = rest / k.shares;
+            k.z = rest - k.h * k.shares;
+            k.first = start + (k.h * nb + k.block) * k.shares;
+            break;
+        }
+        sum += all_here;
+    }
+    return k;
+}
+
+// The workgroup's 256 threads walk up the tree from a row each.
+__device__ __forceinline__ void climb(const PagedQuery& q, const Unit& u, Tree& tree) {
+    const int i = threadIdx.x;
+    if (i < u.count) {
+        const int p = q.parents[(int64_t)u.s * q.n + i];
+        tree.parent[i] = (uint16_t)(p >= 0 && p < i ? p : 0xffff);
+    }
+    __syncthreads();
+    if (i < u.count) {
+        uint64_t up[kTreeRows / 64] = {};
+        int steps = 0;
+        for (int v = i; v != 0xffff; v = tree.parent[v], ++steps)  // falls
+            if (steps < u.window || u.begin + v < u.prefix_all) {
+#pragma unroll
+                for (int w = 0; w < kTreeRows / 64; ++w) up[w] |= v >> 6 == w ? 1ull << (v & 63) : 0ull;
+            }
+        tree.depth[i] = (uint16_t)(steps - 1);
+#pragma unroll
+        for (int w = 0; w < kTreeRows / 64; ++w) tree.above[i][w] = up[w];
+    }
+    __syncthreads();
+}
+
+// Bounds of what rows [ra, rb) see, the same for all lanes: nothing outside [low, high) and
+// [least_first, prefix); each row all of [open_lo, open_hi), if that is not empty.
+struct Span {
+    int low, high, least_first, open_lo, open_hi;
+};
+__device__ __forceinline__ Span span_of(const PagedQuery& q, const Unit& u, int ra, int rb) {
+    const int i0 = (int)fdiv((unsigned)ra, q.by_group), i1 = (int)fdiv((unsigned)(rb - 1), q.by_group);
+    const int p0 = u.begin + i0, p1 = u.begin + i1;
+    Span v;
+    // a tree's rows are at positions from begin up to their place
+    v.low = max((u.drafted ? u.begin : p0) - u.window + 1, 0);
+    v.high = max(p1 + 1, 0);
+    v.open_lo = p0 < 0 ? 0x7fffffff : max(p1 - u.window + 1, 0);
+    v.open_hi = u.drafted ? u.begin : p0 + 1;
+    v.least_first = 0;
+    if (q.first) {
+        int a = 0x7fffffff, b = 0;
+        for (int i = i0 + (threadIdx.x & 63); i <= i1; i += 64) {
+            const int f = max(q.first[(int64_t)u.s * q.n + i], 0);
+            a = min(a, f);
+            b = max(b, f);
+        }
+#pragma unroll
+        for (int o = 32; o > 0; o >>= 1) {
+            a = min(a, __shfl_xor(a, o));
+            b = max(b, __shfl_xor(b, o));
+        }
+        v.least_first = __builtin_amdgcn_readfirstlane(a);
+        v.low = max(v.low, v.least_first);
+        v.open_lo = max(v.open_lo, __builtin_amdgcn_readfirstlane(b));
+    }
+    return v;
+}
+
+// The tiles of T tokens that any row of a span sees a token of: of the prefix [a0, a0 + na), then from b0 on.
+template <int T>
+struct Tiles {
+    int a0, na, b0, all;
+    __device__ __forceinline__ Tiles(const Unit& u, const Span& v) {
+        a0 = v.least_first / T;
+        na = u.prefix > v.least_first ? (u.prefix + T - 1) / T - a0 : 0;
+        b0 = na ? max(v.low / T, a0 + na) : v.low / T;
+        all = na + max((min(v.high, u.len) + T - 1) / T - b0, 0);
+    }
+    __device__ __forceinline__ int begin(int k) const { return (k < na ? a0 + k : b0 + k - na) * T; }
+};
+
+// Which tokens a row sees: [first, len) of those in [lo, hi), before the prefix or among its tree's.
 struct Sight {
     int lo, hi, first, position, node;
 };
 
+// 16 * MT rows of a wavefront, and what it has of their softmax.
 template <class E, int D, int MT>
-__global__ __launch_bounds__(256, 2) void paged_attend_kernel(Paged c, PagedQuery q, int least, float* part,
-                                                              int* counters) {
-    constexpr bool F32 = kF32<E>;
-    constexpr int NP = kPieces<E>, NO = D / 16, TT = kTile<E, D>, NJ = TT / 16;
-    constexpr int NQ = F32 ? D / 16 : D / 32;  // 16-byte pieces of a row of K that a lane takes
-    constexpr int ROWS = 16 * MT, WAVES = 4, PW = D + 4;
-    constexpr int EX = MT * (NO * 4 + 2) * 64;
-    __shared__ __attribute__((aligned(16))) float ex[2][EX];
-    static_assert(sizeof(Tree) <= sizeof(ex), "the tree lies where the wavefronts' parts go later");
-    __shared__ int arrived;
-    Tree& tree = *reinterpret_cast<Tree*>(&ex[0][0]);
-    const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int sh = blockIdx.x, s = sh / c.kv, h = sh - s * c.kv;
-    const int len = paged_length(c, s), count = paged_count(q.counts, q.n, s), begin = len - count;
-    const int nrows = count * q.group;
-    const int r0 = (int)(gridDim.y - 1 - blockIdx.y) * ROWS;  // those that see most begin first
-    if (r0 >= nrows) return;
-    const bool drafted = q.parents != nullptr;
-    const int window = q.window ? min(q.window, 1 << 30) : 1 << 30;
-    const int prefix_all = q.prefix ? min(max(q.prefix[s], 0), len) : 0;
-    const int prefix = drafted ? min(prefix_all, max(begin, 0)) : prefix_all;
-
-    if (drafted) {
-        const int i = threadIdx.x;
-        if (i < count) {
-            const int p = q.parents[(int64_t)s * q.n + i];
-            tree.parent[i] = (uint16_t)(p >= 0 && p < i ? p : 0xffff);
-        }
-        __syncthreads();
-        if (i < count) {
-            uint64_t up[kTreeRows / 64] = {};
-            int steps = 0;
-            for (int u = i; u != 0xffff; u = tree.parent[u], ++steps)  // falls
-                if (steps < window || begin + u < prefix_all) {
-#pragma unroll
-                    for (int w = 0; w < kTreeRows / 64; ++w)
-                        up[w] |= u >> 6 == w ? 1ull << (u & 63) : 0ull;
-                }
-            tree.depth[i] = (uint16_t)(steps - 1);
-#pragma unroll
-            for (int w = 0; w < kTreeRows / 64; ++w) tree.above[i][w] = up[w];
-        }
-        __syncthreads();
-    }
-
-    // the lane's rows; those behind the last repeat it
-    Sight see[MT];
-    float slope[MT];
-    const float* qrow[MT];
-    int low = 0x7fffffff, high = 0, least_first = 0x7fffffff, open_lo = 0, open_hi = 0x7fffffff;
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        const int r = min(r0 + 16 * t + li, nrows - 1), i = r / q.group, head = h * q.group + r - i * q.group;
-        const int place = begin + i;
-        Sight& v = see[t];
-        v.node = i;
-        v.position = drafted ? begin + tree.depth[i] : place;
-        v.hi = drafted ? begin : place + 1;
-        v.lo = max(v.position - window + 1, 0);
-        v.first = q.first ? max(q.first[(int64_t)s * q.n + i], 0) : 0;
-        if (place < 0) v.first = 0x7fffffff;  // sees nothing
-        slope[t] = q.slopes ? q.slopes[head] * kLog2e : 0.0f;
-        qrow[t] = q.q + s * q.q_seq + i * q.q_row + head * q.q_head;
-        low = min(low, max(v.lo, v.first));
-        high = max(high, place < 0 ? 0 : drafted ? place + 1 : v.hi);
-        least_first = min(least_first, v.first);
-        open_lo = max(open_lo, max(v.lo, v.first));
-        open_hi = min(open_hi, v.hi);
-    }
-    low = min_over_rows(low);
-    high = max_over_rows(high);
-    least_first = min_over_rows(least_first);
-    open_lo = max_over_rows(open_lo);
-    open_hi = min_over_rows(open_hi);
-    // a token of a tree may be nearer by position than by place
-    if (drafted) low = min(low, max(begin, 0));
-
-    // the tiles that any row sees a token of: of the prefix [a0, a0 + na), then [b0, b0 + nb)
-    const int a0 = min(least_first, prefix) / TT, na = prefix > least_first ? (prefix + TT - 1) / TT - a0 : 0;
-    const int b0 = na ? max(low / TT, a0 + na) : low / TT, nb = max((min(high, len) + TT - 1) / TT - b0, 0);
-    const int tiles = na + nb;
-    const int share = max((tiles + (int)gridDim.z - 1) / (int)gridDim.z, least);
-    const int splits = max((tiles + share - 1) / share, 1);
-    if ((int)blockIdx.z >= splits) return;
-    const int tile0 = (int)blockIdx.z * share, tile1 = min(tiles, tile0 + share);
-
-    // q's pieces in the B layout
-    float m[MT], l[MT], back[MT];
-    f4 o[MT][NO];
-    u4 qp[MT][NQ][NP];
-    const bool capped = q.cap > 0.0f;
-    const float factor = capped ? q.scale / q.cap : q.scale * kLog2e;
-#pragma unroll
-    for (int t = 0; t < MT; ++t) {
-        m[t] = -__builtin_inff();
-        l[t] = 0.0f;
-        back[t] = 1.0f;
-#pragma unroll
-        for (int d = 0; d < NO; ++d) o[t][d] = f4{0.f, 0.f, 0.f, 0.f};
-        if constexpr (F32) {
-#pragma unroll
-            for (int a = 0; a < NQ; ++a)
-                qp[t][a][0] = __builtin_bit_cast(u4, *reinterpret_cast<const f4*>(qrow[t] + 16 * a + 4 * g) * factor);
-        } else {
-            f4 v[2 * NQ];
-            float top = 0.0f;
-#pragma unroll
-            for (int a = 0; a < 2 * NQ; ++a) {
-                v[a] = *reinterpret_cast<const f4*>(qrow[t] + 32 * (a >> 1) + 8 * g + 4 * (a & 1)) * factor;
-#pragma unroll
-                for (int b = 0; b < 4; ++b) top = fmaxf(top, fabsf(v[a][b]));
-            }
-            if constexpr (NP == 2) {
-                top = max_over_groups(top);
-                const int e = min(kQBits - __builtin_amdgcn_frexp_expf(top), 100);
-                back[t] = __builtin_amdgcn_ldexpf(1.0f, -e);
-#pragma unroll
-                for (int a = 0; a < 2 * NQ; ++a)
-#pragma unroll
-                    for (int b = 0; b < 4; ++b) v[a][b] = __builtin_amdgcn_ldexpf(v[a][b], e);
-            }
-#pragma unroll
-            for (int a = 0; a < NQ; ++a)
-#pragma unroll
-                for (int b = 0; b < 4; ++b) {
-                    unsigned piece[NP];
-                    cut<E>(v[2 * a + (b >> 1)][2 * (b & 1)], v[2 * a + (b >> 1)][2 * (b & 1) + 1], piece);
-#pragma unroll
-                    for (int p = 0; p < NP; ++p) qp[t][a][p][b] = piece[p];
-                }
-        }
-    }
-    const float shift = NP == 2 ? (float)-kLift : (float)(32 - __builtin_clz(max(len, 1)));
-    const E* const kb = (const E*)c.k;
-    const E* const vb = (const E*)c.v;
-    const int last = max(len - 1, 0);
-    // what lies in a lane's registers of a tile: tokens 16 j + li of K, and of V those of its k slots
-    constexpr int VW = F32 ? D / 64 : 1;         // loads of a row of V
-    constexpr int VB = F32 ? 4 : D / 32;         // words of each
+struct Wave {
+    static constexpr bool F32 = kF32<E>;
+    static constexpr int NP = kPieces<E>, NO = D / 16, TT = kTile<E, D>, NJ = TT / 16;
+    static constexpr int NQ = F32 ? D / 16 : D / 32;  // 16-byte pieces of a row of K that a lane takes
+    static constexpr int VW = F32 ? D / 64 : 1;       // loads of a row of V
+    static constexpr int VB = F32 ? 4 : D / 32;       // words of each
+    static constexpr int PW = D + 4;                  // floats of a row's part: sums, maximum, weight, two of padding
     typedef unsigned VWord __attribute__((ext_vector_type(VB)));
+    // The lowest of three pieces of 32 rows of 128 dimensions stays in LDS, which the registers do not hold with
+    // the other two (a tree of 60 rows x 4 heads 16 times on 4,100 tokens: 610 us where they spill).
+    static constexpr int NL = NP == 3 && MT == 2 && D == 128 ? 1 : 0, NR = NP - NL;
 
-    for (int at = tile0 + wave; at < tile1; at += WAVES) {
-        const int t0 = (at < na ? a0 + at : b0 + at - na) * TT;
-        u4 kr[NJ][NQ];
-        VWord vr[NJ][4][VW];
-        uint64_t there = ~0ull;
+    f4 o[MT][NO];
+    u4 qp[MT][NQ][NR];
+    float m[MT], l[MT], slope[MT], back[MT];
+    Sight see[MT];
+
+    // Rows from r0 on; those behind the last repeat it.  raw: the lane's part of them.
+    __device__ __forceinline__ void begin(const PagedQuery& q, const Unit& u, const Tree& tree, int r0, f4 raw[MT][2 * D / 32]) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            const int t = min(t0 + 16 * j, last & ~15);  // a page holds whole groups of 16
-            int page = page_of(c, s, t);
-            if (page < 0) {
-                page = 0;
-                there &= ~(0xffffull << (16 * j));
-            }
-            const int64_t row = row_of(c, page, h, t) * D;
+        for (int t = 0; t < MT; ++t) {
+            const int r = min(r0 + 16 * t + li, u.nrows - 1), i = (int)fdiv((unsigned)r, q.by_group);
+            const int head = u.h * q.group + r - i * q.group, place = u.begin + i;
+            const float* x = q.q + u.s * q.q_seq + i * q.q_row + head * q.q_head;
 #pragma unroll
-            for (int a = 0; a < NQ; ++a)
-                kr[j][a] = *reinterpret_cast<const u4*>(kb + row + li * D + (F32 ? 16 * a + 4 * g : 32 * a + 8 * g));
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int w = 0; w < VW; ++w)
-                    vr[j][i][w] = *reinterpret_cast<const VWord*>(vb + row + (4 * g + i) * D + (F32 ? 64 * w + 4 * li : NO * li));
+            for (int a = 0; a < D / 16; ++a)
+                raw[t][a] = *reinterpret_cast<const f4*>(x + (F32 ? 16 * a + 4 * g : 32 * (a >> 1) + 8 * g + 4 * (a & 1)));
+            Sight& v = see[t];
+            v.node = i;
+            v.position = u.drafted ? u.begin + tree.depth[i] : place;
+            v.hi = u.drafted ? u.begin : place + 1;
+            v.lo = max(v.position - u.window + 1, 0);
+            v.first = q.first ? max(q.first[(int64_t)u.s * q.n + i], 0) : 0;
+            if (place < 0) v.first = 0x7fffffff;  // sees nothing
+            slope[t] = q.slopes ? q.slopes[head] * kLog2e : 0.0f;
         }
-        // whether every row sees the whole tile
-        const bool edge = (~there & below(TT)) || t0 < open_lo || t0 + TT > open_hi;
+    }
+    // The rows' pieces in the B layout, times the scale; nothing seen yet.  low: those that LDS holds.
+    __device__ __forceinline__ void pieces(const PagedQuery& q, f4 v[MT][2 * D / 32], u4* low) {
+        const float factor = q.cap > 0.0f ? q.scale / q.cap : q.scale * kLog2e;
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            back[t] = 1.0f;
+#pragma unroll
+            for (int a = 0; a < D / 16; ++a) v[t][a] *= factor;
+            if constexpr (F32) {
+#pragma unroll
+                for (int a = 0; a < NQ; ++a) qp[t][a][0] = __builtin_bit_cast(u4, v[t][a]);
+            } else {
+                if constexpr (NP == 2) {
+                    float top = 0.0f;
+#pragma unroll
+                    for (int a = 0; a < 2 * NQ; ++a)
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) top = fmaxf(top, fabsf(v[t][a][b]));
+                    top = max_over_groups(top);
+                    const int e = min(kQBits - __builtin_amdgcn_frexp_expf(top), 100);
+                    back[t] = __builtin_amdgcn_ldexpf(1.0f, -e);
+#pragma unroll
+                    for (int a = 0; a < 2 * NQ; ++a)
+#pragma unroll
+                        for (int b = 0; b < 4; ++b) v[t][a][b] = __builtin_amdgcn_ldexpf(v[t][a][b], e);
+                }
+#pragma unroll
+                for (int a = 0; a < NQ; ++a) {
+                    u4 lowest;
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) {
+                        unsigned piece[NP];
+                        cut<E>(v[t][2 * a + (b >> 1)][2 * (b & 1)], v[t][2 * a + (b >> 1)][2 * (b & 1) + 1], piece);
+#pragma unroll
+                        for (int p = 0; p < NR; ++p) qp[t][a][p][b] = piece[p];
+                        lowest[b] = piece[NP - 1];
+                    }
+                    if (NL && threadIdx.x < 64) low[(t * NQ + a) * 64 + threadIdx.x] = lowest;
+                }
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);  // the sums take the registers that the rows had
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            m[t] = -__builtin_inff();
+            l[t] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < NO; ++d) o[t][d] = f4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+
+    // A tile from token t0 on.  key(j, a) gives 16 bytes of token 16 j + l % 16, value(j, i, w) words of token
+    // 16 j + 4 g + i; `there` says which of its tokens have a page.
+    // number(token, dimension) is one of the tile's values.
+    template <class K, class V, class N>
+    __device__ __forceinline__ void step(const PagedQuery& q, const Unit& u, const Tree& tree, const Span& span, float shift,
+                                         int t0, uint64_t there, const u4* low, K key, V value, N number) {
+        const int g = (threadIdx.x & 63) >> 4;
+        // whether some row does not see some token
+        const bool edge = (~there & below(TT)) || t0 < span.open_lo || t0 + TT > span.open_hi;
         f4 sc[MT][NJ];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
+        for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int t = 0; t < MT; ++t) sc[t][j] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int a = 0; a < NQ; ++a)
+        for (int a = 0; a < NQ; ++a) {
+            if constexpr (NL) {
+                u4 lowest[MT];
 #pragma unroll
-                for (int p = NP - 1; p >= 0; --p)
+                for (int t = 0; t < MT; ++t) lowest[t] = low[(t * NQ + a) * 64 + (threadIdx.x & 63)];
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        if constexpr (F32) {
+                for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                            for (int b = 0; b < 4; ++b)
-                                sc[t][j] = mfma4(__uint_as_float(kr[j][a][b]), __uint_as_float(qp[t][a][0][b]), sc[t][j]);
-                        } else {
-                            sc[t][j] = mfma32<E>(kr[j][a], qp[t][a][p], sc[t][j]);
+                    for (int t = 0; t < MT; ++t) sc[t][j] = mfma32<E>(key(j, a), lowest[t], sc[t][j]);
+            }
+#pragma unroll
+            for (int p = NR - 1; p >= 0; --p)
+#pragma unroll
+                for (int b = 0; b < (F32 ? 4 : 1); ++b)
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int t = 0; t < MT; ++t) {
+                            if constexpr (F32)
+                                sc[t][j] = mfma4(__uint_as_float(key(j, a)[b]), __uint_as_float(qp[t][a][0][b]), sc[t][j]);
+                            else
+                                sc[t][j] = mfma32<E>(key(j, a), qp[t][a][p], sc[t][j]);
                         }
-                    }
         }
         // sc[t][j][i]: token t0 + 16 j + 4 g + i, row r0 + 16 t + li
-        uint64_t seen[MT];  // bit 16 j + i: the lane's tokens
+        uint64_t seen[MT];  // the row's tokens of the tile
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             if constexpr (NP == 2) {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) sc[t][j] *= back[t];
             }
-            if (capped) {
+            if (q.cap > 0.0f) {
                 const float top = q.cap * kLog2e;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
@@ -362,40 +470,49 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(Paged c, PagedQuer
                     for (int i = 0; i < 4; ++i) sc[t][j][i] = top * tanh_of(sc[t][j][i]);
             }
             if (q.slopes) {
-                const bool mixed = drafted && t0 + TT > begin;
+                if (u.drafted && t0 + TT > u.begin) {
 #pragma unroll
-                for (int j = 0; j < NJ; ++j)
+                    for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        int at_k = t0 + 16 * j + 4 * g + i;
-                        if (mixed && at_k >= begin && at_k < len) at_k = begin + tree.depth[at_k - begin];
-                        sc[t][j][i] -= slope[t] * fabsf((float)(see[t].position - at_k));
-                    }
+                        for (int i = 0; i < 4; ++i) {
+                            const int at = t0 + 16 * j + 4 * g + i, up = min(max(at - u.begin, 0), max(u.count - 1, 0));
+                            const int position = at < u.begin ? at : u.begin + tree.depth[up];
+                            sc[t][j][i] -= slope[t] * fabsf((float)(see[t].position - position));
+                        }
+                } else {
+                    const float far = (float)(see[t].position - t0 - 4 * g);
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[t][j][i] -= slope[t] * fabsf(far - (float)(16 * j + i));
+                }
             }
             seen[t] = ~0ull;
             if (edge) {
                 const Sight& v = see[t];
-                uint64_t bits = (below(v.hi - t0) & ~below(v.lo - t0)) | below(prefix - t0);
-                if (drafted && t0 + TT > begin) {
+                uint64_t bits = (below(v.hi - t0) & ~below(v.lo - t0)) | below(u.prefix - t0);
+                if (u.drafted && t0 + TT > u.begin) {
                     // the tree's bits from t0 on: those of rows t0 - begin ..
                     const uint64_t* up = tree.above[v.node];
-                    const int u = t0 - begin;
-                    if (u < 0) {
-                        bits |= up[0] << -u;  // -u < TT
+                    const int from = t0 - u.begin;
+                    if (from < 0) {
+                        bits |= up[0] << -from;  // -from < TT
                     } else {
-                        const int w = u >> 6, b = u & 63;
+                        const int w = from >> 6, b = from & 63;
                         uint64_t x = w < kTreeRows / 64 ? up[w] >> b : 0ull;
                         if (b && w + 1 < kTreeRows / 64) x |= up[w + 1] << (64 - b);
                         bits |= x;
                     }
                 }
-                bits &= below(len - t0) & ~below(v.first == 0x7fffffff ? 64 : v.first - t0) & there;
-                seen[t] = bits >> (4 * g);
+                bits &= below(u.len - t0) & ~below(v.first == 0x7fffffff ? 64 : v.first - t0) & there;
+                seen[t] = bits;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (!(seen[t] >> (16 * j + i) & 1)) sc[t][j][i] = -__builtin_inff();
+                    for (int i = 0; i < 4; ++i) {
+                        const unsigned w = mask_of(bits >> (4 * g), 16 * j + i);
+                        sc[t][j][i] = __uint_as_float((__float_as_uint(sc[t][j][i]) & w) | (0xff800000u & ~w));
+                    }
             }
             float best = -__builtin_inff();
 #pragma unroll
@@ -413,20 +530,39 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(Paged c, PagedQuer
                 m[t] = top;
             }
             float sum = 0.0f;
+            if (edge) {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
+                for (int j = 0; j < NJ; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float w = __builtin_amdgcn_exp2f(sc[t][j][i] - m[t]);
-                    sc[t][j][i] = edge && !(seen[t] >> (16 * j + i) & 1) ? 0.0f : w;
-                    sum += sc[t][j][i];
-                }
+                    for (int i = 0; i < 4; ++i) {
+                        const float w = __builtin_amdgcn_exp2f(sc[t][j][i] - m[t]);
+                        sc[t][j][i] = __uint_as_float(__float_as_uint(w) & mask_of(seen[t] >> (4 * g), 16 * j + i));
+                        sum += sc[t][j][i];
+                    }
+            } else {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        sc[t][j][i] = __builtin_amdgcn_exp2f(sc[t][j][i] - m[t]);
+                        sum += sc[t][j][i];
+                    }
+            }
             l[t] += sum;
         }
 
+        VWord vr[NJ][4][VW];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int w = 0; w < VW; ++w) vr[j][i][w] = value(j, i, w);
         // Where some row does not see some token, a value that is not finite would spoil that row too: such a
-        // value is added to the rows that see it, as an infinity of its sign, a NaN as both, and taken out.
+        // value is added to the rows that see it and taken out.
         if (edge) {
+            // the largest exponents, of 16-bit values in both halves of a word
+            us2 top2 = {0, 0};
             unsigned top = 0;
 #pragma unroll
             for (int j = 0; j < NJ; ++j)
@@ -436,43 +572,22 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(Paged c, PagedQuer
                     for (int w = 0; w < VW; ++w)
 #pragma unroll
                         for (int b = 0; b < VB; ++b) {
-                            const unsigned x = vr[j][i][w][b] & 0x7fffffffu;
-                            top = max(top, F32 ? x : max(x, (x & 0x7fffu) << 16));
+                            const unsigned x = vr[j][i][w][b];
+                            if constexpr (F32) top = max(top, x & 0x7fffffffu);
+                            else top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(us2, x & 0x7fff7fffu));
                         }
-            if (__any(top >= kInf<E> << (F32 ? 0 : 16))) {
+            if constexpr (!F32) top = max((unsigned)top2.x, (unsigned)top2.y);
+            if (__any(top >= kInf<E>)) {
+#pragma unroll 1
+                for (int token = 0; token < TT; ++token)
 #pragma unroll
-                for (int d = 0; d < NO; ++d)
+                    for (int d = 0; d < NO; ++d)
 #pragma unroll
-                    for (int minus = 0; minus < 2; ++minus)
+                        for (int i = 0; i < 4; ++i) {
+                            const float x = number(token, dim_of(g, d, i));
 #pragma unroll
-                        for (int t = 0; t < MT; ++t) {
-                            f4 hits = {0.f, 0.f, 0.f, 0.f};
-                            if constexpr (F32) {
-#pragma unroll
-                                for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i)
-                                        hits = mfma4(not_finite<E>(vr[j][i][d >> 2][d & 3], minus) ? 1.0f : 0.0f,
-                                                     seen[t] >> (16 * j + i) & 1 ? 1.0f : 0.0f, hits);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < NJ / 2; ++e) {
-                                    u4 x, y;
-#pragma unroll
-                                    for (int b = 0; b < 4; ++b) {
-                                        const int j = 2 * e + (b >> 1), i = 2 * (b & 1);
-                                        const unsigned v = dims_of(vr[j][i][0][d >> 1], vr[j][i + 1][0][d >> 1], d);
-                                        x[b] = (not_finite<E>(v & 0xffffu, minus) ? kOne<E> : 0u) |
-                                               (not_finite<E>(v >> 16, minus) ? kOne<E> << 16 : 0u);
-                                        y[b] = (seen[t] >> (16 * j + i) & 1 ? kOne<E> : 0u) |
-                                               (seen[t] >> (16 * j + i + 1) & 1 ? kOne<E> << 16 : 0u);
-                                    }
-                                    hits = mfma32<E>(x, y, hits);
-                                }
-                            }
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (hits[i] > 0.0f) o[t][d][i] += minus ? -__builtin_inff() : __builtin_inff();
+                            for (int t = 0; t < MT; ++t)
+                                if (!(fabsf(x) <= 3.4028234663852886e+38f) && (seen[t] >> token & 1)) o[t][d][i] += x;
                         }
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
@@ -482,13 +597,14 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(Paged c, PagedQuer
                         for (int w = 0; w < VW; ++w)
 #pragma unroll
                             for (int b = 0; b < VB; ++b) {
-                                unsigned& x = *(reinterpret_cast<unsigned*>(&vr[j][i][w]) + b);
+                                unsigned x = vr[j][i][w][b];
                                 if constexpr (F32) {
                                     if ((x & kInf<E>) == kInf<E>) x = 0u;
                                 } else {
                                     if ((x & kInf<E>) == kInf<E>) x &= 0xffff0000u;
                                     if ((x >> 16 & kInf<E>) == kInf<E>) x &= 0xffffu;
                                 }
+                                vr[j][i][w][b] = x;
                             }
             }
         }
@@ -534,199 +650,313 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(Paged c, PagedQuer
         }
     }
 
-    // the lane's numbers once more, which the loop's registers need not hold so
-    const int ln = __lane_id(), row = ln & 15, quad = ln >> 4, tid = wave * 64 + ln;
+    // The dimension that o[t][d][i] of lane group g is.
+    static __device__ __forceinline__ int dim_of(int g, int d, int i) {
+        return !F32 && D == 128 ? 32 * g + 8 * i + d : 64 * (d >> 2) + 16 * g + 4 * i + (d & 3);
+    }
+    // Four dimensions next to each other of the lane's, and the first of them.
+    __device__ __forceinline__ f4 run(int t, int n) const {
+        constexpr bool WIDE = !F32 && D == 128;  // a lane holds 8 dimensions in a row, not 4
+        const int i = WIDE ? n >> 1 : n & 3, x = WIDE ? 4 * (n & 1) : 4 * (n >> 2);
+        return f4{o[t][x][i], o[t][x + 1][i], o[t][x + 2][i], o[t][x + 3][i]};
+    }
+    static __device__ __forceinline__ int dim(int quad, int n) {
+        return !F32 && D == 128 ? 32 * quad + 4 * n : 64 * (n >> 2) + 16 * quad + 4 * (n & 3);
+    }
+    // The results of rows r0 .., which saw all of their tokens.
+    __device__ __forceinline__ void store(const PagedQuery& q, const Unit& u, int r0) const;
+    // The same as parts of the rows, `row` floats in front of the first.
+    __device__ __forceinline__ void store_part(__amdgpu_buffer_rsrc_t to, int row, int rows) const {
+        const int ln = __lane_id(), li = ln & 15, quad = ln >> 4;
 #pragma unroll
-    for (int t = 0; t < MT; ++t) l[t] = sum_over_groups(l[t]);
+        for (int t = 0; t < MT; ++t) {
+            const int r = 16 * t + li;
+            if (r >= rows) continue;
+            const unsigned at = (unsigned)((row + r) * PW) * 4u;
+#pragma unroll
+            for (int n = 0; n < NO; ++n) {
+                const f4 x = run(t, n);
+                st_coh16(to, at + dim(quad, n) * 4u, make_float4(x.x, x.y, x.z, x.w));
+            }
+            if (quad == 0) st_coh16(to, at + D * 4u, make_float4(m[t], l[t], 0.f, 0.f));
+        }
+    }
+};
 
+// A row's place in out and lse.
+__device__ __forceinline__ void place_of(const PagedQuery& q, const Unit& u, int r, int64_t& to, int64_t& to_lse) {
+    const int i = (int)fdiv((unsigned)r, q.by_group), head = u.h * q.group + r - i * q.group;
+    to = u.s * q.o_seq + i * q.o_row + head * q.o_head;
+    to_lse = ((int64_t)u.s * q.heads + head) * q.n + i;
+}
+
+template <class E, int D, int MT>
+__device__ __forceinline__ void Wave<E, D, MT>::store(const PagedQuery& q, const Unit& u, int r0) const {
+    const int ln = __lane_id(), li = ln & 15, quad = ln >> 4;
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+        const int r = r0 + 16 * t + li;
+        if (r >= u.nrows) continue;
+        int64_t to, to_lse;
+        place_of(q, u, r, to, to_lse);
+        const float inv = inverse(l[t]);
+#pragma unroll
+        for (int n = 0; n < NO; ++n) *reinterpret_cast<f4*>(q.out + to + dim(quad, n)) = run(t, n) * inv;
+        if (q.lse && quad == 0) q.lse[to_lse] = log_sum(m[t], l[t]);
+    }
+}
+
+// The workgroup has stored its part of rows r0 .. r0 + rows - 1 past the caches that other XCDs do not
+// see; the last of `splits` to arrive joins the parts, 32 rows at a time, and leaves the counter at zero
+// for the next launch.  `room`: (32 + 2) * min(ROWS, 32) floats of LDS.
+template <int D, int ROWS>
+__device__ __forceinline__ void join(const PagedQuery& q, const Unit& u, __amdgpu_buffer_rsrc_t pr, int* counter, int splits,
+                                     int r0, int rows, float* room, int* arrived) {
+    constexpr int PW = D + 4, RB = ROWS < 32 ? ROWS : 32;
+    const int tid = threadIdx.x;
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's parts are stored
+    __syncthreads();
+    if (tid == 0)
+        *arrived = __hip_atomic_fetch_add((SHP_GLOBAL int*)counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (*arrived != splits - 1) return;
+    if (tid == 0) __hip_atomic_store((SHP_GLOBAL int*)counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    // What the shares hold of the rows is on its way (B loads an output at a time) while their maxima and
+    // sums, a share to one of 32 lanes, give the factors 2^(m_i - m) and the rows' m and l.
+    constexpr int T = D / 4, NE = RB * T / 256, B = NE == 1 ? 16 : 8, NR = RB / 8;
+    float* const factors = room;            // [RB][32]
+    float* const total = factors + RB * 32;  // [RB][2]
+    const int share_i = tid & 31;
+    for (int rb = 0; rb < rows; rb += RB) {
+        const int left = min(rows - rb, RB);
+        float4 ml[NR], x[NE][B];
+#pragma unroll
+        for (int k = 0; k < NR; ++k) {
+            const int r = (tid >> 5) + 8 * k;
+            ml[k] = make_float4(-__builtin_inff(), 0.f, 0.f, 0.f);
+            if (share_i < splits && r < left)
+                ml[k] = ld_coh16(pr, (unsigned)((share_i * ROWS + rb + r) * PW + D) * 4u, 0);
+        }
+        auto load = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < B; ++i)
+                if (i0 + i < splits)
+#pragma unroll
+                    for (int n = 0; n < NE; ++n) {
+                        const int e = tid + 256 * n, r = min(e / T, left - 1);
+                        x[n][i] = ld_coh16(pr, (unsigned)(((i0 + i) * ROWS + rb + r) * PW + e % T * 4) * 4u, 0);
+                    }
+        };
+        load(0);
+        if (rb) __syncthreads();  // the factors of the rows before have been used
+#pragma unroll
+        for (int k = 0; k < NR; ++k) {
+            float top = ml[k].x;
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
+            const float f = factor_of(ml[k].x, top);
+            float sum = ml[k].y * f;
+#pragma unroll
+            for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor(sum, w);
+            const int r = (tid >> 5) + 8 * k;
+            factors[r * 32 + share_i] = f;
+            if (share_i == 0) {
+                total[2 * r] = top;
+                total[2 * r + 1] = sum;
+            }
+        }
+        __syncthreads();
+        f4 sum[NE];
+#pragma unroll
+        for (int n = 0; n < NE; ++n) sum[n] = f4{0.f, 0.f, 0.f, 0.f};
+        for (int i0 = 0; i0 < splits; i0 += B) {
+            if (i0) load(i0);
+#pragma unroll
+            for (int i = 0; i < B; ++i)
+                if (i0 + i < splits)
+#pragma unroll
+                    for (int n = 0; n < NE; ++n)
+                        sum[n] += f4{x[n][i].x, x[n][i].y, x[n][i].z, x[n][i].w} *
+                                  factors[(tid + 256 * n) / T * 32 + i0 + i];
+        }
+#pragma unroll
+        for (int n = 0; n < NE; ++n) {
+            const int e = tid + 256 * n, r = e / T, d = e % T * 4;
+            if (r >= left) continue;
+            int64_t to, to_lse;
+            place_of(q, u, r0 + rb + r, to, to_lse);
+            const float all = total[2 * r + 1];
+            *reinterpret_cast<f4*>(q.out + to + d) = sum[n] * inverse(all);
+            if (q.lse && d == 0) q.lse[to_lse] = log_sum(total[2 * r], all);
+        }
+    }
+}
+
+// Few rows: the four wavefronts of a workgroup hold the same rows and take a tile each in turn; their parts
+// meet in LDS at the end.  K and V go from memory to registers.
+template <class E, int D, int MT>
+__global__ __launch_bounds__(256, 2) void paged_attend_kernel(Paged c, PagedQuery q, int target, int least, float* part,
+                                                              int* counters) {
+    typedef Wave<E, D, MT> W;
+    constexpr int NO = W::NO, TT = W::TT, NJ = W::NJ, NQ = W::NQ, ROWS = 16 * MT, WAVES = 4, PW = W::PW;
+    constexpr bool F32 = W::F32;
+    constexpr int EX = MT * (NO * 4 + 2) * 64;
+    __shared__ __attribute__((aligned(16))) float ex[2][EX];
+    static_assert(sizeof(Tree) <= sizeof(ex), "the tree lies where the wavefronts' parts go later");
+    __shared__ u4 low[W::NL ? MT * NQ * 64 : 1];
+    __shared__ int arrived;
+    Tree& tree = *reinterpret_cast<Tree*>(&ex[0][0]);
+    const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Task task = task_of<TT, ROWS>(c, q, target, least);
+    if (!task.any) return;
+    const Unit u = unit_of(c, q, task.s, task.h);
+    const int r0 = task.block * ROWS;
+    if (r0 >= u.nrows) return;
+    const Span span = span_of(q, u, r0, min(r0 + ROWS, u.nrows));
+    const Tiles<TT> tiles(u, span);
+    const int splits = min(max((tiles.all + task.share - 1) / task.share, 1), task.shares);
+    if (task.z >= splits) return;
+    const int tile0 = task.z * task.share, tile1 = task.z == splits - 1 ? tiles.all : tile0 + task.share;
+    if (u.drafted) climb(q, u, tree);
+
+    W x;
+    f4 raw[MT][D / 16];
+    x.begin(q, u, tree, r0, raw);
+    const float shift = W::NP == 2 ? (float)-kLift : (float)(32 - __builtin_clz(max(u.len, 1)));
+    const E* const kb = (const E*)c.k;
+    const E* const vb = (const E*)c.v;
+    const int last = max(u.len - 1, 0) & ~15;
+    u4 kr[NJ][NQ];
+    typename W::VWord vr[NJ][4][W::VW];
+    uint64_t there;
+    auto fetch = [&](int t0) __attribute__((always_inline)) {
+        there = ~0ull;
+        int pages[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) pages[j] = shared_page_of(c, u.s, min(t0 + 16 * j, last));  // a page holds whole groups of 16
+        int64_t row[NJ];
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            if (pages[j] < 0) there &= ~(0xffffull << (16 * j));
+            row[j] = row_of(c, max(pages[j], 0), u.h, min(t0 + 16 * j, last)) * D;
+#pragma unroll
+            for (int a = 0; a < NQ; ++a)
+                kr[j][a] = *reinterpret_cast<const u4*>(kb + row[j] + li * D + (F32 ? 16 * a + 4 * g : 32 * a + 8 * g));
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int w = 0; w < W::VW; ++w)
+                    vr[j][i][w] = *reinterpret_cast<const typename W::VWord*>(
+                        vb + row[j] + (4 * g + i) * D + (F32 ? 64 * w + 4 * li : NO * li));
+        // all of them on their way before the first is used: left to itself the compiler keeps few
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    x.pieces(q, raw, low);
+    if (W::NL) __syncthreads();
+    for (int at = tile0 + wave; at < tile1; at += WAVES) {
+        fetch(tiles.begin(at));
+        x.step(q, u, tree, span, shift, tiles.begin(at), there, low,
+               [&](int j, int a) __attribute__((always_inline)) { return kr[j][a]; },
+               [&](int j, int i, int w) __attribute__((always_inline)) { return vr[j][i][w]; },
+               [&](int token, int d) __attribute__((always_inline)) {
+                   const int t = min(tiles.begin(at) + token, u.len - 1);
+                   return (float)vb[row_of(c, max(page_of(c, u.s, t), 0), u.h, t) * D + d];
+               });
+    }
+
+    const int ln = __lane_id();
+#pragma unroll
+    for (int t = 0; t < MT; ++t) x.l[t] = sum_over_groups(x.l[t]);
     // the wavefronts' parts, in pairs: the upper one's goes through LDS (where the tree was)
     __syncthreads();
 #pragma unroll
     for (int step = WAVES / 2; step > 0; step >>= 1) {
-        float* x = ex[wave & (step - 1)];
+        float* e = ex[wave & (step - 1)];
         if (wave >= step && wave < 2 * step)
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
 #pragma unroll
                 for (int d = 0; d < NO; ++d)
-                    *reinterpret_cast<f4*>(&x[((t * NO + d) * 64 + ln) * 4]) = o[t][d];
-                x[(MT * NO * 4 + 2 * t) * 64 + ln] = m[t];
-                x[(MT * NO * 4 + 2 * t + 1) * 64 + ln] = l[t];
+                    *reinterpret_cast<f4*>(&e[((t * NO + d) * 64 + ln) * 4]) = x.o[t][d];
+                e[(MT * NO * 4 + 2 * t) * 64 + ln] = x.m[t];
+                e[(MT * NO * 4 + 2 * t + 1) * 64 + ln] = x.l[t];
             }
         __syncthreads();
         if (wave < step)
 #pragma unroll
             for (int t = 0; t < MT; ++t) {
-                const float m1 = x[(MT * NO * 4 + 2 * t) * 64 + ln];
-                const float l1 = x[(MT * NO * 4 + 2 * t + 1) * 64 + ln];
-                const float top = fmaxf(m[t], m1);
-                const float f0 = factor_of(m[t], top), f1 = factor_of(m1, top);
-                l[t] = l[t] * f0 + l1 * f1;
-                m[t] = top;
+                const float m1 = e[(MT * NO * 4 + 2 * t) * 64 + ln];
+                const float l1 = e[(MT * NO * 4 + 2 * t + 1) * 64 + ln];
+                const float top = fmaxf(x.m[t], m1);
+                const float f0 = factor_of(x.m[t], top), f1 = factor_of(m1, top);
+                x.l[t] = x.l[t] * f0 + l1 * f1;
+                x.m[t] = top;
 #pragma unroll
                 for (int d = 0; d < NO; ++d)
-                    o[t][d] = o[t][d] * f0 +
-                              *reinterpret_cast<const f4*>(&x[((t * NO + d) * 64 + ln) * 4]) * f1;
+                    x.o[t][d] = x.o[t][d] * f0 +
+                                *reinterpret_cast<const f4*>(&e[((t * NO + d) * 64 + ln) * 4]) * f1;
             }
         __syncthreads();
     }
-
-    // four dimensions next to each other of the lane's, and the first of them
-    auto run = [&](int t, int n) __attribute__((always_inline)) {
-        constexpr bool WIDE = !F32 && D == 128;  // a lane holds 8 dimensions in a row, not 4
-        const int i = WIDE ? n >> 1 : n & 3, x = WIDE ? 4 * (n & 1) : 4 * (n >> 2);
-        return f4{o[t][x][i], o[t][x + 1][i], o[t][x + 2][i], o[t][x + 3][i]};
-    };
-    auto dim = [&](int n) __attribute__((always_inline)) {
-        return !F32 && D == 128 ? 32 * quad + 4 * n : 64 * (n >> 2) + 16 * quad + 4 * (n & 3);
-    };
-    // a row's place in out and lse
-    auto place = [&](int r, int64_t& to, int64_t& to_lse) __attribute__((always_inline)) {
-        const int i = r / q.group, head = h * q.group + r - i * q.group;
-        to = s * q.o_seq + i * q.o_row + head * q.o_head;
-        to_lse = ((int64_t)s * q.heads + head) * q.n + i;
-    };
     if (splits == 1) {
-        if (wave) return;
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const int r = r0 + 16 * t + row;
-            if (r >= nrows) continue;
-            int64_t to, to_lse;
-            place(r, to, to_lse);
-#pragma unroll
-            for (int n = 0; n < NO; ++n)
-                *reinterpret_cast<f4*>(q.out + to + dim(n)) = l[t] == 0.0f ? f4{0.f, 0.f, 0.f, 0.f} : run(t, n) / l[t];
-            if (q.lse && quad == 0) q.lse[to_lse] = log_sum(m[t], l[t]);
-        }
+        if (wave == 0) x.store(q, u, r0);
         return;
     }
-
-    // Every share stores its rows' parts past the caches that other XCDs do not see; the last to
-    // arrive joins them, and leaves the counter at zero for the next launch.
-    const int unit = (int)blockIdx.y * (int)gridDim.x + sh, rows = min(nrows - r0, ROWS);
-    const __amdgpu_buffer_rsrc_t pr =
-        buffer_rsrc(part + (int64_t)unit * gridDim.z * ROWS * PW, (int64_t)gridDim.z * ROWS * PW);
-    if (wave == 0) {
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            const int r = 16 * t + row;
-            if (r >= rows) continue;
-            const unsigned to = (unsigned)(((int)blockIdx.z * ROWS + r) * PW) * 4u;
-#pragma unroll
-            for (int n = 0; n < NO; ++n) {
-                const f4 x = run(t, n);
-                st_coh16(pr, to + dim(n) * 4u, make_float4(x.x, x.y, x.z, x.w));
-            }
-            if (quad == 0) st_coh16(pr, to + D * 4u, make_float4(m[t], l[t], 0.f, 0.f));
-        }
-    }
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wavefront's parts are stored
-    __syncthreads();
-    if (tid == 0)
-        arrived = __hip_atomic_fetch_add((SHP_GLOBAL int*)(counters + unit), 1, __ATOMIC_RELAXED,
-                                         __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (arrived != splits - 1) return;
-    if (tid == 0)
-        __hip_atomic_store((SHP_GLOBAL int*)(counters + unit), 0, __ATOMIC_RELAXED,
-                           __HIP_MEMORY_SCOPE_AGENT);
-    // What the shares hold of the rows is on its way (B loads an output at a time) while their maxima and
-    // sums, a share to one of 32 lanes, give the factors 2^(m_i - m) and the rows' m and l.
-    constexpr int T = D / 4, NE = ROWS * T / 256, B = NE == 1 ? 16 : 8, NR = ROWS / 8;
-    float* const factors = &ex[0][0];          // [ROWS][32]
-    float* const total = factors + ROWS * 32;  // [ROWS][2]
-    const int share_i = tid & 31;
-    float4 ml[NR], x[NE][B];
-#pragma unroll
-    for (int k = 0; k < NR; ++k) {
-        const int r = (tid >> 5) + 8 * k;
-        ml[k] = make_float4(-__builtin_inff(), 0.f, 0.f, 0.f);
-        if (share_i < splits && r < rows)
-            ml[k] = ld_coh16(pr, (unsigned)((share_i * ROWS + r) * PW + D) * 4u, 0);
-    }
-    auto load = [&](int i0) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < B; ++i)
-            if (i0 + i < splits)
-#pragma unroll
-                for (int n = 0; n < NE; ++n) {
-                    const int e = tid + 256 * n, r = min(e / T, rows - 1);
-                    x[n][i] = ld_coh16(pr, (unsigned)(((i0 + i) * ROWS + r) * PW + e % T * 4) * 4u, 0);
-                }
-    };
-    load(0);
-#pragma unroll
-    for (int k = 0; k < NR; ++k) {
-        float top = ml[k].x;
-#pragma unroll
-        for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor(top, w));
-        const float f = factor_of(ml[k].x, top);
-        float sum = ml[k].y * f;
-#pragma unroll
-        for (int w = 16; w > 0; w >>= 1) sum += __shfl_xor(sum, w);
-        const int r = (tid >> 5) + 8 * k;
-        factors[r * 32 + share_i] = f;
-        if (share_i == 0) {
-            total[2 * r] = top;
-            total[2 * r + 1] = sum;
-        }
-    }
-    __syncthreads();
-    f4 sum[NE];
-#pragma unroll
-    for (int n = 0; n < NE; ++n) sum[n] = f4{0.f, 0.f, 0.f, 0.f};
-    for (int i0 = 0; i0 < splits; i0 += B) {
-        if (i0) load(i0);
-#pragma unroll
-        for (int i = 0; i < B; ++i)
-            if (i0 + i < splits)
-#pragma unroll
-                for (int n = 0; n < NE; ++n)
-                    sum[n] += f4{x[n][i].x, x[n][i].y, x[n][i].z, x[n][i].w} *
-                              factors[(tid + 256 * n) / T * 32 + i0 + i];
-    }
-#pragma unroll
-    for (int n = 0; n < NE; ++n) {
-        const int e = tid + 256 * n, r = e / T, d = e % T * 4;
-        if (r >= rows) continue;
-        int64_t to, to_lse;
-        place(r0 + r, to, to_lse);
-        const float all = total[2 * r + 1];
-        *reinterpret_cast<f4*>(q.out + to + d) = all == 0.0f ? f4{0.f, 0.f, 0.f, 0.f} : sum[n] / all;
-        if (q.lse && d == 0) q.lse[to_lse] = log_sum(total[2 * r], all);
-    }
+    const int rows = min(u.nrows - r0, ROWS);
+    const __amdgpu_buffer_rsrc_t pr = buffer_rsrc(part + (int64_t)task.first * ROWS * PW, (int64_t)splits * ROWS * PW);
+    if (wave == 0) x.store_part(pr, task.z * ROWS, rows);
+    join<D, ROWS>(q, u, pr, counters + task.first, splits, r0, rows, &ex[0][0], &arrived);
 }
 
 }  // namespace
 
 namespace shp {
 
-PagedPlan paged_attend_plan(const Paged& c, int head_dim, int64_t rows, int cu_count, bool may_split) {
+PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t rows, int cu_count, bool may_split) {
     PagedPlan p;
-    const int64_t cu = std::max(cu_count, 1), heads = (int64_t)c.n_seqs * c.kv;
-    p.row_tiles = rows > 16 ? 2 : 1;
-    const int64_t per = 16 * p.row_tiles;
-    p.row_blocks = (int)((rows + per - 1) / per);
+    const int cu = std::max(cu_count, 1), tile = 8192 / (head_dim * (format == SHP_PAGED_F32 ? 4 : 2));
+    const int64_t heads = (int64_t)c.n_seqs * c.kv, tiles = (c.cap + tile - 1) / tile;
+    // 32 rows a workgroup use each tile for twice the work (60 rows x 4 heads of 16 sequences on 4,100 tokens x 8
+    // heads x 128 in bf16 177 us, with 16 rows 287; prompts of 1,000 tokens 80 and 104).  fp32's products take so
+    // long that 16 rows, twice the workgroups, are better until there are 32 pairs of 32 rows and a tile a CU (24
+    // rows x 8 heads on 700 tokens x 4 heads x 64 11 us and 15, prompts of 200 tokens 24 and 27).
+    p.rows = rows > 16 && (format != SHP_PAGED_F32 || heads * ((rows + 31) / 32) * tiles >= 32 * cu) ? 32 : 16;
+    p.row_blocks = (int)((rows + p.rows - 1) / p.rows);
     const int64_t units = heads * p.row_blocks;
-    const int64_t want = ((p.row_blocks > 1 ? 2 : 8) * cu + units - 1) / units;
+    // Shares for 8 workgroups on every CU with 16 rows, which evens out what single ones wait for memory (16 x 131,072
+    // tokens 1,468 us, 1,533 with 4 a CU), for 3 with 32 (the trees above 177 us, 212 with 2 and 229 with 4).
+    p.target = (p.rows == 32 ? 3 : 8) * cu;
     p.least = 8;
-    const int64_t most = (c.cap / 16 + p.least - 1) / p.least;
-    p.splits = (int)std::max<int64_t>(std::min<int64_t>(std::min(want, most), 32), 1);
-    if (!may_split || units * (int64_t)sizeof(int) > (int64_t)kSplitCounterBytes) p.splits = 1;
-    p.scratch = p.splits > 1 ? (size_t)units * per * p.splits * (head_dim + 4) : 0;
+    const int64_t shares = (tiles + p.least - 1) / p.least;  // of the longest sequence there can be
+    const int64_t grid = std::min(p.target + units + 8, units * shares) + 8;  // (8: for the rounding of the count, and of runs)
+    if (!may_split || shares == 1 || units >= 2 * p.target || c.n_seqs > 512 ||
+        grid * (int64_t)sizeof(int) > (int64_t)kSplitCounterBytes) {
+        p.target = 0;
+        p.grid = (int)heads;
+        p.scratch = 0;
+    } else {
+        p.grid = (int)grid;
+        p.row_blocks = 1;
+        p.scratch = (size_t)grid * p.rows * (head_dim + 4);
+    }
     return p;
 }
 
-int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format, const PagedQuery& q,
+int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format, const PagedQuery& query,
                         const PagedPlan& p, float* scratch, int* counters) {
+    PagedQuery q = query;
+    q.by_kv = shpd::fast_div((unsigned)c.kv);
+    q.by_group = shpd::fast_div((unsigned)q.group);
     with_format(format, [&](auto e) {
         using E = decltype(e);
-        auto kern = head_dim == 64
-                        ? (p.row_tiles == 1 ? paged_attend_kernel<E, 64, 1> : paged_attend_kernel<E, 64, 2>)
-                        : (p.row_tiles == 1 ? paged_attend_kernel<E, 128, 1> : paged_attend_kernel<E, 128, 2>);
-        hipLaunchKernelGGL(kern, dim3(c.n_seqs * c.kv, p.row_blocks, p.splits), dim3(256), 0, s, c, q, p.least,
-                           scratch, counters);
+        auto kern = head_dim == 64 ? (p.rows == 16 ? paged_attend_kernel<E, 64, 1> : paged_attend_kernel<E, 64, 2>)
+                                   : (p.rows == 16 ? paged_attend_kernel<E, 128, 1> : paged_attend_kernel<E, 128, 2>);
+        hipLaunchKernelGGL(kern, dim3(p.grid, p.row_blocks), dim3(256), 0, s, c, q, p.target,
+                           p.least, scratch, counters);
     });
     SHP_HIP_CHECK(hipGetLastError());
     return SHP_OK;

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "common.h"
+#include "fastdiv.h"
 
 namespace shp {
 
@@ -37,16 +38,17 @@ struct PagedQuery {
     const int32_t *prefix, *first, *parents;
     int n, heads, group, window;
     float scale, cap;
+    shpd::FastDiv by_kv, by_group;  // set by the launch
 };
-// How attention splits the tokens of a sequence, and the floats of scratch that takes (0: none).
+// How attention shares out rows and tokens, and the floats of scratch that takes (0: none).
 struct PagedPlan {
-    int row_tiles;   // 16-row tiles a workgroup owns
-    int row_blocks;  // workgroups over the rows of one KV head
-    int splits;      // workgroups over the tokens of a sequence at most
-    int least;       // tiles a workgroup takes at least
+    int rows;              // a workgroup owns: 16 or 32
+    int target;            // workgroups that the tokens are shared out for; 0: a workgroup takes all of them
+    int least;             // tiles a workgroup takes at least
+    int grid, row_blocks;  // workgroups: over KV heads and blocks of rows, or (row_blocks 1) over shares
     size_t scratch;
 };
-PagedPlan paged_attend_plan(const Paged& c, int head_dim, int64_t rows, int cu_count, bool may_split);
+PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t rows, int cu_count, bool may_split);
 int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format, const PagedQuery& q,
                         const PagedPlan& p, float* scratch, int* counters);
 
@@ -75,6 +77,17 @@ __device__ __forceinline__ int paged_count(const int32_t* counts, int n, int s) 
 // The page of a sequence that holds token t (0 <= t < cap), -1 where there is none.
 __device__ __forceinline__ int page_of(const shp::Paged& c, int s, int t) {
     const int p = c.table[(int64_t)s * c.max_pages + (t >> c.page_log2)];
+    return (unsigned)p < (unsigned)c.n_pages ? p : -1;
+}
+// What the launch only reads, at an index that all lanes share: by the scalar unit.
+__device__ __forceinline__ int shared_int(const int32_t* p, int64_t i) {
+    typedef const __attribute__((address_space(4))) int32_t* Constant;
+    return ((Constant)(uintptr_t)p)[i];
+}
+// page_of where all lanes ask for the same sequence and token.
+__device__ __forceinline__ int shared_page_of(const shp::Paged& c, int s, int t) {
+    const int p = shared_int(c.table, __builtin_amdgcn_readfirstlane(s) * (int64_t)c.max_pages +
+                                          (__builtin_amdgcn_readfirstlane(t) >> c.page_log2));
     return (unsigned)p < (unsigned)c.n_pages ? p : -1;
 }
 // Rows before the row of KV head h and token t, which lies in `page`.
