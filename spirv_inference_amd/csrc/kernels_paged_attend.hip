@@ -19,6 +19,8 @@
 // times V are no larger than V, down by 14 for fp16, so that the low piece stays a normal number
 // longer.  Scaling is by powers of two, which rounds nothing, and seldom: a maximum has to pass a
 // whole number.
+#include <type_traits>
+
 #include "coherent.h"
 #include "gemm.h"
 #include "paged.h"
@@ -148,36 +150,44 @@ struct Unit {
     int window, prefix_all, prefix;  // prefix: of it what is no tree's
     bool drafted;
 };
-__device__ __forceinline__ Unit unit_of(const Paged& c, const PagedQuery& q, int s, int h) {
-    Unit u;
-    u.s = s;
-    u.h = h;
-    u.len = paged_length(c, u.s);
-    u.count = paged_count(q.counts, q.n, u.s);
-    u.begin = u.len - u.count;
-    u.nrows = u.count * q.group;
-    u.drafted = q.parents != nullptr;
-    u.window = q.window ? min(q.window, 1 << 30) : 1 << 30;
-    u.prefix_all = q.prefix ? min(max(q.prefix[u.s], 0), u.len) : 0;
-    u.prefix = u.drafted ? min(u.prefix_all, max(u.begin, 0)) : u.prefix_all;
-    return u;
-}
 
 // What a workgroup does: a block of rows of a KV head, and of the tiles that they see the shares
 // z * share .. of `shares`.  With target = 0 it is a place in the grid, and all tiles.  Else the blocks and the tiles
-// of all sequences are counted and cut into shares of one size, about `target` of them, which evens out
+// of all sequences are counted and cut into shares of one size, `target` of them or a little less, which evens out
 // sequences of different lengths; a workgroup finds its own in their running sum, or that there is none for it.
 struct Task {
-    int s, h, block, z, share, shares, first;  // first: the place of its rows' first part and of their counter
+    int s, h, len, count, block, z, share, shares, first;  // first: the place of its rows' first part and of their counter
     bool any;
 };
-template <int T, int ROWS>
+// The running f over the lanes, in six steps that stay in registers; f(x, 0) = x.
+template <class T, class F>
+__device__ __forceinline__ T over_lanes(T x, F f) {
+    auto step = [&](auto shift, auto rows) __attribute__((always_inline)) {
+        const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), shift.value, rows.value, 0xf, false);
+        x = f(x, __builtin_bit_cast(T, y));
+    };
+    using std::integral_constant;
+    step(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());  // from 1, 2, 4 and 8 lanes below in a row of 16
+    step(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+    step(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+    step(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+    step(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());  // rows 1 and 3 from the last lane below
+    step(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());  // rows 2 and 3 from lane 31
+    return x;
+}
+template <class T>
+__device__ __forceinline__ T last_lane(T x) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+template <int T, int ROWS, int D>
 __device__ __forceinline__ Task task_of(const Paged& c, const PagedQuery& q, int target, int least) {
     Task k;
     if (target == 0) {
         const int id = (int)blockIdx.x;
         k.s = (int)fdiv((unsigned)id, q.by_kv);
         k.h = id - k.s * c.kv;
+        k.len = paged_length(c, k.s);
+        k.count = paged_count(q.counts, q.n, k.s);
         k.block = (int)(gridDim.y - 1 - blockIdx.y);  // those that see most begin first
         k.z = 0;
         k.share = 1 << 30;
@@ -187,43 +197,49 @@ __device__ __forceinline__ Task task_of(const Paged& c, const PagedQuery& q, int
         return k;
     }
     const int lane = threadIdx.x & 63;
-    // blocks of sequence s, and the tiles that a block sees of it, no more than those that a window touches
+    // a sequence's blocks, and the tiles that a block sees of it, no more than those that a window touches
     const int most = q.window && !q.prefix ? (min(q.window, 1 << 22) + q.n) / T + 2 : 1 << 22;
-    auto size = [&](int s, int& blocks, int& tiles) __attribute__((always_inline)) {
-        const bool real = s < c.n_seqs;
-        const int len = real ? paged_length(c, s) : 0, count = real ? paged_count(q.counts, q.n, s) : 0;
+    int len, count, blocks, tiles;
+    auto size = [&](int s0) __attribute__((always_inline)) {
+        const bool real = s0 + lane < c.n_seqs;
+        len = real ? paged_length(c, s0 + lane) : 0;
+        count = real ? paged_count(q.counts, q.n, s0 + lane) : 0;
         blocks = (count * q.group + ROWS - 1) / ROWS;
         tiles = max(min((len + T - 1) / T, most), 1);
     };
-    int blocks, tiles, top = 1;
+    int top = 1, units = 0;
     float all = 0.0f;
     for (int s0 = 0; s0 < c.n_seqs; s0 += 64) {
-        size(s0 + lane, blocks, tiles);
+        size(s0);
         all += (float)blocks * (float)tiles;
         top = max(top, tiles);
+        units += blocks;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        all += __shfl_xor(all, o);
-        top = max(top, __shfl_xor(top, o));
-    }
-    // (32 shares of a block at most, whose parts one workgroup joins)
-    k.share = max(max((int)(all * (float)c.kv / (float)target) + 1, (top + 31) / 32), least);
-    k.share = __builtin_amdgcn_readfirstlane(k.share);
+    const auto add = [](auto a, auto b) { return a + b; };
+    all = last_lane(over_lanes(all, add));
+    units = last_lane(over_lanes(units, add)) * c.kv;
+    top = last_lane(over_lanes(top, [](int a, int b) { return max(a, b); }));
     // running sums of the sequences' workgroups, 64 sequences at a time
     int mine, to;
     auto count_up = [&](int s0) __attribute__((always_inline)) {
-        if (c.n_seqs > 64) size(s0 + lane, blocks, tiles);
-        to = mine = c.kv * blocks * ((tiles + k.share - 1) / k.share);
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int x = __shfl_up(to, o);
-            if (lane >= o) to += x;
-        }
-        return __builtin_amdgcn_readlane(to, 63);
+        if (c.n_seqs > 64) size(s0);
+        mine = c.kv * blocks * ((tiles + k.share - 1) / k.share);
+        to = over_lanes(mine, add);
+        return last_lane(to);
     };
-    int n = 0;
-    for (int s0 = 0; s0 < c.n_seqs; s0 += 64) n += count_up(s0);
+    // as many workgroups as the GPU holds at once, or a whole number of times that
+    const int room = max((units + target - 1) / target, 1) * target;
+    // (32 shares of a block at most, 16 of 32 rows of 128 dimensions, whose parts one workgroup joins: at the
+    // 30 GB/s that a CU reads it takes 9 us for 270 KB.  8 rows x 4 heads of 2 sequences on 100,000 tokens 132 us, 153
+    // with twice as many; of 64 dimensions 57 with 32, 70 with 16)
+    constexpr int kShares = ROWS * D <= 2048 ? 32 : 16;
+    k.share = max(max((int)(all * (float)c.kv / (float)room), (top + kShares - 1) / kShares), least);
+    int n;
+    for (;; k.share += k.share / 16 + 1) {
+        n = 0;
+        for (int s0 = 0; s0 < c.n_seqs; s0 += 64) n += count_up(s0);
+        if (n <= room) break;  // no more than `units` where a share has all tiles
+    }
     // Workgroups with numbers 8 apart run on one XCD, one after the other: each XCD gets a run of the tasks, in which
     // blocks of rows that read the same tokens are neighbours.
     const int run = (n + 7) / 8, id = (int)(blockIdx.x & 7) * run + (int)(blockIdx.x >> 3);
@@ -234,11 +250,18 @@ __device__ __forceinline__ Task task_of(const Paged& c, const PagedQuery& q, int
         if (behind) {
             const int at = __builtin_ctzll(behind);
             k.s = s0 + at;
+            k.len = __builtin_amdgcn_readlane(len, at);
+            k.count = __builtin_amdgcn_readlane(count, at);
             const int nb = __builtin_amdgcn_readlane(blocks, at);
             const int start = sum + __builtin_amdgcn_readlane(to, at) - __builtin_amdgcn_readlane(mine, at);
             k.shares = (__builtin_amdgcn_readlane(tiles, at) + k.share - 1) / k.share;
             const int off = id - start, rest = off / nb;
-            k.block = off - rest * nb;
+            // those that see most first, every eighth one after the other: an XCD that gets a part of them gets a
+            // part of each kind
+            const int p = off - rest * nb, eighth = nb >> 3, more = nb & 7, head = more * (eighth + 1);
+            const int x = p < head ? p / (eighth + 1) : more + (p - head) / max(eighth, 1);
+            const int y = p < head ? p - x * (eighth + 1) : p - head - (x - more) * eighth;
+            k.block = nb - 1 - (y * 8 + x);
             k.h = rest / k.shares;
             k.z = rest - k.h * k.shares;
             k.first = start + (k.h * nb + k.block) * k.shares;
@@ -247,6 +270,20 @@ __device__ __forceinline__ Task task_of(const Paged& c, const PagedQuery& q, int
         sum += all_here;
     }
     return k;
+}
+__device__ __forceinline__ Unit unit_of(const PagedQuery& q, const Task& k) {
+    Unit u;
+    u.s = k.s;
+    u.h = k.h;
+    u.len = k.len;
+    u.count = k.count;
+    u.begin = u.len - u.count;
+    u.nrows = u.count * q.group;
+    u.drafted = q.parents != nullptr;
+    u.window = q.window ? min(q.window, 1 << 30) : 1 << 30;
+    u.prefix_all = q.prefix ? min(max(shared_int(q.prefix, k.s), 0), u.len) : 0;
+    u.prefix = u.drafted ? min(u.prefix_all, max(u.begin, 0)) : u.prefix_all;
+    return u;
 }
 
 // The workgroup's 256 threads walk up the tree from a row each.
@@ -801,16 +838,16 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(Paged c, PagedQuer
     constexpr int NO = W::NO, TT = W::TT, NJ = W::NJ, NQ = W::NQ, ROWS = 16 * MT, WAVES = 4, PW = W::PW;
     constexpr bool F32 = W::F32;
     constexpr int EX = MT * (NO * 4 + 2) * 64;
-    __shared__ __attribute__((aligned(16))) float ex[2][EX];
+    __shared__ __attribute__((aligned(16))) float ex[WAVES / 2][EX];
     static_assert(sizeof(Tree) <= sizeof(ex), "the tree lies where the wavefronts' parts go later");
     __shared__ u4 low[W::NL ? MT * NQ * 64 : 1];
     __shared__ int arrived;
     Tree& tree = *reinterpret_cast<Tree*>(&ex[0][0]);
     const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Task task = task_of<TT, ROWS>(c, q, target, least);
+    const Task task = task_of<TT, ROWS, D>(c, q, target, least);
     if (!task.any) return;
-    const Unit u = unit_of(c, q, task.s, task.h);
+    const Unit u = unit_of(q, task);
     const int r0 = task.block * ROWS;
     if (r0 >= u.nrows) return;
     const Span span = span_of(q, u, r0, min(r0 + ROWS, u.nrows));
@@ -927,13 +964,15 @@ PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t ro
     p.rows = rows > 16 && (format != SHP_PAGED_F32 || heads * ((rows + 31) / 32) * tiles >= 32 * cu) ? 32 : 16;
     p.row_blocks = (int)((rows + p.rows - 1) / p.rows);
     const int64_t units = heads * p.row_blocks;
-    // Shares for 8 workgroups on every CU with 16 rows, which evens out what single ones wait for memory (16 x 131,072
-    // tokens 1,468 us, 1,533 with 4 a CU), for 3 with 32 (the trees above 177 us, 212 with 2 and 229 with 4).
-    p.target = (p.rows == 32 ? 3 : 8) * cu;
-    p.least = 8;
+    // Two workgroups on every CU, or a whole number of times that (of 32 rows a CU holds no more: trees of 60 rows in
+    // 16 sequences 91 us, 104 with one and a half times as many), none with fewer tiles than pay for the parts' way
+    // through memory, about 3 us: more where there are many blocks anyway (one row of 64 sequences on 1,000 tokens
+    // x 8 heads 32 us with 32 tiles, 46 with 4; of one sequence on 700 tokens 11.4 with 4, 14.8 with 16).
+    p.target = 2 * cu;
+    p.least = (int)std::min<int64_t>(std::max<int64_t>((units / 8 + 3) / 4 * 4, 4), 32);
     const int64_t shares = (tiles + p.least - 1) / p.least;  // of the longest sequence there can be
-    const int64_t grid = std::min(p.target + units + 8, units * shares) + 8;  // (8: for the rounding of the count, and of runs)
-    if (!may_split || shares == 1 || units >= 2 * p.target || c.n_seqs > 512 ||
+    const int64_t grid = std::min((units + p.target - 1) / p.target * p.target, units * shares) + 8;  // (8: XCDs' runs are rounded up)
+    if (!may_split || shares == 1 || units > 2 * p.target || c.n_seqs > 512 ||
         grid * (int64_t)sizeof(int) > (int64_t)kSplitCounterBytes) {
         p.target = 0;
         p.grid = (int)heads;
