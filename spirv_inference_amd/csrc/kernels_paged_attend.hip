@@ -137,10 +137,11 @@ __device__ __forceinline__ float log_sum(float m, float l) {
     return l == 0.0f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * kLn2;
 }
 
-// A drafted tree's rows: bit u of above[i] says that row u is row i or above it and within its window or
-// the prefix, depth[i] how many rows are above row i.
+// A drafted tree's rows: bit u of above[i] says that row u is row i of the workgroup's or above it and within its
+// window or the prefix; depth[i] is how many rows are above row i of the tree.
+template <int N>  // N query rows are of N tokens at most
 struct Tree {
-    uint64_t above[kTreeRows][kTreeRows / 64];
+    uint64_t above[N][kTreeRows / 64];
     uint16_t parent[kTreeRows], depth[kTreeRows];
 };
 
@@ -286,8 +287,9 @@ __device__ __forceinline__ Unit unit_of(const PagedQuery& q, const Task& k) {
     return u;
 }
 
-// The workgroup's 256 threads walk up the tree from a row each.
-__device__ __forceinline__ void climb(const PagedQuery& q, const Unit& u, Tree& tree) {
+// The workgroup's 256 threads walk up the tree from a row each.  Its own rows are those from `own` on.
+template <int N>
+__device__ __forceinline__ void climb(const PagedQuery& q, const Unit& u, int own, Tree<N>& tree) {
     const int i = threadIdx.x;
     if (i < u.count) {
         const int p = q.parents[(int64_t)u.s * q.n + i];
@@ -303,8 +305,10 @@ __device__ __forceinline__ void climb(const PagedQuery& q, const Unit& u, Tree& 
                 for (int w = 0; w < kTreeRows / 64; ++w) up[w] |= v >> 6 == w ? 1ull << (v & 63) : 0ull;
             }
         tree.depth[i] = (uint16_t)(steps - 1);
+        if (i >= own && i < own + N) {
 #pragma unroll
-        for (int w = 0; w < kTreeRows / 64; ++w) tree.above[i][w] = up[w];
+            for (int w = 0; w < kTreeRows / 64; ++w) tree.above[i - own][w] = up[w];
+        }
     }
     __syncthreads();
 }
@@ -358,7 +362,7 @@ struct Tiles {
 
 // Which tokens a row sees: [first, len) of those in [lo, hi), before the prefix or among its tree's.
 struct Sight {
-    int lo, hi, first, position, node;
+    int lo, hi, first, position, node;  // node: of the workgroup's
 };
 
 // 16 * MT rows of a wavefront, and what it has of their softmax.
@@ -381,7 +385,7 @@ struct Wave {
     Sight see[MT];
 
     // Rows from r0 on; those behind the last repeat it.  raw: the lane's part of them.
-    __device__ __forceinline__ void begin(const PagedQuery& q, const Unit& u, const Tree& tree, int r0, f4 raw[MT][2 * D / 32]) {
+    __device__ __forceinline__ void begin(const PagedQuery& q, const Unit& u, const uint16_t* depth, int node0, int r0, f4 raw[MT][2 * D / 32]) {
         const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
@@ -392,8 +396,8 @@ struct Wave {
             for (int a = 0; a < D / 16; ++a)
                 raw[t][a] = *reinterpret_cast<const f4*>(x + (F32 ? 16 * a + 4 * g : 32 * (a >> 1) + 8 * g + 4 * (a & 1)));
             Sight& v = see[t];
-            v.node = i;
-            v.position = u.drafted ? u.begin + tree.depth[i] : place;
+            v.node = i - node0;
+            v.position = u.drafted ? u.begin + depth[i] : place;
             v.hi = u.drafted ? u.begin : place + 1;
             v.lo = max(v.position - u.window + 1, 0);
             v.first = q.first ? max(q.first[(int64_t)u.s * q.n + i], 0) : 0;
@@ -402,7 +406,7 @@ struct Wave {
         }
     }
     // The rows' pieces in the B layout, times the scale; nothing seen yet.  low: those that LDS holds.
-    __device__ __forceinline__ void pieces(const PagedQuery& q, f4 v[MT][2 * D / 32], u4* low) {
+    __device__ __forceinline__ void pieces(const PagedQuery& q, f4 v[MT][2 * D / 32], u4* low, bool mine) {
         const float factor = q.cap > 0.0f ? q.scale / q.cap : q.scale * kLog2e;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
@@ -438,7 +442,7 @@ struct Wave {
                         for (int p = 0; p < NR; ++p) qp[t][a][p][b] = piece[p];
                         lowest[b] = piece[NP - 1];
                     }
-                    if (NL && threadIdx.x < 64) low[(t * NQ + a) * 64 + threadIdx.x] = lowest;
+                    if (NL && mine) low[(t * NQ + a) * 64 + (threadIdx.x & 63)] = lowest;
                 }
             }
         }
@@ -456,7 +460,8 @@ struct Wave {
     // 16 j + 4 g + i; `there` says which of its tokens have a page.
     // number(token, dimension) is one of the tile's values.
     template <class K, class V, class N>
-    __device__ __forceinline__ void step(const PagedQuery& q, const Unit& u, const Tree& tree, const Span& span, float shift,
+    __device__ __forceinline__ void step(const PagedQuery& q, const Unit& u, const uint64_t (*above)[kTreeRows / 64],
+                                         const uint16_t* depth, const Span& span, float shift,
                                          int t0, uint64_t there, const u4* low, K key, V value, N number) {
         const int g = (threadIdx.x & 63) >> 4;
         // whether some row does not see some token
@@ -513,7 +518,7 @@ struct Wave {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int at = t0 + 16 * j + 4 * g + i, up = min(max(at - u.begin, 0), max(u.count - 1, 0));
-                            const int position = at < u.begin ? at : u.begin + tree.depth[up];
+                            const int position = at < u.begin ? at : u.begin + depth[up];
                             sc[t][j][i] -= slope[t] * fabsf((float)(see[t].position - position));
                         }
                 } else {
@@ -530,7 +535,7 @@ struct Wave {
                 uint64_t bits = (below(v.hi - t0) & ~below(v.lo - t0)) | below(u.prefix - t0);
                 if (u.drafted && t0 + TT > u.begin) {
                     // the tree's bits from t0 on: those of rows t0 - begin ..
-                    const uint64_t* up = tree.above[v.node];
+                    const uint64_t* up = above[v.node];
                     const int from = t0 - u.begin;
                     if (from < 0) {
                         bits |= up[0] << -from;  // -from < TT
@@ -597,24 +602,7 @@ struct Wave {
                 for (int w = 0; w < VW; ++w) vr[j][i][w] = value(j, i, w);
         // Where some row does not see some token, a value that is not finite would spoil that row too: such a
         // value is added to the rows that see it and taken out.
-        if (edge) {
-            // the largest exponents, of 16-bit values in both halves of a word
-            us2 top2 = {0, 0};
-            unsigned top = 0;
-#pragma unroll
-            for (int j = 0; j < NJ; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int w = 0; w < VW; ++w)
-#pragma unroll
-                        for (int b = 0; b < VB; ++b) {
-                            const unsigned x = vr[j][i][w][b];
-                            if constexpr (F32) top = max(top, x & 0x7fffffffu);
-                            else top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(us2, x & 0x7fff7fffu));
-                        }
-            if constexpr (!F32) top = max((unsigned)top2.x, (unsigned)top2.y);
-            if (__any(top >= kInf<E>)) {
+        if (edge && not_finite(vr)) {
 #pragma unroll 1
                 for (int token = 0; token < TT; ++token)
 #pragma unroll
@@ -643,7 +631,6 @@ struct Wave {
                                 }
                                 vr[j][i][w][b] = x;
                             }
-            }
         }
         // O^T += V^T P^T
         if constexpr (F32) {
@@ -690,6 +677,26 @@ struct Wave {
     // The dimension that o[t][d][i] of lane group g is.
     static __device__ __forceinline__ int dim_of(int g, int d, int i) {
         return !F32 && D == 128 ? 32 * g + 8 * i + d : 64 * (d >> 2) + 16 * g + 4 * i + (d & 3);
+    }
+    // Whether some of a tile's values is an infinity or a NaN.
+    static __device__ __forceinline__ bool not_finite(const VWord vr[NJ][4][VW]) {
+        // the largest exponents, of 16-bit values in both halves of a word
+        us2 top2 = {0, 0};
+        unsigned top = 0;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int w = 0; w < VW; ++w)
+#pragma unroll
+                    for (int b = 0; b < VB; ++b) {
+                        const unsigned x = vr[j][i][w][b];
+                        if constexpr (F32) top = max(top, x & 0x7fffffffu);
+                        else top2 = __builtin_elementwise_max(top2, __builtin_bit_cast(us2, x & 0x7fff7fffu));
+                    }
+        if constexpr (!F32) top = max((unsigned)top2.x, (unsigned)top2.y);
+        return __any(top >= kInf<E>);
     }
     // Four dimensions next to each other of the lane's, and the first of them.
     __device__ __forceinline__ f4 run(int t, int n) const {
@@ -829,50 +836,59 @@ __device__ __forceinline__ void join(const PagedQuery& q, const Unit& u, __amdgp
     }
 }
 
-// Few rows: the four wavefronts of a workgroup hold the same rows and take a tile each in turn; their parts
-// meet in LDS at the end.  K and V go from memory to registers.
-template <class E, int D, int MT>
-__global__ __launch_bounds__(256, 2) void paged_attend_kernel(Paged c, PagedQuery q, int target, int least, float* part,
-                                                              int* counters) {
+// Few rows, or a long way through the tokens: the four wavefronts of a workgroup hold the same rows and take a tile each
+// in turn; their parts meet in LDS at the end.  Many rows that see little each (SIDE): the wavefronts hold rows of their
+// own, side by side, and read the same tiles at about the same time.  K and V go from memory to registers.
+template <class E, int D, int MT, bool SIDE>
+__global__ __launch_bounds__(256, MT == 1 ? (D == 64 ? 4 : 3) : 2) void paged_attend_kernel(
+    Paged c, PagedQuery q, int target, int least, float* part, int* counters) {
     typedef Wave<E, D, MT> W;
-    constexpr int NO = W::NO, TT = W::TT, NJ = W::NJ, NQ = W::NQ, ROWS = 16 * MT, WAVES = 4, PW = W::PW;
+    constexpr int NO = W::NO, TT = W::TT, NJ = W::NJ, NQ = W::NQ, WAVES = 4, PW = W::PW;
+    constexpr int ROWS = 16 * MT * (SIDE ? WAVES : 1), EX = MT * (NO * 4 + 2) * 64;  // floats of a wavefront's part
     constexpr bool F32 = W::F32;
-    constexpr int EX = MT * (NO * 4 + 2) * 64;
-    __shared__ __attribute__((aligned(16))) float ex[WAVES / 2][EX];
-    static_assert(sizeof(Tree) <= sizeof(ex), "the tree lies where the wavefronts' parts go later");
-    __shared__ u4 low[W::NL ? MT * NQ * 64 : 1];
+    __shared__ __attribute__((aligned(16))) float ex[SIDE ? 1 : WAVES / 2][SIDE ? 4 : EX];
+    __shared__ u4 lowest[W::NL ? (SIDE ? WAVES : 1) * MT * NQ * 64 : 1];
+    __shared__ Tree<SIDE ? 128 : 32> tree;
     __shared__ int arrived;
-    Tree& tree = *reinterpret_cast<Tree*>(&ex[0][0]);
     const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Task task = task_of<TT, ROWS, D>(c, q, target, least);
     if (!task.any) return;
     const Unit u = unit_of(q, task);
-    const int r0 = task.block * ROWS;
-    if (r0 >= u.nrows) return;
-    const Span span = span_of(q, u, r0, min(r0 + ROWS, u.nrows));
+    const int block0 = task.block * ROWS;
+    if (block0 >= u.nrows) return;
+    const int node0 = (int)fdiv((unsigned)block0, q.by_group);  // the first row's token
+    if (SIDE && u.drafted) climb(q, u, node0, tree);
+    const int r0 = SIDE ? block0 + 16 * MT * wave : block0;
+    if (SIDE && r0 >= u.nrows) return;
+    const Span span = span_of(q, u, r0, min(r0 + 16 * MT, u.nrows));
     const Tiles<TT> tiles(u, span);
     const int splits = min(max((tiles.all + task.share - 1) / task.share, 1), task.shares);
     if (task.z >= splits) return;
     const int tile0 = task.z * task.share, tile1 = task.z == splits - 1 ? tiles.all : tile0 + task.share;
-    if (u.drafted) climb(q, u, tree);
+    if (!SIDE && u.drafted) climb(q, u, node0, tree);
 
     W x;
-    f4 raw[MT][D / 16];
-    x.begin(q, u, tree, r0, raw);
+    u4* const low = lowest + (W::NL && SIDE ? wave * MT * NQ * 64 : 0);
+    {
+        f4 raw[MT][D / 16];
+        x.begin(q, u, tree.depth, node0, r0, raw);
+        x.pieces(q, raw, low, SIDE || wave == 0);
+    }
+    if (W::NL && !SIDE) __syncthreads();
     const float shift = W::NP == 2 ? (float)-kLift : (float)(32 - __builtin_clz(max(u.len, 1)));
     const E* const kb = (const E*)c.k;
     const E* const vb = (const E*)c.v;
     const int last = max(u.len - 1, 0) & ~15;
-    u4 kr[NJ][NQ];
-    typename W::VWord vr[NJ][4][W::VW];
-    uint64_t there;
-    auto fetch = [&](int t0) __attribute__((always_inline)) {
-        there = ~0ull;
+    for (int at = tile0 + (SIDE ? 0 : wave); at < tile1; at += SIDE ? 1 : WAVES) {
+        const int t0 = tiles.begin(at);
+        uint64_t there = ~0ull;  // the tokens that have a page, of which each holds whole groups of 16
         int pages[NJ];
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) pages[j] = shared_page_of(c, u.s, min(t0 + 16 * j, last));  // a page holds whole groups of 16
+        for (int j = 0; j < NJ; ++j) pages[j] = shared_page_of(c, u.s, min(t0 + 16 * j, last));
         int64_t row[NJ];
+        u4 kr[NJ][NQ];
+        typename W::VWord vr[NJ][4][W::VW];
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             if (pages[j] < 0) there &= ~(0xffffull << (16 * j));
@@ -891,62 +907,60 @@ __global__ __launch_bounds__(256, 2) void paged_attend_kernel(Paged c, PagedQuer
                         vb + row[j] + (4 * g + i) * D + (F32 ? 64 * w + 4 * li : NO * li));
         // all of them on their way before the first is used: left to itself the compiler keeps few
         __builtin_amdgcn_sched_barrier(0);
-    };
-    x.pieces(q, raw, low);
-    if (W::NL) __syncthreads();
-    for (int at = tile0 + wave; at < tile1; at += WAVES) {
-        fetch(tiles.begin(at));
-        x.step(q, u, tree, span, shift, tiles.begin(at), there, low,
+        x.step(q, u, tree.above, tree.depth, span, shift, t0, there, low,
                [&](int j, int a) __attribute__((always_inline)) { return kr[j][a]; },
                [&](int j, int i, int w) __attribute__((always_inline)) { return vr[j][i][w]; },
                [&](int token, int d) __attribute__((always_inline)) {
-                   const int t = min(tiles.begin(at) + token, u.len - 1);
+                   const int t = min(t0 + token, u.len - 1);
                    return (float)vb[row_of(c, max(page_of(c, u.s, t), 0), u.h, t) * D + d];
                });
     }
 
-    const int ln = __lane_id();
 #pragma unroll
     for (int t = 0; t < MT; ++t) x.l[t] = sum_over_groups(x.l[t]);
-    // the wavefronts' parts, in pairs: the upper one's goes through LDS (where the tree was)
-    __syncthreads();
+    if constexpr (SIDE) {
+        x.store(q, u, r0);
+    } else {
+        const int ln = __lane_id();
+        // the wavefronts' parts, in pairs: the upper one's goes through LDS
 #pragma unroll
-    for (int step = WAVES / 2; step > 0; step >>= 1) {
-        float* e = ex[wave & (step - 1)];
-        if (wave >= step && wave < 2 * step)
+        for (int step = WAVES / 2; step > 0; step >>= 1) {
+            float* e = ex[wave & (step - 1)];
+            if (wave >= step && wave < 2 * step)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
+                for (int t = 0; t < MT; ++t) {
 #pragma unroll
-                for (int d = 0; d < NO; ++d)
-                    *reinterpret_cast<f4*>(&e[((t * NO + d) * 64 + ln) * 4]) = x.o[t][d];
-                e[(MT * NO * 4 + 2 * t) * 64 + ln] = x.m[t];
-                e[(MT * NO * 4 + 2 * t + 1) * 64 + ln] = x.l[t];
-            }
-        __syncthreads();
-        if (wave < step)
+                    for (int d = 0; d < NO; ++d)
+                        *reinterpret_cast<f4*>(&e[((t * NO + d) * 64 + ln) * 4]) = x.o[t][d];
+                    e[(MT * NO * 4 + 2 * t) * 64 + ln] = x.m[t];
+                    e[(MT * NO * 4 + 2 * t + 1) * 64 + ln] = x.l[t];
+                }
+            __syncthreads();
+            if (wave < step)
 #pragma unroll
-            for (int t = 0; t < MT; ++t) {
-                const float m1 = e[(MT * NO * 4 + 2 * t) * 64 + ln];
-                const float l1 = e[(MT * NO * 4 + 2 * t + 1) * 64 + ln];
-                const float top = fmaxf(x.m[t], m1);
-                const float f0 = factor_of(x.m[t], top), f1 = factor_of(m1, top);
-                x.l[t] = x.l[t] * f0 + l1 * f1;
-                x.m[t] = top;
+                for (int t = 0; t < MT; ++t) {
+                    const float m1 = e[(MT * NO * 4 + 2 * t) * 64 + ln];
+                    const float l1 = e[(MT * NO * 4 + 2 * t + 1) * 64 + ln];
+                    const float top = fmaxf(x.m[t], m1);
+                    const float f0 = factor_of(x.m[t], top), f1 = factor_of(m1, top);
+                    x.l[t] = x.l[t] * f0 + l1 * f1;
+                    x.m[t] = top;
 #pragma unroll
-                for (int d = 0; d < NO; ++d)
-                    x.o[t][d] = x.o[t][d] * f0 +
-                                *reinterpret_cast<const f4*>(&e[((t * NO + d) * 64 + ln) * 4]) * f1;
-            }
-        __syncthreads();
+                    for (int d = 0; d < NO; ++d)
+                        x.o[t][d] = x.o[t][d] * f0 +
+                                    *reinterpret_cast<const f4*>(&e[((t * NO + d) * 64 + ln) * 4]) * f1;
+                }
+            __syncthreads();
+        }
+        if (splits == 1) {
+            if (wave == 0) x.store(q, u, r0);
+            return;
+        }
+        const int rows = min(u.nrows - r0, ROWS);
+        const __amdgpu_buffer_rsrc_t pr = buffer_rsrc(part + (int64_t)task.first * ROWS * PW, (int64_t)splits * ROWS * PW);
+        if (wave == 0) x.store_part(pr, task.z * ROWS, rows);
+        join<D, ROWS>(q, u, pr, counters + task.first, splits, r0, rows, &ex[0][0], &arrived);
     }
-    if (splits == 1) {
-        if (wave == 0) x.store(q, u, r0);
-        return;
-    }
-    const int rows = min(u.nrows - r0, ROWS);
-    const __amdgpu_buffer_rsrc_t pr = buffer_rsrc(part + (int64_t)task.first * ROWS * PW, (int64_t)splits * ROWS * PW);
-    if (wave == 0) x.store_part(pr, task.z * ROWS, rows);
-    join<D, ROWS>(q, u, pr, counters + task.first, splits, r0, rows, &ex[0][0], &arrived);
 }
 
 }  // namespace
@@ -955,13 +969,19 @@ namespace shp {
 
 PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t rows, int cu_count, bool may_split) {
     PagedPlan p;
-    const int cu = std::max(cu_count, 1), tile = 8192 / (head_dim * (format == SHP_PAGED_F32 ? 4 : 2));
+    const bool f32 = format == SHP_PAGED_F32;
+    const int cu = std::max(cu_count, 1), tile = 8192 / (head_dim * (f32 ? 4 : 2));
     const int64_t heads = (int64_t)c.n_seqs * c.kv, tiles = (c.cap + tile - 1) / tile;
     // 32 rows a workgroup use each tile for twice the work (60 rows x 4 heads of 16 sequences on 4,100 tokens x 8
-    // heads x 128 in bf16 177 us, with 16 rows 287; prompts of 1,000 tokens 80 and 104).  fp32's products take so
+    // heads x 128 in bf16 180 us, with 16 rows 287; prompts of 1,000 tokens 80 and 104).  fp32's products take so
     // long that 16 rows, twice the workgroups, are better until there are 32 pairs of 32 rows and a tile a CU (24
-    // rows x 8 heads on 700 tokens x 4 heads x 64 11 us and 15, prompts of 200 tokens 24 and 27).
-    p.rows = rows > 16 && (format != SHP_PAGED_F32 || heads * ((rows + 31) / 32) * tiles >= 32 * cu) ? 32 : 16;
+    // rows x 8 heads on 700 tokens x 4 heads x 64 11 us and 15, prompts of 200 tokens 20 and 30).
+    p.rows = rows > 16 && (!f32 || heads * ((rows + 31) / 32) * tiles >= 32 * cu) ? 32 : 16;
+    // Where blocks of 128 rows nearly fill the GPU, wavefronts side by side begin and end once for each 32 rows, not four
+    // times (4,000 tokens with a window of 500 113 us, 155 so; prompts of 100 tokens of 32 sequences 32 and 54; at 2,000
+    // tokens x 8 heads, 504 blocks, both take 123; with 256 blocks of 8 sequences on 2,000 tokens 115 and 101).  In
+    // fp32 the products outweigh that (prompts of 1,000 tokens 247 and 186).
+    if (!f32 && 4 * heads * ((rows + 127) / 128) >= 7 * cu) p.rows = 128;
     p.row_blocks = (int)((rows + p.rows - 1) / p.rows);
     const int64_t units = heads * p.row_blocks;
     // Two workgroups on every CU, or a whole number of times that (of 32 rows a CU holds no more: trees of 60 rows in
@@ -972,7 +992,7 @@ PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t ro
     p.least = (int)std::min<int64_t>(std::max<int64_t>((units / 8 + 3) / 4 * 4, 4), 32);
     const int64_t shares = (tiles + p.least - 1) / p.least;  // of the longest sequence there can be
     const int64_t grid = std::min((units + p.target - 1) / p.target * p.target, units * shares) + 8;  // (8: XCDs' runs are rounded up)
-    if (!may_split || shares == 1 || units > 2 * p.target || c.n_seqs > 512 ||
+    if (p.rows == 128 || !may_split || shares == 1 || units > 2 * p.target || c.n_seqs > 512 ||
         grid * (int64_t)sizeof(int) > (int64_t)kSplitCounterBytes) {
         p.target = 0;
         p.grid = (int)heads;
@@ -985,6 +1005,15 @@ PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t ro
     return p;
 }
 
+namespace {
+template <class E, int D>
+auto kernel_of(int rows) {
+    if constexpr (sizeof(E) == 2)
+        if (rows == 128) return paged_attend_kernel<E, D, 2, true>;
+    return rows == 16 ? paged_attend_kernel<E, D, 1, false> : paged_attend_kernel<E, D, 2, false>;
+}
+}  // namespace
+
 int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format, const PagedQuery& query,
                         const PagedPlan& p, float* scratch, int* counters) {
     PagedQuery q = query;
@@ -992,10 +1021,8 @@ int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format,
     q.by_group = shpd::fast_div((unsigned)q.group);
     with_format(format, [&](auto e) {
         using E = decltype(e);
-        auto kern = head_dim == 64 ? (p.rows == 16 ? paged_attend_kernel<E, 64, 1> : paged_attend_kernel<E, 64, 2>)
-                                   : (p.rows == 16 ? paged_attend_kernel<E, 128, 1> : paged_attend_kernel<E, 128, 2>);
-        hipLaunchKernelGGL(kern, dim3(p.grid, p.row_blocks), dim3(256), 0, s, c, q, p.target,
-                           p.least, scratch, counters);
+        auto kern = head_dim == 64 ? kernel_of<E, 64>(p.rows) : kernel_of<E, 128>(p.rows);
+        hipLaunchKernelGGL(kern, dim3(p.grid, p.row_blocks), dim3(256), 0, s, c, q, p.target, p.least, scratch, counters);
     });
     SHP_HIP_CHECK(hipGetLastError());
     return SHP_OK;
