@@ -151,8 +151,7 @@ __global__ __launch_bounds__(256) void paged_accept_kernel(Paged c, PagedTree t)
 namespace shp {
 
 int paged_append_launch(hipStream_t s, const Paged& c, int head_dim, int format, const PagedRows& r) {
-    const int64_t rows = (int64_t)c.n_seqs * r.n;
-    if (rows > 0x7fffffff) return fail(SHP_ERR_UNSUPPORTED, "shp_paged_append: more than 2^31 rows");
+    const int64_t rows = (int64_t)c.n_seqs * r.n;  // 16,000,000 at most
     const int64_t units = (int64_t)(r.heads + 2 * c.kv) * (head_dim / 8);
     const dim3 grid((unsigned)rows, (unsigned)std::min<int64_t>((units + 255) / 256, 65535));
     with_format(format, [&](auto e) {

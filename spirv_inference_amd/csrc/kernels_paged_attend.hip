@@ -977,11 +977,12 @@ PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t ro
     // long that 16 rows, twice the workgroups, are better until there are 32 pairs of 32 rows and a tile a CU (24
     // rows x 8 heads on 700 tokens x 4 heads x 64 11 us and 15, prompts of 200 tokens 20 and 30).
     p.rows = rows > 16 && (!f32 || heads * ((rows + 31) / 32) * tiles >= 32 * cu) ? 32 : 16;
-    // Where blocks of 128 rows nearly fill the GPU, wavefronts side by side begin and end once for each 32 rows, not four
-    // times (4,000 tokens with a window of 500 113 us, 155 so; prompts of 100 tokens of 32 sequences 32 and 54; at 2,000
-    // tokens x 8 heads, 504 blocks, both take 123; with 256 blocks of 8 sequences on 2,000 tokens 115 and 101).  In
-    // fp32 the products outweigh that (prompts of 1,000 tokens 247 and 186).
-    if (!f32 && 4 * heads * ((rows + 127) / 128) >= 7 * cu) p.rows = 128;
+    // Where blocks of 128 rows nearly fill the GPU, each with work for three wavefronts at least, wavefronts side by
+    // side begin and end once for each 32 rows, not four times (4,000 tokens with a window of 500 113 us, 155 the
+    // other way; prompts of 100 tokens of 32 sequences 32 and 54; at 2,000 tokens x 8 heads, 504 blocks, both take
+    // 123; with 256 blocks of 8 sequences on 2,000 tokens 115 and 101).  In fp32 the products outweigh that (prompts
+    // of 1,000 tokens 247 and 186).
+    if (!f32 && rows > 64 && 4 * heads * ((rows + 127) / 128) >= 7 * cu) p.rows = 128;
     p.row_blocks = (int)((rows + p.rows - 1) / p.rows);
     const int64_t units = heads * p.row_blocks;
     // Two workgroups on every CU, or a whole number of times that (of 32 rows a CU holds no more: trees of 60 rows in

@@ -116,6 +116,7 @@ int shp_paged_append(shp_ctx* ctx, const shp_paged* cache, const shp_paged_appen
         rc = shp::check_heads(me, c, a->n, c.kv);
         if (rc) return rc;
     }
+    if ((int64_t)c.n_seqs * a->n > 16000000) return bad(me, "more than 16000000 rows", SHP_ERR_UNSUPPORTED);
     if (a->rot < 0 || a->rot > cache->head_dim || a->rot % 8)
         return bad(me, "rot must be a multiple of 8, 0 to head_dim", SHP_ERR_SHAPE);
     if (a->rot && !a->inv_freq) return bad(me, "rot without inv_freq");
@@ -149,7 +150,8 @@ int shp_paged_attend(shp_ctx* ctx, const shp_paged* cache, const shp_paged_atten
     if (!rc) rc = shp::check_rows(me, "out", a->out, a->o_seq, a->o_row, a->o_head);
     if (rc) return rc;
     if (!std::isfinite(a->scale)) return bad(me, "scale is not finite");
-    if (!std::isfinite(a->cap) || a->cap < 0) return bad(me, "cap must be finite, and 0 or more");
+    if (!std::isfinite(a->cap) || a->cap < 0 || (a->cap > 0 && !std::isfinite(a->scale / a->cap)))
+        return bad(me, "cap must be finite, and 0 or large enough for scale / cap");
     if (a->window < 0) return bad(me, "window < 0");
     if (a->parents && a->n > shp::kTreeRows)
         return bad(me, "a tree of more than 256 rows", SHP_ERR_UNSUPPORTED);

@@ -115,6 +115,8 @@ def test_bad_caches_are_refused(over, code, what):
     ("shp_paged_append", dict(rot=72), "rot"),
     ("shp_paged_append", dict(inv_freq=0), "inv_freq"),
     ("shp_paged_append", dict(n=600000), "500000"),
+    ("shp_paged_attend", dict(cap=1e-45, scale=1.0), "cap"),
+    ("shp_paged_attend", dict(cap=1e-3, scale=1e37), "cap"),
     ("shp_paged_attend", dict(n=-1), "n < 0"),
     ("shp_paged_attend", dict(q=0), "null q"),
     ("shp_paged_attend", dict(out=0), "null out"),
@@ -142,6 +144,13 @@ def test_bad_caches_are_refused(over, code, what):
 def test_bad_arguments_are_refused(name, over, what):
     rc, msg = call(name, cache(), args(CALLS[name], **over))
     assert rc != 0 and what in msg and "ctx" not in msg, (rc, msg)
+
+
+def test_appends_of_too_many_rows_are_refused():
+    rc, msg = call("shp_paged_append", cache(n_seqs=40, n_kv_heads=1), args(PagedAppendArgs, n=400001, n_heads=1))
+    assert rc == _lib.SHP_ERR_UNSUPPORTED and "16000000" in msg
+    assert call("shp_paged_append", cache(n_seqs=40, n_kv_heads=1),
+                args(PagedAppendArgs, n=400000, n_heads=1))[1].endswith("null ctx")
 
 
 @pytest.mark.parametrize("name,fields", [

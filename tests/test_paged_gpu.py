@@ -345,6 +345,66 @@ def test_attention_of_trees(ctx, fmt, d, kv, group, n, page, lens, counts, how):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+def test_trees_of_sequences_that_are_shorter(ctx, fmt):
+    """Rows before the first token see nothing, and their places are nobody's."""
+    rng = np.random.default_rng(29)
+    with filled(ctx, rng, 3, 1, 64, 6, 16, fmt, [20, 90, 1]) as p:
+        for n in (33, 70, 128):
+            for how in ({}, dict(window=4), dict(prefix=[5, 80, 1], bias=True)):
+                p.check_attend(rows(rng, 3, n, 3, 64), parents=trees(rng, 3, n), **options(how, rng, n, 3, [20, 90, 1]))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("first", [0, 63, 64, 2 ** 31 - 1, -2 ** 31, 2 ** 31 - 64, 1 << 30])
+def test_first_tokens_of_any_size(ctx, fmt, first):
+    rng = np.random.default_rng(30)
+    with filled(ctx, rng, 2, 1, 64, 8, 16, fmt, [128, 70]) as p:
+        for n in (1, 20, 70):
+            f = np.full((2, n), first, np.int64)
+            p.check_attend(rows(rng, 2, n, 3, 64), first=f)
+            f[:, ::2] = 5
+            p.check_attend(rows(rng, 2, n, 3, 64), first=f, window=2 ** 31 - 1, prefix=[2 ** 31 - 1, -2 ** 31])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_table_with_room_for_millions(ctx, fmt):
+    """Most of the table names no page, and most workgroups have nothing to do."""
+    rng = np.random.default_rng(34)
+    with PagedCache(ctx, 2, 2, 64, 20, 16, 1 << 18, fmt=fmt) as dev:
+        table = np.full((2, 1 << 18), -1, np.int32)
+        table[0, :10], table[1, :10] = np.arange(10), np.arange(10, 20)
+        dev.set_table(table)
+        for lens in ([150, 33], [1 << 22, 5]):  # the second: of four million tokens 160 are there
+            dev.set_lengths([150, 33])
+            k, v = rows(rng, 2, 150, 2, 64), rows(rng, 2, 150, 2, 64)
+            ts = [ctx.tensor(x) for x in (k, v)]
+            counts = ctx.tensor(np.array([150, 33]), np.int32)
+            dev.append(ts[0], ts[1], 150, counts=counts)
+            dev.set_lengths(lens)
+            ref = R.RefPaged(2, 2, 64, 160, fmt)
+            for s, ln in enumerate((150, 33)):
+                ref.k[s, :, :ln] = R.stored(k[s, :ln], fmt).transpose(1, 0, 2)
+                ref.v[s, :, :ln] = R.stored(v[s, :ln], fmt).transpose(1, 0, 2)
+            ref.lens = [150, lens[1]]
+            if lens[0] > 160:  # places 150 .. 159 hold zeros
+                ref.lens[0] = 160
+                w = np.zeros((20, 2, 16, 64), dev.k.dtype)
+                for name in "kv":
+                    t = getattr(dev, name)
+                    w = t.download().reshape(20, 2, 16, 64)
+                    w[9, :, 6:] = 0
+                    t.upload(w)
+            q = rows(rng, 2, 1, 6, 64)
+            out, dq = ctx.empty(q.size), ctx.tensor(q)
+            dev.attend(dq, out, 6, 1)
+            ctx.sync()
+            want, _, tol, _ = ref.attend(q, [1, 1], 0.125)
+            assert (np.abs(out.download().reshape(q.shape) - want) <= tol).all()
+            for t in (*ts, counts, out, dq):
+                t.free()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_a_chain_of_rows_is_a_deep_tree(ctx, fmt):
     """Row i on row i - 1: 256 levels, the same as causal rows."""
     rng = np.random.default_rng(14)
@@ -493,6 +553,65 @@ def test_long_sequences(ctx, fmt, d, kv, group, n, ln, page):
         q = rows(rng, 1, n, kv * group, d)
         p.check_attend(q)
         p.check_attend(q, window=ln // 2, prefix=[200])
+
+
+# So many blocks of 128 rows of a KV head that the wavefronts of a workgroup take rows of their own.
+@pytest.mark.parametrize("fmt", ["f16", "bf16"])
+@pytest.mark.parametrize("d,kv,group,n,lens,counts", [
+    (64, 56, 4, 101, [101, 230], None), (128, 75, 3, 90, [77, 90], [77, 3]), (64, 224, 1, 70, [70, 4], None)])
+@pytest.mark.parametrize("how", ["cap", "window", "prefix and window", "first", "all", "tree"])
+def test_attention_of_many_blocks(ctx, fmt, d, kv, group, n, lens, counts, how):
+    rng = np.random.default_rng(25 + n)
+    with filled(ctx, rng, 2, kv, d, 16, 16, fmt, lens) as p:
+        opts = dict(parents=trees(rng, 2, n), bias=True) if how == "tree" else HOW[how]
+        if how == "first":
+            p.drop(0, 1)
+        p.check_attend(rows(rng, 2, n, kv * group, d), counts=counts,
+                       **options(opts, rng, n, kv * group, lens))
+
+
+@pytest.mark.parametrize("bad", [np.inf, np.nan])
+def test_many_blocks_do_not_see_what_is_masked(ctx, bad):
+    rng = np.random.default_rng(26)
+    n, ln = 64, 100
+    k, v = rows(rng, 1, 224, ln, 64), rows(rng, 1, 224, ln, 64)
+    v[0, :, 90, 7] = bad
+    with Pair(ctx, 1, 224, 64, 7, 16, "bf16") as p:
+        p.put([ln], k, v)
+        q = rows(rng, 1, n, 448, 64)
+        out, _ = p.attend(q)
+        hit = np.arange(n) + ln - n >= 90
+        p.ref.v[0, :, 90, 7] = 0
+        want, _, tol, _ = p.ref.attend(q, [n], 0.125)
+        assert (np.abs(out[0, ~hit] - want[0, ~hit]) <= tol[0, ~hit]).all()
+        got, ok = out[0, hit], np.ones(64, bool)
+        ok[7] = False
+        assert not np.isfinite(got[..., 7]).any()
+        assert (np.abs(got - want[0, hit]) <= tol[0, hit])[..., ok].all()
+
+
+@pytest.mark.parametrize("fmt", ["f32", "bf16"])
+@pytest.mark.parametrize("n_seqs,kv,group,n", [(65, 1, 2, 1), (130, 2, 1, 2), (300, 1, 4, 5), (600, 1, 1, 1)])
+def test_attention_of_many_sequences(ctx, fmt, n_seqs, kv, group, n):
+    rng = np.random.default_rng(27)
+    lens = rng.integers(0, 200, n_seqs).tolist()
+    lens[3] = 0
+    with filled(ctx, rng, n_seqs, kv, 64, 13, 16, fmt, lens) as p:
+        counts = rng.integers(0, n + 1, n_seqs).tolist()
+        p.check_attend(rows(rng, n_seqs, n, kv * group, 64), counts=counts)
+        p.check_attend(rows(rng, n_seqs, n, kv * group, 64), window=20)
+
+
+# Lengths so different that a sequence has many shares and others none, and shares that end where a sequence does.
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("kv,group,n,lens", [(1, 4, 1, [5000, 1, 0, 640, 641, 33]), (2, 8, 5, [4096, 100, 5, 2049])])
+def test_attention_of_uneven_sequences(ctx, fmt, kv, group, n, lens):
+    rng = np.random.default_rng(28)
+    with filled(ctx, rng, len(lens), kv, 64, 320, 16, fmt, lens) as p:
+        q = rows(rng, len(lens), n, kv * group, 64)
+        p.check_attend(q)
+        p.check_attend(q, window=700, slopes=np.float32(rng.uniform(0, 0.1, kv * group)))
+        p.check_attend(q, window=64, prefix=[40] * len(lens))
 
 
 def test_results_do_not_depend_on_chance(ctx):
