@@ -303,7 +303,8 @@ typedef struct shp_paged {
  * (nothing is turned, inv_freq is not read).  v and the other dimensions are stored as they are.  q
  * [n_heads heads a row] goes to q_out turned, and may be q_out with the same strides; both NULL: no
  * queries.  Rows of tokens before the first (lengths[s] < counts[s]) are not stored, their queries
- * are turned all the same. */
+ * are turned all the same.  At most 16,000,000 rows of all sequences together, and as many of a KV head
+ * as shp_paged_attend takes. */
 typedef struct shp_paged_append_args {
     const float *k, *v;
     int64_t k_seq, k_row, k_head;
@@ -329,7 +330,17 @@ int shp_paged_append(shp_ctx* ctx, const shp_paged* cache, const shp_paged_appen
  * n_heads query heads share the n_kv_heads KV heads in order; a KV head has at most 500,000 rows of a
  * sequence.  A row that sees no token, or lies before the first token itself, gets zeros.  lse (may be
  * NULL) [n_seqs][n_heads][n]: log of the sum of exp(x), minus infinity for such a row.  What a row does
- * not see has no part in its result, whatever it holds.  Statistics and sums are fp32.  */
+ * not see has no part in its result, whatever it holds; a row that sees a key or a value that is not
+ * finite may get NaN where the formula gives a number.  cap is 0 (none) or so large that scale / cap is
+ * finite.
+ * Statistics and sums are fp32.  Over fp32 and bf16 caches q and the weights enter the products with
+ * all of their bits, but a value 2^100 times smaller than 1 may lose its last bits, or all.  Over fp16
+ * caches they have 22 bits: an element of q that is 2^15 times smaller than the largest of its row has
+ * fewer, and one 2^39 times smaller none; so has a token in the product with V whose weight is 2^28 and
+ * 2^38 times smaller than the row's largest (it counts in the sum and in lse all the same).
+ * The tokens are split over workgroups whose partial results go through the context's workspace, as
+ * those of shp_cache8_attend do; a captured call that finds it too small runs without the split: run the
+ * call once before it is captured.  The same arguments give the same bits. */
 typedef struct shp_paged_attend_args {
     const float* q;
     float* out;

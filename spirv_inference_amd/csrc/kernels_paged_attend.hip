@@ -836,9 +836,20 @@ __device__ __forceinline__ void join(const PagedQuery& q, const Unit& u, __amdgp
     }
 }
 
-// Few rows, or a long way through the tokens: the four wavefronts of a workgroup hold the same rows and take a tile each
-// in turn; their parts meet in LDS at the end.  Many rows that see little each (SIDE): the wavefronts hold rows of their
-// own, side by side, and read the same tiles at about the same time.  K and V go from memory to registers.
+// Few rows, or a long way through the tokens: the four wavefronts of a workgroup hold the same rows and take a tile
+// each in turn; their parts meet in LDS at the end.  Many rows that see little each (SIDE): the wavefronts hold rows of
+// their own, side by side, and read the same tiles at about the same time.  K and V go from memory to registers.
+//
+// With 16 rows reading the cache bounds it: 16 x 128,001-131,072 tokens x 8 heads x 128 in fp16 (8.5 GB) 1,410 us,
+// 6.0 TB/s; 24 sequences of 0-8,100 tokens in bf16 with capped scores (399 MB) 82 us, 4.9 TB/s; 300 tokens 8.7 us, which
+// is latency (a CU reads 30 GB/s, and shares cost 3 us for their parts' way through memory).  With more rows the vector
+// and the matrix unit do: a SIMD runs instructions of the two side by side only in small part (48 products and 192
+// additions, each 0.36 us by itself for a thousand rounds of one wavefront, take 0.61 interleaved as well as they can be), so
+// that the kernel's time is nearly the sum of both: 60-row trees of 16 sequences in bf16 91 us, 38 % of it products and
+// 46 % other instructions; documents in 4,090 tokens 153 us, 37 % and 54 %.  512 rows x 4 heads on 8,190 tokens x 8 heads x
+// 128 in fp32 659 us, 101 TFLOP/s, its matrix unit busy for 68 %.  (Loads of K and V that run ahead into LDS change none of
+// these: 192, 96 and 631 us; nor do wavefronts of different priority.)
+// (Launch bounds: the wavefronts a SIMD that each variant reaches with few spills, which are outside the loop.)
 template <class E, int D, int MT, bool SIDE>
 __global__ __launch_bounds__(256, MT == 1 ? (D == 64 ? 4 : 3) : 2) void paged_attend_kernel(
     Paged c, PagedQuery q, int target, int least, float* part, int* counters) {
