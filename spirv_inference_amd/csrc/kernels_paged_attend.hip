@@ -139,9 +139,8 @@ __device__ __forceinline__ float log_sum(float m, float l) {
 
 // A drafted tree's rows: bit u of above[i] says that row u is row i of the workgroup's or above it and within its
 // window or the prefix; depth[i] is how many rows are above row i of the tree.
-template <int N>  // N query rows are of N tokens at most
 struct Tree {
-    uint64_t above[N][kTreeRows / 64];
+    uint64_t above[32][kTreeRows / 64];  // 32 query rows are of 32 tokens at most
     uint16_t parent[kTreeRows], depth[kTreeRows];
 };
 
@@ -287,16 +286,15 @@ __device__ __forceinline__ Unit unit_of(const PagedQuery& q, const Task& k) {
     return u;
 }
 
-// The workgroup's 256 threads walk up the tree from a row each.  Its own rows are those from `own` on.
-template <int N>
-__device__ __forceinline__ void climb(const PagedQuery& q, const Unit& u, int own, Tree<N>& tree) {
-    const int i = threadIdx.x;
-    if (i < u.count) {
+// The workgroup's threads walk up the tree from a row each.  Its own rows are those from `own` on.
+template <int THREADS>
+__device__ __forceinline__ void climb(const PagedQuery& q, const Unit& u, int own, Tree& tree) {
+    for (int i = threadIdx.x; i < u.count; i += THREADS) {
         const int p = q.parents[(int64_t)u.s * q.n + i];
         tree.parent[i] = (uint16_t)(p >= 0 && p < i ? p : 0xffff);
     }
     __syncthreads();
-    if (i < u.count) {
+    for (int i = threadIdx.x; i < u.count; i += THREADS) {
         uint64_t up[kTreeRows / 64] = {};
         int steps = 0;
         for (int v = i; v != 0xffff; v = tree.parent[v], ++steps)  // falls
@@ -305,7 +303,7 @@ __device__ __forceinline__ void climb(const PagedQuery& q, const Unit& u, int ow
                 for (int w = 0; w < kTreeRows / 64; ++w) up[w] |= v >> 6 == w ? 1ull << (v & 63) : 0ull;
             }
         tree.depth[i] = (uint16_t)(steps - 1);
-        if (i >= own && i < own + N) {
+        if (i >= own && i < own + 32) {
 #pragma unroll
             for (int w = 0; w < kTreeRows / 64; ++w) tree.above[i - own][w] = up[w];
         }
@@ -837,8 +835,8 @@ __device__ __forceinline__ void join(const PagedQuery& q, const Unit& u, __amdgp
 }
 
 // Few rows, or a long way through the tokens: the four wavefronts of a workgroup hold the same rows and take a tile
-// each in turn; their parts meet in LDS at the end.  Many rows that see little each (SIDE): the wavefronts hold rows of
-// their own, side by side, and read the same tiles at about the same time.  K and V go from memory to registers.
+// each in turn; their parts meet in LDS at the end.  Many rows that see little each (SIDE): a workgroup is one
+// wavefront, which takes all tiles.  K and V go from memory to registers.
 //
 // With 16 rows reading the cache bounds it: 16 x 128,001-131,072 tokens x 8 heads x 128 in fp16 (8.5 GB) 1,410 us,
 // 6.0 TB/s; 24 sequences of 0-8,100 tokens in bf16 with capped scores (399 MB) 82 us, 4.9 TB/s; 300 tokens 8.7 us, which
@@ -846,52 +844,48 @@ __device__ __forceinline__ void join(const PagedQuery& q, const Unit& u, __amdgp
 // and the matrix unit do: a SIMD runs instructions of the two side by side only in small part (48 products and 192
 // additions, each 0.36 us by itself for a thousand rounds of one wavefront, take 0.61 interleaved as well as they can be), so
 // that the kernel's time is nearly the sum of both: 60-row trees of 16 sequences in bf16 91 us, 38 % of it products and
-// 46 % other instructions; documents in 4,090 tokens 153 us, 37 % and 54 %.  512 rows x 4 heads on 8,190 tokens x 8 heads x
+// 46 % other instructions; documents in 4,090 tokens 155 us, 37 % and 54 %.  512 rows x 4 heads on 8,190 tokens x 8 heads x
 // 128 in fp32 659 us, 101 TFLOP/s, its matrix unit busy for 68 %.  (Loads of K and V that run ahead into LDS change none of
 // these: 192, 96 and 631 us; nor do wavefronts of different priority.)
 // (Launch bounds: the wavefronts a SIMD that each variant reaches with few spills, which are outside the loop.)
 template <class E, int D, int MT, bool SIDE>
-__global__ __launch_bounds__(256, MT == 1 ? (D == 64 ? 4 : 3) : 2) void paged_attend_kernel(
+__global__ __launch_bounds__(SIDE ? 64 : 256, MT == 1 ? (D == 64 ? 4 : 3) : 2) void paged_attend_kernel(
     Paged c, PagedQuery q, int target, int least, float* part, int* counters) {
     typedef Wave<E, D, MT> W;
-    constexpr int NO = W::NO, TT = W::TT, NJ = W::NJ, NQ = W::NQ, WAVES = 4, PW = W::PW;
-    constexpr int ROWS = 16 * MT * (SIDE ? WAVES : 1), EX = MT * (NO * 4 + 2) * 64;  // floats of a wavefront's part
+    constexpr int NO = W::NO, TT = W::TT, NJ = W::NJ, NQ = W::NQ, WAVES = SIDE ? 1 : 4, PW = W::PW;
+    constexpr int ROWS = 16 * MT, EX = MT * (NO * 4 + 2) * 64;  // floats of a wavefront's part
     constexpr bool F32 = W::F32;
     __shared__ __attribute__((aligned(16))) float ex[SIDE ? 1 : WAVES / 2][SIDE ? 4 : EX];
-    __shared__ u4 lowest[W::NL ? (SIDE ? WAVES : 1) * MT * NQ * 64 : 1];
-    __shared__ Tree<SIDE ? 128 : 32> tree;
+    __shared__ u4 lowest[W::NL ? MT * NQ * 64 : 1];
+    __shared__ Tree tree;
     __shared__ int arrived;
     const int lane = threadIdx.x & 63, g = lane >> 4, li = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Task task = task_of<TT, ROWS, D>(c, q, target, least);
     if (!task.any) return;
     const Unit u = unit_of(q, task);
-    const int block0 = task.block * ROWS;
-    if (block0 >= u.nrows) return;
-    const int node0 = (int)fdiv((unsigned)block0, q.by_group);  // the first row's token
-    if (SIDE && u.drafted) climb(q, u, node0, tree);
-    const int r0 = SIDE ? block0 + 16 * MT * wave : block0;
-    if (SIDE && r0 >= u.nrows) return;
-    const Span span = span_of(q, u, r0, min(r0 + 16 * MT, u.nrows));
+    const int r0 = task.block * ROWS;
+    if (r0 >= u.nrows) return;
+    const Span span = span_of(q, u, r0, min(r0 + ROWS, u.nrows));
     const Tiles<TT> tiles(u, span);
     const int splits = min(max((tiles.all + task.share - 1) / task.share, 1), task.shares);
     if (task.z >= splits) return;
     const int tile0 = task.z * task.share, tile1 = task.z == splits - 1 ? tiles.all : tile0 + task.share;
-    if (!SIDE && u.drafted) climb(q, u, node0, tree);
+    const int node0 = (int)fdiv((unsigned)r0, q.by_group);  // the first row's token
+    if (u.drafted) climb<64 * WAVES>(q, u, node0, tree);
 
     W x;
-    u4* const low = lowest + (W::NL && SIDE ? wave * MT * NQ * 64 : 0);
     {
         f4 raw[MT][D / 16];
         x.begin(q, u, tree.depth, node0, r0, raw);
-        x.pieces(q, raw, low, SIDE || wave == 0);
+        x.pieces(q, raw, lowest, wave == 0);
     }
     if (W::NL && !SIDE) __syncthreads();
     const float shift = W::NP == 2 ? (float)-kLift : (float)(32 - __builtin_clz(max(u.len, 1)));
     const E* const kb = (const E*)c.k;
     const E* const vb = (const E*)c.v;
     const int last = max(u.len - 1, 0) & ~15;
-    for (int at = tile0 + (SIDE ? 0 : wave); at < tile1; at += SIDE ? 1 : WAVES) {
+    for (int at = tile0 + wave; at < tile1; at += WAVES) {
         const int t0 = tiles.begin(at);
         uint64_t there = ~0ull;  // the tokens that have a page, of which each holds whole groups of 16
         int pages[NJ];
@@ -918,7 +912,7 @@ __global__ __launch_bounds__(256, MT == 1 ? (D == 64 ? 4 : 3) : 2) void paged_at
                         vb + row[j] + (4 * g + i) * D + (F32 ? 64 * w + 4 * li : NO * li));
         // all of them on their way before the first is used: left to itself the compiler keeps few
         __builtin_amdgcn_sched_barrier(0);
-        x.step(q, u, tree.above, tree.depth, span, shift, t0, there, low,
+        x.step(q, u, tree.above, tree.depth, span, shift, t0, there, lowest,
                [&](int j, int a) __attribute__((always_inline)) { return kr[j][a]; },
                [&](int j, int i, int w) __attribute__((always_inline)) { return vr[j][i][w]; },
                [&](int token, int d) __attribute__((always_inline)) {
@@ -988,12 +982,11 @@ PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t ro
     // long that 16 rows, twice the workgroups, are better until there are 32 pairs of 32 rows and a tile a CU (24
     // rows x 8 heads on 700 tokens x 4 heads x 64 11 us and 15, prompts of 200 tokens 20 and 30).
     p.rows = rows > 16 && (!f32 || heads * ((rows + 31) / 32) * tiles >= 32 * cu) ? 32 : 16;
-    // Where blocks of 128 rows nearly fill the GPU, each with work for three wavefronts at least, wavefronts side by
-    // side begin and end once for each 32 rows, not four times (4,000 tokens with a window of 500 113 us, 155 the
-    // other way; prompts of 100 tokens of 32 sequences 32 and 54; at 2,000 tokens x 8 heads, 504 blocks, both take
-    // 123; with 256 blocks of 8 sequences on 2,000 tokens 115 and 101).  In fp32 the products outweigh that (prompts
-    // of 1,000 tokens 247 and 186).
-    if (!f32 && rows > 64 && 4 * heads * ((rows + 127) / 128) >= 7 * cu) p.rows = 128;
+    // Where blocks of 32 rows are seven times as many as CUs, one wavefront takes all tiles of a block: it begins and
+    // ends once, not four times (4,000 tokens with a window of 500 113 us, 155 the other way; prompts of 100 tokens of
+    // 32 sequences 29 and 54; 2,000 tokens x 8 heads 127 and 130; trees of 60 rows of 16 sequences 252 and 188, for
+    // whose 960 blocks it is not taken).  In fp32 the products outweigh that (prompts of 1,000 tokens 247 and 186).
+    p.side = !f32 && rows > 64 && heads * ((rows + 31) / 32) >= 7 * cu;
     p.row_blocks = (int)((rows + p.rows - 1) / p.rows);
     const int64_t units = heads * p.row_blocks;
     // Two workgroups on every CU, or a whole number of times that (of 32 rows a CU holds no more: trees of 60 rows in
@@ -1004,7 +997,7 @@ PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t ro
     p.least = (int)std::min<int64_t>(std::max<int64_t>((units / 8 + 3) / 4 * 4, 4), 32);
     const int64_t shares = (tiles + p.least - 1) / p.least;  // of the longest sequence there can be
     const int64_t grid = std::min((units + p.target - 1) / p.target * p.target, units * shares) + 8;  // (8: XCDs' runs are rounded up)
-    if (p.rows == 128 || !may_split || shares == 1 || units > 2 * p.target || c.n_seqs > 512 ||
+    if (p.side || !may_split || shares == 1 || units > 2 * p.target || c.n_seqs > 512 ||
         grid * (int64_t)sizeof(int) > (int64_t)kSplitCounterBytes) {
         p.target = 0;
         p.grid = (int)heads;
@@ -1019,9 +1012,9 @@ PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t ro
 
 namespace {
 template <class E, int D>
-auto kernel_of(int rows) {
+auto kernel_of(int rows, bool side) {
     if constexpr (sizeof(E) == 2)
-        if (rows == 128) return paged_attend_kernel<E, D, 2, true>;
+        if (side) return paged_attend_kernel<E, D, 2, true>;
     return rows == 16 ? paged_attend_kernel<E, D, 1, false> : paged_attend_kernel<E, D, 2, false>;
 }
 }  // namespace
@@ -1033,8 +1026,8 @@ int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format,
     q.by_group = shpd::fast_div((unsigned)q.group);
     with_format(format, [&](auto e) {
         using E = decltype(e);
-        auto kern = head_dim == 64 ? kernel_of<E, 64>(p.rows) : kernel_of<E, 128>(p.rows);
-        hipLaunchKernelGGL(kern, dim3(p.grid, p.row_blocks), dim3(256), 0, s, c, q, p.target, p.least, scratch, counters);
+        auto kern = head_dim == 64 ? kernel_of<E, 64>(p.rows, p.side) : kernel_of<E, 128>(p.rows, p.side);
+        hipLaunchKernelGGL(kern, dim3(p.grid, p.row_blocks), dim3(p.side ? 64 : 256), 0, s, c, q, p.target, p.least, scratch, counters);
     });
     SHP_HIP_CHECK(hipGetLastError());
     return SHP_OK;

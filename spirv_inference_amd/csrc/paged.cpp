@@ -149,6 +149,8 @@ int shp_paged_attend(shp_ctx* ctx, const shp_paged* cache, const shp_paged_atten
     if (!rc) rc = shp::check_rows(me, "q", a->q, a->q_seq, a->q_row, a->q_head);
     if (!rc) rc = shp::check_rows(me, "out", a->out, a->o_seq, a->o_row, a->o_head);
     if (rc) return rc;
+    if (a->q == a->out && (a->q_seq != a->o_seq || a->q_row != a->o_row || a->q_head != a->o_head))
+        return bad(me, "out is q with other strides");
     if (!std::isfinite(a->scale)) return bad(me, "scale is not finite");
     if (!std::isfinite(a->cap) || a->cap < 0 || (a->cap > 0 && !std::isfinite(a->scale / a->cap)))
         return bad(me, "cap must be finite, and 0 or large enough for scale / cap");

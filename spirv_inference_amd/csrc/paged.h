@@ -42,7 +42,8 @@ struct PagedQuery {
 };
 // How attention shares out rows and tokens, and the floats of scratch that takes (0: none).
 struct PagedPlan {
-    int rows;              // a workgroup owns: 16 or 32 (its wavefronts share the tokens) or 128 (they share the rows)
+    int rows;              // a workgroup owns: 16 or 32
+    bool side;             // a workgroup is one wavefront, else four, which share the tokens
     int target;            // workgroups that the tokens are shared out for; 0: a workgroup takes all of them
     int least;             // tiles a workgroup takes at least
     int grid, row_blocks;  // workgroups: over KV heads and blocks of rows, or (row_blocks 1) over shares

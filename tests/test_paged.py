@@ -115,6 +115,7 @@ def test_bad_caches_are_refused(over, code, what):
     ("shp_paged_append", dict(rot=72), "rot"),
     ("shp_paged_append", dict(inv_freq=0), "inv_freq"),
     ("shp_paged_append", dict(n=600000), "500000"),
+    ("shp_paged_attend", dict(q=P, out=P, o_seq=128), "other strides"),
     ("shp_paged_attend", dict(cap=1e-45, scale=1.0), "cap"),
     ("shp_paged_attend", dict(cap=1e-3, scale=1e37), "cap"),
     ("shp_paged_attend", dict(n=-1), "n < 0"),

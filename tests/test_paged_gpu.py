@@ -555,7 +555,7 @@ def test_long_sequences(ctx, fmt, d, kv, group, n, ln, page):
         p.check_attend(q, window=ln // 2, prefix=[200])
 
 
-# So many blocks of 128 rows of a KV head that the wavefronts of a workgroup take rows of their own.
+# So many blocks of rows that a wavefront takes one by itself.
 @pytest.mark.parametrize("fmt", ["f16", "bf16"])
 @pytest.mark.parametrize("d,kv,group,n,lens,counts", [
     (64, 56, 4, 101, [101, 230], None), (128, 75, 3, 90, [77, 90], [77, 3]), (64, 224, 1, 70, [70, 4], None)])
@@ -612,6 +612,26 @@ def test_attention_of_uneven_sequences(ctx, fmt, kv, group, n, lens):
         p.check_attend(q)
         p.check_attend(q, window=700, slopes=np.float32(rng.uniform(0, 0.1, kv * group)))
         p.check_attend(q, window=64, prefix=[40] * len(lens))
+
+
+@pytest.mark.parametrize("kv,n,how", [(1, 4000, {}), (29, 2000, dict(window=150)), (2, 3999, dict(prefix=[700]))])
+def test_long_prompts(ctx, kv, n, how):
+    """Blocks of rows that see from one to 4,000 tokens, in any order."""
+    rng = np.random.default_rng(35)
+    with filled(ctx, rng, 1, kv, 64, 4000 // 64 + 1, 64, "bf16", [n]) as p:
+        p.check_attend(rows(rng, 1, n, kv, 64), **how)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("kv,group,n,lens", [(2, 4, 1, [3000, 5]), (2, 8, 9, [900, 40]), (56, 4, 101, [130, 101])])
+def test_out_in_place_of_q(ctx, fmt, kv, group, n, lens):
+    rng = np.random.default_rng(36)
+    with filled(ctx, rng, 2, kv, 64, 190, 16, fmt, lens) as p:
+        q = rows(rng, 2, n, kv * group, 64)
+        want, t = p.attend(q)[0], p.up(q)
+        p.dev.attend(t, t, kv * group, n)
+        ctx.sync()
+        np.testing.assert_array_equal(t.download().reshape(q.shape), want)
 
 
 def test_results_do_not_depend_on_chance(ctx):
