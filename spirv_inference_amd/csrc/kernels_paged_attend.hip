@@ -843,9 +843,9 @@ __device__ __forceinline__ void join(const PagedQuery& q, const Unit& u, __amdgp
 // is latency (a CU reads 30 GB/s, and shares cost 3 us for their parts' way through memory).  With more rows the vector
 // and the matrix unit do: a SIMD runs instructions of the two side by side only in small part (48 products and 192
 // additions, each 0.36 us by itself for a thousand rounds of one wavefront, take 0.61 interleaved as well as they can be), so
-// that the kernel's time is nearly the sum of both: 60-row trees of 16 sequences in bf16 91 us, 38 % of it products and
-// 46 % other instructions; documents in 4,090 tokens 155 us, 37 % and 54 %.  512 rows x 4 heads on 8,190 tokens x 8 heads x
-// 128 in fp32 659 us, 101 TFLOP/s, its matrix unit busy for 68 %.  (Loads of K and V that run ahead into LDS change none of
+// that the kernel's time is nearly the sum of both: 60-row trees of 16 sequences in bf16 90 us, 38 % of it products and
+// 37 % other instructions; documents in 4,090 tokens 151 us, 38 % and 46 %.  512 rows x 4 heads on 8,190 tokens x 8 heads x
+// 128 in fp32 655 us, 102 TFLOP/s, its matrix unit busy for 68 %.  (Loads of K and V that run ahead into LDS change none of
 // these: 192, 96 and 631 us; nor do wavefronts of different priority.)
 // (Launch bounds: the wavefronts a SIMD that each variant reaches with few spills, which are outside the loop.)
 template <class E, int D, int MT, bool SIDE>
