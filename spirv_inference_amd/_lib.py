@@ -233,11 +233,14 @@ SIGNATURES = [
 ]
 
 # Internal hooks for tests and experiments, exported by the library but not declared in
-# include/spirv_hip.h: per-context planner overrides and split-K workspace control.
+# include/spirv_hip.h: per-context planner overrides, split-K workspace control and the paged
+# attention's plan.
 INTERNAL = [
     ("shp_tune", C.c_int, [C.c_void_p, C.c_char_p, C.c_int]),
     ("shp_reserve_workspace", C.c_int, [C.c_void_p, C.c_uint64]),
     ("shp_workspace_info", C.c_int, [C.c_void_p, C.POINTER(C.c_void_p), C.POINTER(C.c_uint64)]),
+    ("shp_paged_attend_plan", C.c_int, [C.c_void_p, C.POINTER(PagedStruct), C.c_int32, C.c_int32,
+                                        C.POINTER(C.c_int32)]),
 ]
 
 _LIB = None

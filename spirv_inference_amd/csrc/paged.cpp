@@ -184,6 +184,26 @@ int shp_paged_attend(shp_ctx* ctx, const shp_paged* cache, const shp_paged_atten
     });
 }
 
+// Internal hook for tests, not in spirv_hip.h: how attention shares out n rows of n_heads heads on the context's
+// device (without a context: on 256 CUs).  out4: rows of a block, 1 where a wavefront takes a block by itself, 1
+// where tokens are shared out, workgroups.
+int shp_paged_attend_plan(shp_ctx* ctx, const shp_paged* cache, int32_t n, int32_t n_heads, int32_t* out4) {
+    const char* const me = "shp_paged_attend_plan";
+    Paged c;
+    int rc = shp::check_paged(me, cache, &c);
+    if (rc) return rc;
+    if (n < 1 || !out4) return bad(me, "n < 1 or null out4");
+    rc = shp::check_heads(me, c, n, n_heads);
+    if (rc) return rc;
+    const int cu = ctx ? reinterpret_cast<Ctx*>(ctx)->cu_count : 256;
+    const shp::PagedPlan p = shp::paged_attend_plan(c, cache->head_dim, cache->format, (int64_t)n * (n_heads / c.kv), cu, true);
+    out4[0] = p.rows;
+    out4[1] = p.side;
+    out4[2] = p.scratch != 0;
+    out4[3] = p.grid * p.row_blocks;
+    return SHP_OK;
+}
+
 int shp_paged_accept(shp_ctx* ctx, const shp_paged* cache, const shp_paged_accept_args* a) {
     const char* const me = "shp_paged_accept";
     Paged c;

@@ -188,6 +188,30 @@ def test_acceptance_refuses_arrays_that_overlap():
                 assert rc == _lib.SHP_ERR_INVALID and "shares memory" in msg, (out, field, msg)
 
 
+@pytest.mark.parametrize("form,n,heads,want", [
+    # rows of a block, a wavefront by itself, tokens shared out
+    (dict(format=2, n_kv_heads=112), 101, 112 * 4, (32, 1, 0)),    # 2 x 112 x 13 blocks
+    (dict(format=2, n_kv_heads=896), 64, 896, (32, 0, 0)),         # 64 rows of a KV head: never
+    (dict(format=2, n_kv_heads=896), 65, 896, (32, 1, 0)),
+    (dict(format=2, n_kv_heads=298, max_pages=8), 70, 298, (32, 0, 0)),  # 3 x 596 = 1,788 blocks: not quite
+    (dict(format=1, n_kv_heads=299, max_pages=8), 70, 299, (32, 1, 0)),  # 1,794 of at least 7 x 256
+    (dict(format=0, n_kv_heads=896), 65, 896, (32, 0, 0)),         # fp32: never
+    (dict(format=1, max_pages=64), 1, 2, (16, 0, 1)),
+    (dict(format=1, max_pages=4), 1, 2, (16, 0, 0)),               # a tile
+    (dict(format=1, max_pages=64, n_kv_heads=512), 1, 512, (16, 0, 0)),   # 16 tiles, a share has 32 with 1,024 blocks
+    (dict(format=1, max_pages=128, n_kv_heads=512), 1, 512, (16, 0, 0)),
+    (dict(format=1, max_pages=129, n_kv_heads=512), 1, 512, (16, 0, 1)),
+    (dict(format=1, max_pages=129, n_kv_heads=513), 1, 513, (16, 0, 0)),  # more than 1,024 blocks
+    (dict(format=0, max_pages=64, n_seqs=512, n_kv_heads=1), 1, 1, (16, 0, 0)),  # 32 tiles
+    (dict(format=0, max_pages=65, n_seqs=512, n_kv_heads=1), 1, 1, (16, 0, 1)),
+    (dict(format=0, max_pages=65, n_seqs=513, n_kv_heads=1), 1, 1, (16, 0, 0))])  # more than 512 sequences
+def test_attention_plans(form, n, heads, want):
+    """Which variant a call takes on 256 CUs, on both sides of each line."""
+    out = (C.c_int32 * 4)()
+    rc = _lib.lib().shp_paged_attend_plan(None, C.byref(cache(**form)), n, heads, out)
+    assert rc == 0 and tuple(out[:3]) == want, _lib.lib().shp_last_error()
+
+
 class FakeTensor:
     def __init__(self, nbytes, ptr=P):
         self.nbytes, self.ptr = nbytes, ptr

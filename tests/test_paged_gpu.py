@@ -2,6 +2,8 @@
 
 What is stored unturned and what acceptance moves are compared bit for bit; rotation and attention
 within the bounds that paged_ref derives from the operations' roundings."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -555,7 +557,7 @@ def test_long_sequences(ctx, fmt, d, kv, group, n, ln, page):
         p.check_attend(q, window=ln // 2, prefix=[200])
 
 
-# So many blocks of rows that a wavefront takes one by itself.
+# So many blocks of rows that their tokens are not shared out.
 @pytest.mark.parametrize("fmt", ["f16", "bf16"])
 @pytest.mark.parametrize("d,kv,group,n,lens,counts", [
     (64, 56, 4, 101, [101, 230], None), (128, 75, 3, 90, [77, 90], [77, 3]), (64, 224, 1, 70, [70, 4], None)])
@@ -588,6 +590,81 @@ def test_many_blocks_do_not_see_what_is_masked(ctx, bad):
         ok[7] = False
         assert not np.isfinite(got[..., 7]).any()
         assert (np.abs(got - want[0, hit]) <= tol[0, hit])[..., ok].all()
+
+
+# So many blocks of rows that a wavefront takes one by itself.
+WAVES = [(64, 72, 4, 101, [101, 230], None), (128, 100, 3, 90, [77, 90], [77, 3]), (64, 300, 1, 70, [70, 4], None),
+         (128, 180, 1, 160, [160, 171], [111, 160])]
+
+
+def takes_waves(p, n, heads):
+    out = (C.c_int32 * 4)()
+    check(lib().shp_paged_attend_plan(p.ctx.handle, C.byref(p.dev._struct), n, heads, out), "shp_paged_attend_plan")
+    return out[1] == 1
+
+
+@pytest.mark.parametrize("fmt", ["f16", "bf16"])
+@pytest.mark.parametrize("d,kv,group,n,lens,counts", WAVES)
+@pytest.mark.parametrize("how", ["plain", "cap", "bias", "window", "prefix and window", "first", "all", "tree", "tree of all"])
+def test_attention_of_a_wavefront_a_block(ctx, fmt, d, kv, group, n, lens, counts, how):
+    rng = np.random.default_rng(46 + n)
+    with filled(ctx, rng, 2, kv, d, 16, 16, fmt, lens) as p:
+        assert takes_waves(p, n, kv * group)
+        opts = {"plain": {}, "tree": dict(parents=trees(rng, 2, n), bias=True),
+                "tree of all": dict(parents=trees(rng, 2, n), **HOW["all"])}.get(how) or HOW.get(how, {})
+        if how in ("first", "tree"):
+            p.drop(0, 1)
+        p.check_attend(rows(rng, 2, n, kv * group, d), counts=counts, **options(opts, rng, n, kv * group, lens))
+
+
+@pytest.mark.parametrize("fmt", ["f16", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [np.inf, -np.inf, np.nan])
+def test_a_wavefront_a_block_does_not_see_what_is_masked(ctx, fmt, d, bad):
+    rng = np.random.default_rng(47)
+    n, ln, kv = 64, 100, 448
+    k, v = rows(rng, 1, kv, ln, d), rows(rng, 1, kv, ln, d)
+    k[0, :, 95, 3] = v[0, :, 90, 7] = bad
+    with Pair(ctx, 1, kv, d, 7, 16, fmt) as p:
+        assert takes_waves(p, n, 2 * kv)
+        p.put([ln], k, v)
+        q = rows(rng, 1, n, 2 * kv, d)
+        out, _ = p.attend(q)
+        place = np.arange(n) + ln - n
+        free, hit = place < 90, (place >= 90) & (place < 95)
+        p.ref.v[0, :, 90, 7] = p.ref.k[0, :, 95, 3] = 0
+        want, _, tol, _ = p.ref.attend(q, [n], d ** -0.5)
+        assert (np.abs(out[0, free] - want[0, free]) <= tol[0, free]).all()
+        got, ok = out[0, hit], np.ones(d, bool)
+        ok[7] = False
+        assert not np.isfinite(got[..., 7]).any()
+        assert (np.abs(got - want[0, hit]) <= tol[0, hit])[..., ok].all()
+
+
+@pytest.mark.parametrize("fmt", ["f16", "bf16"])
+@pytest.mark.parametrize("d,kv,group,n,lens", [(64, 72, 4, 101, [130, 101]), (128, 100, 3, 90, [90, 200])])
+def test_a_wavefront_a_block_in_place_and_replayed(ctx, fmt, d, kv, group, n, lens):
+    """out in place of q gives the same bits; so does every replay of a captured call."""
+    rng = np.random.default_rng(48)
+    with filled(ctx, rng, 2, kv, d, 13, 16, fmt, lens) as p:
+        assert takes_waves(p, n, kv * group)
+        q = rows(rng, 2, n, kv * group, d)
+        want, t = p.attend(q)[0], p.up(q)
+        p.dev.attend(t, t, kv * group, n)
+        ctx.sync()
+        np.testing.assert_array_equal(t.download().reshape(q.shape), want)
+        t.upload(q)
+        out = p.new(q.size)
+        ctx.capture_begin()
+        p.dev.attend(t, out, kv * group, n)
+        g = ctx.capture_end()
+        for _ in range(3):
+            out.upload(np.full(out.n, -3))
+            g.launch()
+            ctx.sync()
+            np.testing.assert_array_equal(out.download().reshape(q.shape), want)
+            p.attend(rows(rng, 2, 3, kv * group, d))
+        g.destroy()
 
 
 @pytest.mark.parametrize("fmt", ["f32", "bf16"])
