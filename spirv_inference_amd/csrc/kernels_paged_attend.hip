@@ -19,6 +19,7 @@
 // times V are no larger than V, down by 14 for fp16, so that the low piece stays a normal number
 // longer.  Scaling is by powers of two, which rounds nothing, and seldom: a maximum has to pass a
 // whole number.
+#include <cmath>
 #include <type_traits>
 
 #include "coherent.h"
@@ -363,8 +364,8 @@ struct Sight {
     int lo, hi, first, position, node;  // node: of the workgroup's
 };
 
-// 16 * MT rows of a wavefront, and what it has of their softmax.
-template <class E, int D, int MT>
+// 16 * MT rows of a wavefront, and what it has of their softmax.  LARGE: the cap is large.
+template <class E, int D, int MT, bool LARGE>
 struct Wave {
     static constexpr bool F32 = kF32<E>;
     static constexpr int NP = kPieces<E>, NO = D / 16, TT = kTile<E, D>, NJ = TT / 16;
@@ -405,7 +406,7 @@ struct Wave {
     }
     // The rows' pieces in the B layout, times the scale; nothing seen yet.  low: those that LDS holds.
     __device__ __forceinline__ void pieces(const PagedQuery& q, f4 v[MT][2 * D / 32], u4* low, bool mine) {
-        const float factor = q.cap > 0.0f ? q.scale / q.cap : q.scale * kLog2e;
+        const float factor = LARGE ? q.factor : q.cap > 0.0f ? q.scale / q.cap : q.scale * kLog2e;
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             back[t] = 1.0f;
@@ -502,7 +503,13 @@ struct Wave {
 #pragma unroll
                 for (int j = 0; j < NJ; ++j) sc[t][j] *= back[t];
             }
-            if (q.cap > 0.0f) {
+            if constexpr (LARGE) {
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        sc[t][j][i] = 2.0f * (q.half * tanh_of(__builtin_amdgcn_ldexpf(sc[t][j][i], -q.lift)));
+            } else if (q.cap > 0.0f) {
                 const float top = q.cap * kLog2e;
 #pragma unroll
                 for (int j = 0; j < NJ; ++j)
@@ -732,8 +739,8 @@ __device__ __forceinline__ void place_of(const PagedQuery& q, const Unit& u, int
     to_lse = ((int64_t)u.s * q.heads + head) * q.n + i;
 }
 
-template <class E, int D, int MT>
-__device__ __forceinline__ void Wave<E, D, MT>::store(const PagedQuery& q, const Unit& u, int r0) const {
+template <class E, int D, int MT, bool LARGE>
+__device__ __forceinline__ void Wave<E, D, MT, LARGE>::store(const PagedQuery& q, const Unit& u, int r0) const {
     const int ln = __lane_id(), li = ln & 15, quad = ln >> 4;
 #pragma unroll
     for (int t = 0; t < MT; ++t) {
@@ -848,10 +855,10 @@ __device__ __forceinline__ void join(const PagedQuery& q, const Unit& u, __amdgp
 // 128 in fp32 655 us, 102 TFLOP/s, its matrix unit busy for 68 %.  (Loads of K and V that run ahead into LDS change none of
 // these: 192, 96 and 631 us; nor do wavefronts of different priority.)
 // (Launch bounds: the wavefronts a SIMD that each variant reaches with few spills, which are outside the loop.)
-template <class E, int D, int MT, bool SIDE>
+template <class E, int D, int MT, bool SIDE, bool LARGE = false>
 __global__ __launch_bounds__(SIDE ? 64 : 256, MT == 1 ? (D == 64 ? 4 : 3) : 2) void paged_attend_kernel(
     Paged c, PagedQuery q, int target, int least, float* part, int* counters) {
-    typedef Wave<E, D, MT> W;
+    typedef Wave<E, D, MT, LARGE> W;
     constexpr int NO = W::NO, TT = W::TT, NJ = W::NJ, NQ = W::NQ, WAVES = SIDE ? 1 : 4, PW = W::PW;
     constexpr int ROWS = 16 * MT, EX = MT * (NO * 4 + 2) * 64;  // floats of a wavefront's part
     constexpr bool F32 = W::F32;
@@ -972,8 +979,10 @@ __global__ __launch_bounds__(SIDE ? 64 : 256, MT == 1 ? (D == 64 ? 4 : 3) : 2) v
 
 namespace shp {
 
-PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t rows, int cu_count, bool may_split) {
+PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t rows, int cu_count, bool may_split,
+                            bool large) {
     PagedPlan p;
+    p.large = large;
     const bool f32 = format == SHP_PAGED_F32;
     const int cu = std::max(cu_count, 1), tile = 8192 / (head_dim * (f32 ? 4 : 2));
     const int64_t heads = (int64_t)c.n_seqs * c.kv, tiles = (c.cap + tile - 1) / tile;
@@ -981,12 +990,12 @@ PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t ro
     // heads x 128 in bf16 180 us, with 16 rows 287; prompts of 1,000 tokens 80 and 104).  fp32's products take so
     // long that 16 rows, twice the workgroups, are better until there are 32 pairs of 32 rows and a tile a CU (24
     // rows x 8 heads on 700 tokens x 4 heads x 64 11 us and 15, prompts of 200 tokens 20 and 30).
-    p.rows = rows > 16 && (!f32 || heads * ((rows + 31) / 32) * tiles >= 32 * cu) ? 32 : 16;
+    p.rows = !large && rows > 16 && (!f32 || heads * ((rows + 31) / 32) * tiles >= 32 * cu) ? 32 : 16;
     // Where blocks of 32 rows are seven times as many as CUs, one wavefront takes all tiles of a block: it begins and
     // ends once, not four times (4,000 tokens with a window of 500 113 us, 155 the other way; prompts of 100 tokens of
     // 32 sequences 29 and 54; 2,000 tokens x 8 heads 127 and 130; trees of 60 rows of 16 sequences 252 and 188, for
     // whose 960 blocks it is not taken).  In fp32 the products outweigh that (prompts of 1,000 tokens 247 and 186).
-    p.side = !f32 && rows > 64 && heads * ((rows + 31) / 32) >= 7 * cu;
+    p.side = !large && !f32 && rows > 64 && heads * ((rows + 31) / 32) >= 7 * cu;
     p.row_blocks = (int)((rows + p.rows - 1) / p.rows);
     const int64_t units = heads * p.row_blocks;
     // Two workgroups on every CU, or a whole number of times that (of 32 rows a CU holds no more: trees of 60 rows in
@@ -1012,7 +1021,8 @@ PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t ro
 
 namespace {
 template <class E, int D>
-auto kernel_of(int rows, bool side) {
+auto kernel_of(int rows, bool side, bool large) {
+    if (large) return paged_attend_kernel<E, D, 1, false, true>;
     if constexpr (sizeof(E) == 2)
         if (side) return paged_attend_kernel<E, D, 2, true>;
     return rows == 16 ? paged_attend_kernel<E, D, 1, false> : paged_attend_kernel<E, D, 2, false>;
@@ -1024,9 +1034,19 @@ int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format,
     PagedQuery q = query;
     q.by_kv = shpd::fast_div((unsigned)c.kv);
     q.by_group = shpd::fast_div((unsigned)q.group);
+    if (p.large) {
+        // q has scale / cap in it, and 2^lift times as much where that is less than 2^-30, so that pieces of 16 bits and
+        // products hold all of q's bits (a denormal score loses 2^-150 of the cap, 2^-22 at most).  Half of the cap
+        // is finite in units of log2 as well.  A kernel of its own: the same instructions in the others, behind a
+        // branch, cost 1 to 3 % of calls that never take it.
+        const int e = std::ilogb(q.cap);
+        q.lift = q.scale == 0.0f ? 0 : std::max(std::min(e - std::ilogb(q.scale) - 30, e), 0);
+        q.factor = q.scale / std::ldexp(q.cap, -q.lift);
+        q.half = q.cap * 0.5f * kLog2e;
+    }
     with_format(format, [&](auto e) {
         using E = decltype(e);
-        auto kern = head_dim == 64 ? kernel_of<E, 64>(p.rows, p.side) : kernel_of<E, 128>(p.rows, p.side);
+        auto kern = head_dim == 64 ? kernel_of<E, 64>(p.rows, p.side, p.large) : kernel_of<E, 128>(p.rows, p.side, p.large);
         hipLaunchKernelGGL(kern, dim3(p.grid, p.row_blocks), dim3(p.side ? 64 : 256), 0, s, c, q, p.target, p.least, scratch, counters);
     });
     SHP_HIP_CHECK(hipGetLastError());

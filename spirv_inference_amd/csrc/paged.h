@@ -39,9 +39,15 @@ struct PagedQuery {
     int n, heads, group, window;
     float scale, cap;
     shpd::FastDiv by_kv, by_group;  // set by the launch
+    // and where the cap is large: q is multiplied by factor, a score is 2 * (half * tanh(2^-lift * products))
+    float factor, half;
+    int lift;
 };
+// Caps from here on are large: 16-bit pieces of scale / cap * q and the cap in units of log2 leave their range.
+constexpr float kLargeCap = 0x1p64f;
 // How attention shares out rows and tokens, and the floats of scratch that takes (0: none).
 struct PagedPlan {
+    bool large;            // the kernel for large caps, which exists for 16 rows and four wavefronts
     int rows;              // a workgroup owns: 16 or 32
     bool side;             // a workgroup is one wavefront, else four, which share the tokens
     int target;            // workgroups that the tokens are shared out for; 0: a workgroup takes all of them
@@ -49,7 +55,8 @@ struct PagedPlan {
     int grid, row_blocks;  // workgroups: over KV heads and blocks of rows, or (row_blocks 1) over shares
     size_t scratch;
 };
-PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t rows, int cu_count, bool may_split);
+PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t rows, int cu_count, bool may_split,
+                            bool large = false);
 int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format, const PagedQuery& q,
                         const PagedPlan& p, float* scratch, int* counters);
 

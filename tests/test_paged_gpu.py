@@ -496,6 +496,47 @@ def test_caps_from_small_to_large(ctx, fmt):
             p.check_attend(rows(rng, 1, 2, 4, 128), cap=cap)
 
 
+FLT_MAX = float(np.finfo(np.float32).max)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("cap", [1e9, 1e18, 1e27, 1e33, 1e36, 2.0 ** 126, 2.3e38, 2.4e38, FLT_MAX])
+@pytest.mark.parametrize("scale", [0.125, 3.0, 1e-3])
+def test_caps_up_to_the_largest(ctx, fmt, cap, scale):
+    """Such caps bend nothing: out and lse are those of the scores themselves."""
+    rng = np.random.default_rng(49)
+    with filled(ctx, rng, 2, 2, 64, 13, 16, fmt, [200, 65]) as p:
+        p.check_attend(rows(rng, 2, 3, 8, 64), cap=cap, scale=scale)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("d,kv,group,n,ln,how", [
+    (64, 1, 4, 1, 3001, {}), (128, 2, 4, 33, 700, HOW["all"]), (128, 1, 8, 60, 500, dict(tree=True, bias=True)),
+    (64, 72, 4, 101, 130, dict(window=37))])
+def test_large_caps_in_every_form(ctx, fmt, d, kv, group, n, ln, how):
+    """Split over shares, with masks, in trees and of many blocks, on both sides of the caps that are large."""
+    rng = np.random.default_rng(52)
+    with filled(ctx, rng, 2, kv, d, -(-ln // 16), 16, fmt, [ln, n]) as p:
+        opts = {**how, **(dict(parents=trees(rng, 2, n)) if how.get("tree") else {})}
+        opts.pop("tree", None)
+        opts = options(opts, rng, n, kv * group, [ln, n])
+        q = rows(rng, 2, n, kv * group, d)
+        for cap in (float(np.nextafter(np.float32(2.0 ** 64), np.float32(0))), 2.0 ** 64, FLT_MAX):
+            p.check_attend(q, **{**opts, "cap": cap})
+
+
+def test_large_caps_bend_large_scores(ctx):
+    """Scores of the cap's own size: out is finite and lse the largest capped score within fp32's roundings."""
+    rng = np.random.default_rng(53)
+    for fmt in ("f32", "bf16"):
+        with Pair(ctx, 1, 1, 64, 13, 16, fmt) as p:
+            k = rows(rng, 1, 1, 200, 64) * np.float32(2.0 ** 50)
+            p.put([200], k, rows(rng, 1, 1, 200, 64))
+            q = rows(rng, 1, 3, 4, 64) * np.float32(2.0 ** 50)
+            for cap in (2.0 ** 63, 2.0 ** 100, 2.0 ** 101):
+                p.check_attend(q, cap=cap)
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_attention_of_large_and_small_values(ctx, fmt):
     """Weights times values near the ends of the range."""
