@@ -382,6 +382,7 @@ struct Wave {
     u4 qp[MT][NQ][NR];
     float m[MT], l[MT], slope[MT], back[MT];
     Sight see[MT];
+    int lift[LARGE ? MT : 1];  // the power of two that a row's products lack
 
     // Rows from r0 on; those behind the last repeat it.  raw: the lane's part of them.
     __device__ __forceinline__ void begin(const PagedQuery& q, const Unit& u, const uint16_t* depth, int node0, int r0, f4 raw[MT][2 * D / 32]) {
@@ -410,6 +411,19 @@ struct Wave {
 #pragma unroll
         for (int t = 0; t < MT; ++t) {
             back[t] = 1.0f;
+            if constexpr (LARGE) {
+                float top = 0.0f;
+#pragma unroll
+                for (int a = 0; a < D / 16; ++a)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) top = fmaxf(top, fabsf(v[t][a][b]));
+                const int e = __builtin_amdgcn_frexp_expf(max_over_groups(top));
+                lift[t] = e + q.lift;
+#pragma unroll
+                for (int a = 0; a < D / 16; ++a)
+#pragma unroll
+                    for (int b = 0; b < 4; ++b) v[t][a][b] = __builtin_amdgcn_ldexpf(v[t][a][b], -e);
+            }
 #pragma unroll
             for (int a = 0; a < D / 16; ++a) v[t][a] *= factor;
             if constexpr (F32) {
@@ -508,7 +522,7 @@ struct Wave {
                 for (int j = 0; j < NJ; ++j)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        sc[t][j][i] = 2.0f * (q.half * tanh_of(__builtin_amdgcn_ldexpf(sc[t][j][i], -q.lift)));
+                        sc[t][j][i] = 2.0f * (q.half * tanh_of(__builtin_amdgcn_ldexpf(sc[t][j][i], lift[t])));
             } else if (q.cap > 0.0f) {
                 const float top = q.cap * kLog2e;
 #pragma unroll
@@ -1035,13 +1049,13 @@ int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format,
     q.by_kv = shpd::fast_div((unsigned)c.kv);
     q.by_group = shpd::fast_div((unsigned)q.group);
     if (p.large) {
-        // q has scale / cap in it, and 2^lift times as much where that is less than 2^-30, so that pieces of 16 bits and
-        // products hold all of q's bits (a denormal score loses 2^-150 of the cap, 2^-22 at most).  Half of the cap
-        // is finite in units of log2 as well.  A kernel of its own: the same instructions in the others, behind a
-        // branch, cost 1 to 3 % of calls that never take it.
-        const int e = std::ilogb(q.cap);
-        q.lift = q.scale == 0.0f ? 0 : std::max(std::min(e - std::ilogb(q.scale) - 30, e), 0);
-        q.factor = q.scale / std::ldexp(q.cap, -q.lift);
+        // A row of q enters the products as numbers up to 1, scale and cap with their digits only, so that pieces of
+        // 16 bits hold them; the powers of two come back behind the sums (a denormal score loses 2^-150 of the cap,
+        // 2^-22 at most).  Half of the cap is finite in units of log2 as well.  A kernel of its own: instructions for
+        // this in the others, behind a branch, cost 1 to 3 % of calls that never take it.
+        const int down = std::ilogb(q.cap), up = q.scale == 0.0f ? 0 : std::ilogb(q.scale);
+        q.lift = up - down;
+        q.factor = std::ldexp(q.scale, -up) / std::ldexp(q.cap, -down);
         q.half = q.cap * 0.5f * kLog2e;
     }
     with_format(format, [&](auto e) {

@@ -39,7 +39,7 @@ struct PagedQuery {
     int n, heads, group, window;
     float scale, cap;
     shpd::FastDiv by_kv, by_group;  // set by the launch
-    // and where the cap is large: q is multiplied by factor, a score is 2 * (half * tanh(2^-lift * products))
+    // and where the cap is large: scale / cap = factor * 2^lift, half the cap in units of log2
     float factor, half;
     int lift;
 };

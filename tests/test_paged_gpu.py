@@ -538,6 +538,16 @@ def test_large_caps_bend_large_scores(ctx):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("scale,cap", [(2.0 ** 126, None), (-2.0 ** 126, None), (2.35e38, None), (-2.35e38, None),
+                                       (3.4e38, 30.0), (3.4e38, 2.0 ** 64), (2.0 ** 126, FLT_MAX)])
+def test_scales_up_to_the_largest(ctx, fmt, scale, cap):
+    """Over queries that are as small."""
+    rng = np.random.default_rng(50)
+    with filled(ctx, rng, 1, 1, 64, 13, 16, fmt, [200]) as p:
+        p.check_attend(rows(rng, 1, 3, 4, 64) * np.float32(2.0 ** -125), scale=scale, cap=cap)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 def test_attention_of_large_and_small_values(ctx, fmt):
     """Weights times values near the ends of the range."""
     rng = np.random.default_rng(19)
