@@ -332,7 +332,8 @@ int shp_paged_append(shp_ctx* ctx, const shp_paged* cache, const shp_paged_appen
  * NULL) [n_seqs][n_heads][n]: log of the sum of exp(x), minus infinity for such a row.  What a row does
  * not see has no part in its result, whatever it holds; a row that sees a key or a value that is not
  * finite may get NaN where the formula gives a number.  cap is 0 (none), or finite and so large that scale /
- * cap is finite.  out may be q with the same strides; otherwise they share no memory.
+ * cap is finite; without a cap scale * log2 e is finite.  q * scale and the scores, also times log2 e, are to be
+ * finite in fp32: a row where they are not may get NaN.  out may be q with the same strides; otherwise they share no memory.
  * Statistics and sums are fp32.  Over fp32 and bf16 caches q and the weights enter the products with
  * all of their bits, but a value 2^100 times smaller than 1 may lose its last bits, or all.  Over fp16
  * caches they have 22 bits: an element of q that is 2^15 times smaller than the largest of its row has

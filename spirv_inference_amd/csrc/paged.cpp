@@ -154,6 +154,8 @@ int shp_paged_attend(shp_ctx* ctx, const shp_paged* cache, const shp_paged_atten
     if (!std::isfinite(a->scale)) return bad(me, "scale is not finite");
     if (!std::isfinite(a->cap) || a->cap < 0 || (a->cap > 0 && !std::isfinite(a->scale / a->cap)))
         return bad(me, "cap must be finite, and 0 or large enough for scale / cap");
+    if (a->cap == 0 && !std::isfinite(a->scale * 1.4426950408889634f))  // q is multiplied by it
+        return bad(me, "scale times log2 e must be finite");
     if (a->window < 0) return bad(me, "window < 0");
     if (a->parents && a->n > shp::kTreeRows)
         return bad(me, "a tree of more than 256 rows", SHP_ERR_UNSUPPORTED);

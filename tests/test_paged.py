@@ -60,7 +60,8 @@ def test_good_arguments_of_appends_and_attention():
                  dict(rot=8, interleaved=1, offsets=P)):
         assert call("shp_paged_append", cache(), args(PagedAppendArgs, **over))[1].endswith("null ctx")
     for over in (dict(lse=0), dict(window=5, cap=30.0, slopes=P, prefix=P, first=P, parents=P, n=256),
-                 dict(n=100000, scale=-1.0)):
+                 dict(n=100000, scale=-1.0), dict(scale=2.35e38), dict(scale=-2.35e38),
+                 dict(scale=3.4e38, cap=30.0), dict(cap=3.4028234663852886e38)):
         assert call("shp_paged_attend", cache(), args(PagedAttendArgs, **over))[1].endswith("null ctx")
 
 
@@ -127,6 +128,8 @@ def test_bad_caches_are_refused(over, code, what):
     ("shp_paged_attend", dict(n_heads=0), "n_heads"),
     ("shp_paged_attend", dict(scale=float("nan")), "scale"),
     ("shp_paged_attend", dict(scale=float("inf")), "scale"),
+    ("shp_paged_attend", dict(scale=2.4e38), "scale times log2 e"),
+    ("shp_paged_attend", dict(scale=-3.4028234663852886e38), "scale times log2 e"),
     ("shp_paged_attend", dict(cap=-1.0), "cap"),
     ("shp_paged_attend", dict(cap=float("inf")), "cap"),
     ("shp_paged_attend", dict(cap=float("nan")), "cap"),
