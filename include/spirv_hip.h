@@ -297,8 +297,8 @@ typedef struct shp_paged {
 
 /* Writes new rows, turned by their positions: the first `rot` dimensions of a row of k (and of q) are
  * rot / 2 pairs (x0, x1), dimensions j and j + rot / 2 or, interleaved, 2 j and 2 j + 1, and become
- * (x0 cos a - x1 sin a, x1 cos a + x0 sin a) with a = position * inv_freq[j], the product of the two
- * exact.  The position is lengths[s] - counts[s] + offsets[s][i], i where offsets is NULL (a tree's
+ * (x0 cos a - x1 sin a, x1 cos a + x0 sin a) with a = position * inv_freq[j], formed in 64 bits: off by
+ * 2^-51 of itself at most.  The position is lengths[s] - counts[s] + offsets[s][i], i where offsets is NULL (a tree's
  * offsets are its depths).  inv_freq [rot / 2] on the device; rot a multiple of 8 up to head_dim, or 0
  * (nothing is turned, inv_freq is not read).  v and the other dimensions are stored as they are.  q
  * [n_heads heads a row] goes to q_out turned, and may be q_out with the same strides; both NULL: no

@@ -12,12 +12,12 @@ using shp::PagedTree;
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
-// cos and sin of position * freq.  The product is exact in 64 bits (31 and 24 bits), and so is the whole
-// number of quarter turns that is taken off, up to 2^-53 of the product; what is left is at most an
-// eighth of a turn, where the Taylor series end within 2^-29 after x^11 and x^10.
-__device__ __forceinline__ void turn(int position, float freq, float& c, float& s) {
+// cos and sin of position * freq.  The product is formed in 64 bits: exact for positions below 2^29 (freq has 24
+// bits), beyond that and in quarter turns rounded to 2^-53 of itself.  What is left without the whole quarter turns
+// is at most an eighth of a turn, where the Taylor series end within 2^-29 after x^11 and x^10.
+__device__ __forceinline__ void turn(double position, float freq, float& c, float& s) {
     constexpr double kQuarters = 0.63661977236758134308, kQuarter = 1.57079632679489661923;
-    const double t = (double)position * (double)freq * kQuarters, n = __builtin_rint(t);
+    const double t = position * (double)freq * kQuarters, n = __builtin_rint(t);
     const float x = (float)((t - n) * kQuarter), y = x * x;
     const int m = (int)(long long)n & 3;
     const float sine = x + x * y * (-1.0f / 6 + y * (1.0f / 120 + y * (-1.0f / 5040 + y * (1.0f / 362880 - y * (1.0f / 39916800)))));
@@ -62,7 +62,7 @@ __global__ __launch_bounds__(256) void paged_append_kernel(Paged c, PagedRows r)
                                 : r.k + s * r.k_seq + i * r.k_row + h * r.k_head;
         f4 a = *reinterpret_cast<const f4*>(x + d0), b = *reinterpret_cast<const f4*>(x + d1);
         if (turned) {
-            const int position = begin + (r.offsets ? r.offsets[(int64_t)s * r.n + i] : i);
+            const double position = (double)begin + (r.offsets ? r.offsets[(int64_t)s * r.n + i] : i);  // of 33 bits
             f4 co, si;
 #pragma unroll
             for (int j = 0; j < 4; ++j) turn(position, r.inv_freq[4 * t + j], ((float*)&co)[j], ((float*)&si)[j]);

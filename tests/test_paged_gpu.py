@@ -192,6 +192,28 @@ def test_append_far_positions(ctx):
             assert (np.abs(kc - R.turned(k[0], offsets, f, False)[:, 0]) <= bound).all()
 
 
+def test_far_offsets_behind_a_context(ctx):
+    """Sums of length and offset that pass 32 bits."""
+    rng = np.random.default_rng(51)
+    d = 64
+    offsets = np.array([2 ** 31 - 1, 2 ** 31 - 1 - 300, 2 ** 31 - 200, 2 ** 31 - 1000, 5, -2 ** 31])
+    n = len(offsets)
+    with Pair(ctx, 1, 1, d, 64, 16, "f32") as p:
+        f = np.geomspace(1e-9, 1e-3, 32).astype(np.float32)
+        q, k = rows(rng, 1, n, 2, d), rows(rng, 1, n, 1, d)
+        dq = p.up(q)
+        p.dev.set_lengths([1000])
+        p.dev.append(p.up(k), p.up(k), n, q=dq, q_out=dq, n_heads=2, inv_freq=p.up(f), offsets=p.up(offsets, np.int32))
+        ctx.sync()
+        got = dq.download().reshape(q.shape)[0]
+        pos = 1000 - n + offsets
+        # two roundings in 64 bits, of the product and of its quarter turns, and one of the quarter turns' length
+        far = 3 * 2.0 ** -53 * np.abs(pos[:, None] * f.astype(np.float64))
+        extra = (np.abs(q[0, ..., :32]) + np.abs(q[0, ..., 32:])) * far[:, None]
+        bound = R.turned_bound(q[0], f, False) + np.concatenate([extra, extra], -1)
+        assert (np.abs(got - R.turned(q[0], pos, f, False)) <= bound).all()
+
+
 @pytest.mark.parametrize("fmt", FORMATS)
 def test_append_of_strided_rows(ctx, fmt):
     """q, k and v side by side in one tensor, as a fused projection leaves them; q in place."""
