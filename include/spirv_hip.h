@@ -333,7 +333,8 @@ int shp_paged_append(shp_ctx* ctx, const shp_paged* cache, const shp_paged_appen
  * not see has no part in its result, whatever it holds; a row that sees a key or a value that is not
  * finite may get NaN where the formula gives a number.  cap is 0 (none), or finite and so large that scale /
  * cap is finite; without a cap scale * log2 e is finite.  q * scale and the scores, also times log2 e, are to be
- * finite in fp32: a row where they are not may get NaN.  out may be q with the same strides; otherwise they share no memory.
+ * finite in fp32: a row where they are not may get NaN.  out may be q with the same strides; otherwise they
+ * share no memory.
  * Statistics and sums are fp32.  Over fp32 and bf16 caches q and the weights enter the products with
  * all of their bits, but a value 2^100 times smaller than 1 may lose its last bits, or all.  Over fp16
  * caches they have 22 bits: an element of q that is 2^15 times smaller than the largest of its row has
@@ -341,7 +342,10 @@ int shp_paged_append(shp_ctx* ctx, const shp_paged* cache, const shp_paged_appen
  * 2^38 times smaller than the row's largest (it counts in the sum and in lse all the same).
  * The tokens are split over workgroups whose partial results go through the context's workspace, as
  * those of shp_cache8_attend do; a captured call that finds it too small runs without the split: run the
- * call once before it is captured.  The same arguments give the same bits. */
+ * call once before it is captured.  The same arguments give the same bits.  There is no split over more than
+ * 512 sequences or 1,024 blocks of 16 or 32 rows (n counts, not counts[s]): few rows on long sequences do
+ * better in a call of their own than beside a chunk of a prompt.
+ * Where scores pass 2^21 in size, values above FLT_MAX / (tokens seen) may overflow. */
 typedef struct shp_paged_attend_args {
     const float* q;
     float* out;
@@ -363,9 +367,9 @@ int shp_paged_attend(shp_ctx* ctx, const shp_paged* cache, const shp_paged_atten
  * == choices[its parent] (the id the model chose there) is kept, until there is none.  Writes path
  * [n_seqs][n] (the rows kept, in order, -1 behind them), accepted [n_seqs] (how many), next [n_seqs]
  * (choices of the last row kept) and lengths_out [n_seqs] (may be the cache's lengths): lengths - counts
- * + accepted.  The kept rows of K and V move to the places behind the context; those of the others are
- * undefined.  A sequence without rows, or with more than it holds tokens, keeps none: next is -1 and
- * the length stays.  parents, tokens and choices [n_seqs][n], n up to 256.  Arrays that are written
+ * + accepted.  The kept rows of K and V move to the places behind the context (a row for which a
+ * page is not there, at either end, stays); those of the others are undefined.  A sequence without rows, or
+ * with more than it holds tokens, keeps none: next is -1 and the length stays.  parents, tokens and choices [n_seqs][n], n up to 256.  Arrays that are written
  * share no memory with others of the call. */
 typedef struct shp_paged_accept_args {
     const int32_t* counts;

@@ -154,8 +154,11 @@ struct Unit {
 
 // What a workgroup does: a block of rows of a KV head, and of the tiles that they see the shares
 // z * share .. of `shares`.  With target = 0 it is a place in the grid, and all tiles.  Else the blocks and the tiles
-// of all sequences are counted and cut into shares of one size, `target` of them or a little less, which evens out
-// sequences of different lengths; a workgroup finds its own in their running sum, or that there is none for it.
+// of all sequences are counted and cut into shares of one size, `target` of them or less; a workgroup finds its own in
+// their running sum, or that there is none for it.  A share is of one block, whose last may be shorter, so that blocks
+// nearly as many as `target` are hardly cut: 24 sequences of 0-8,100 tokens x 8 heads have shares of 58 tiles where a
+// workgroup's mean is 48 (82 us, 94 with a number of shares by sequence), trees of 60 rows of 16 sequences 123 and 73, and
+// 64 such sequences have the longest whole, 254 and 127 (224 us, 190 of as many tokens in equal lengths).
 struct Task {
     int s, h, len, count, block, z, share, shares, first;  // first: the place of its rows' first part and of their counter
     bool any;
@@ -198,7 +201,9 @@ __device__ __forceinline__ Task task_of(const Paged& c, const PagedQuery& q, int
         return k;
     }
     const int lane = threadIdx.x & 63;
-    // a sequence's blocks, and the tiles that a block sees of it, no more than those that a window touches
+    // a sequence's blocks, and the tiles that a block sees of it, no more than those that a window touches (with a
+    // prefix all count: a row on 100,000 tokens x 8 heads x 128 in bf16 with a window of 4,096 14 us, and 37 with a
+    // prefix of 4 as well)
     const int most = q.window && !q.prefix ? (min(q.window, 1 << 22) + q.n) / T + 2 : 1 << 22;
     int len, count, blocks, tiles;
     auto size = [&](int s0) __attribute__((always_inline)) {
@@ -228,7 +233,7 @@ __device__ __forceinline__ Task task_of(const Paged& c, const PagedQuery& q, int
         to = over_lanes(mine, add);
         return last_lane(to);
     };
-    // as many workgroups as the GPU holds at once, or a whole number of times that
+    // `target` workgroups, or a whole number of times that
     const int room = max((units + target - 1) / target, 1) * target;
     // (32 shares of a block at most, 16 of 32 rows of 128 dimensions, whose parts one workgroup joins: at the
     // 30 GB/s that a CU reads it takes 9 us for 270 KB.  8 rows x 4 heads of 2 sequences on 100,000 tokens 132 us, 153
@@ -478,6 +483,7 @@ struct Wave {
                                          int t0, uint64_t there, const u4* low, K key, V value, N number) {
         const int g = (threadIdx.x & 63) >> 4;
         // whether some row does not see some token
+        // (a tile of the prefix in front of the window as well, though all rows see it whole)
         const bool edge = (~there & below(TT)) || t0 < span.open_lo || t0 + TT > span.open_hi;
         f4 sc[MT][NJ];
 #pragma unroll
@@ -866,8 +872,9 @@ __device__ __forceinline__ void join(const PagedQuery& q, const Unit& u, __amdgp
 // additions, each 0.36 us by itself for a thousand rounds of one wavefront, take 0.61 interleaved as well as they can be), so
 // that the kernel's time is nearly the sum of both: 60-row trees of 16 sequences in bf16 90 us, 38 % of it products and
 // 37 % other instructions; documents in 4,090 tokens 151 us, 38 % and 46 %.  512 rows x 4 heads on 8,190 tokens x 8 heads x
-// 128 in fp32 655 us, 102 TFLOP/s, its matrix unit busy for 68 %.  (Loads of K and V that run ahead into LDS change none of
-// these: 192, 96 and 631 us; nor do wavefronts of different priority.)
+// 128 in fp32 655 us, 102 TFLOP/s, its matrix unit busy for 68 % and its vector unit for 6 %: a tile has 16 tokens
+// there, and a step of the softmax, lookups and the wait for K and V come after every 128 products.  (Loads of K and V
+// that ran ahead into LDS gained nothing, nor did wavefronts of different priority.)
 // (Launch bounds: the wavefronts a SIMD that each variant reaches with few spills, which are outside the loop.)
 template <class E, int D, int MT, bool SIDE, bool LARGE = false>
 __global__ __launch_bounds__(SIDE ? 64 : 256, MT == 1 ? (D == 64 ? 4 : 3) : 2) void paged_attend_kernel(
@@ -1008,18 +1015,21 @@ PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t ro
     // Where blocks of 32 rows are seven times as many as CUs, one wavefront takes all tiles of a block: it begins and
     // ends once, not four times (4,000 tokens with a window of 500 113 us, 155 the other way; prompts of 100 tokens of
     // 32 sequences 29 and 54; 2,000 tokens x 8 heads 127 and 130; trees of 60 rows of 16 sequences 252 and 188, for
-    // whose 960 blocks it is not taken).  In fp32 the products outweigh that (prompts of 1,000 tokens 247 and 186).
+    // whose 1,024 blocks it is not taken).  In fp32 the products outweigh that (prompts of 1,000 tokens 247 and 186).
     p.side = !large && !f32 && rows > 64 && heads * ((rows + 31) / 32) >= 7 * cu;
     p.row_blocks = (int)((rows + p.rows - 1) / p.rows);
     const int64_t units = heads * p.row_blocks;
-    // Two workgroups on every CU, or a whole number of times that (of 32 rows a CU holds no more: trees of 60 rows in
-    // 16 sequences 91 us, 104 with one and a half times as many), none with fewer tiles than pay for the parts' way
+    // Two workgroups on every CU, or a whole number of times that (of 32 rows a CU holds no more, of 16 three or four:
+    // trees of 60 rows in 16 sequences 91 us, 104 with one and a half times as many), none with fewer tiles than pay for the parts' way
     // through memory, about 3 us: more where there are many blocks anyway (one row of 64 sequences on 1,000 tokens
     // x 8 heads 32 us with 32 tiles, 46 with 4; of one sequence on 700 tokens 11.4 with 4, 14.8 with 16).
     p.target = 2 * cu;
     p.least = (int)std::min<int64_t>(std::max<int64_t>((units / 8 + 3) / 4 * 4, 4), 32);
     const int64_t shares = (tiles + p.least - 1) / p.least;  // of the longest sequence there can be
     const int64_t grid = std::min((units + p.target - 1) / p.target * p.target, units * shares) + 8;  // (8: XCDs' runs are rounded up)
+    // Without shares a block has one workgroup, however long its sequence: 131,000 tokens x 128 in bf16 beside 127 or 159
+    // sequences of 500 take 1.9 ms (160 of 500 67 us); beside a chunk of 512 rows 15 sequences of 8,000 tokens with one row
+    // each 1,015 us (96 in a call of their own, and the chunk 188).
     if (p.side || !may_split || shares == 1 || units > 2 * p.target || c.n_seqs > 512 ||
         grid * (int64_t)sizeof(int) > (int64_t)kSplitCounterBytes) {
         p.target = 0;
