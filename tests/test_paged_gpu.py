@@ -1041,6 +1041,38 @@ def test_a_long_call_captured_before_it_ever_ran(ctx):
         g.destroy()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_two_graphs_share_a_workspace_that_grows(ctx, fmt):
+    """Two captured calls whose tokens are shared out, and an eager one that needs more workspace than both: replays of
+    the two, in turn and one behind the other, give the eager calls' bits."""
+    rng = np.random.default_rng(54)
+    with Context("any") as own, filled(own, rng, 2, 2, 64, 190, 16, fmt, [3000, 700]) as p:
+        calls = []
+        for n in (1, 3):
+            q = rows(rng, 2, n, 4, 64)
+            want, t, out = p.attend(q)[0], p.up(q), p.new(q.size)
+            own.capture_begin()
+            p.dev.attend(t, out, 4, n)
+            calls.append((own.capture_end(), out, want))
+        size = C.c_uint64()
+        where = C.c_void_p()
+        check(lib().shp_workspace_info(own.handle, C.byref(where), C.byref(size)), "shp_workspace_info")
+        before = where.value
+        check(lib().shp_reserve_workspace(own.handle, 2 * size.value), "shp_reserve_workspace")
+        check(lib().shp_workspace_info(own.handle, C.byref(where), C.byref(size)), "shp_workspace_info")
+        assert before and where.value != before
+        for _ in range(3):
+            p.attend(rows(rng, 2, 30, 4, 64))
+            for g, out, _ in calls:
+                out.upload(np.full(out.n, -3))
+                g.launch()
+            own.sync()
+            for _, out, want in calls:
+                np.testing.assert_array_equal(out.download().reshape(want.shape), want)
+        for g, _, _ in calls:
+            g.destroy()
+
+
 def test_calls_on_another_stream(ctx):
     rng = np.random.default_rng(44)
     with Context("any") as other, Context("any") as own, filled(own, rng, 2, 2, 64, 20, 16, "f32", [300, 77]) as p:
