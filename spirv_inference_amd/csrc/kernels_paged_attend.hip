@@ -875,9 +875,10 @@ __device__ __forceinline__ void join(const PagedQuery& q, const Unit& u, __amdgp
 // 128 in fp32 655 us, 102 TFLOP/s, its matrix unit busy for 68 % and its vector unit for 6 %: a tile has 16 tokens
 // there, and a step of the softmax, lookups and the wait for K and V come after every 128 products.  (Loads of K and V
 // that ran ahead into LDS gained nothing, nor did wavefronts of different priority.)
-// (Launch bounds: the wavefronts a SIMD that each variant reaches with few spills, which are outside the loop.)
-template <class E, int D, int MT, bool SIDE, bool LARGE = false>
-__global__ __launch_bounds__(SIDE ? 64 : 256, MT == 1 ? (D == 64 ? 4 : 3) : 2) void paged_attend_kernel(
+// (Launch bounds: the wavefronts a SIMD that each variant reaches with few spills, which are outside the loop.  With a
+// large cap 16 rows of 128 dimensions in bf16 reach two: 24 sequences 83 us, 98 with three.)
+template <class E, int D, int MT, bool SIDE, bool LARGE>
+__global__ __launch_bounds__(SIDE ? 64 : 256, MT == 1 ? (D == 64 ? 4 : LARGE ? 2 : 3) : 2) void paged_attend_kernel(
     Paged c, PagedQuery q, int target, int least, float* part, int* counters) {
     typedef Wave<E, D, MT, LARGE> W;
     constexpr int NO = W::NO, TT = W::TT, NJ = W::NJ, NQ = W::NQ, WAVES = SIDE ? 1 : 4, PW = W::PW;
@@ -1000,10 +1001,8 @@ __global__ __launch_bounds__(SIDE ? 64 : 256, MT == 1 ? (D == 64 ? 4 : 3) : 2) v
 
 namespace shp {
 
-PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t rows, int cu_count, bool may_split,
-                            bool large) {
+PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t rows, int cu_count, bool may_split) {
     PagedPlan p;
-    p.large = large;
     const bool f32 = format == SHP_PAGED_F32;
     const int cu = std::max(cu_count, 1), tile = 8192 / (head_dim * (f32 ? 4 : 2));
     const int64_t heads = (int64_t)c.n_seqs * c.kv, tiles = (c.cap + tile - 1) / tile;
@@ -1011,12 +1010,12 @@ PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t ro
     // heads x 128 in bf16 180 us, with 16 rows 287; prompts of 1,000 tokens 80 and 104).  fp32's products take so
     // long that 16 rows, twice the workgroups, are better until there are 32 pairs of 32 rows and a tile a CU (24
     // rows x 8 heads on 700 tokens x 4 heads x 64 11 us and 15, prompts of 200 tokens 20 and 30).
-    p.rows = !large && rows > 16 && (!f32 || heads * ((rows + 31) / 32) * tiles >= 32 * cu) ? 32 : 16;
+    p.rows = rows > 16 && (!f32 || heads * ((rows + 31) / 32) * tiles >= 32 * cu) ? 32 : 16;
     // Where blocks of 32 rows are seven times as many as CUs, one wavefront takes all tiles of a block: it begins and
     // ends once, not four times (4,000 tokens with a window of 500 113 us, 155 the other way; prompts of 100 tokens of
     // 32 sequences 29 and 54; 2,000 tokens x 8 heads 127 and 130; trees of 60 rows of 16 sequences 252 and 188, for
     // whose 1,024 blocks it is not taken).  In fp32 the products outweigh that (prompts of 1,000 tokens 247 and 186).
-    p.side = !large && !f32 && rows > 64 && heads * ((rows + 31) / 32) >= 7 * cu;
+    p.side = !f32 && rows > 64 && heads * ((rows + 31) / 32) >= 7 * cu;
     p.row_blocks = (int)((rows + p.rows - 1) / p.rows);
     const int64_t units = heads * p.row_blocks;
     // Two workgroups on every CU, or a whole number of times that (of 32 rows a CU holds no more, of 16 three or four:
@@ -1044,12 +1043,15 @@ PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t ro
 }
 
 namespace {
+template <class E, int D, bool LARGE>
+auto kernel_of(int rows, bool side) {
+    if constexpr (sizeof(E) == 2)
+        if (side) return paged_attend_kernel<E, D, 2, true, LARGE>;
+    return rows == 16 ? paged_attend_kernel<E, D, 1, false, LARGE> : paged_attend_kernel<E, D, 2, false, LARGE>;
+}
 template <class E, int D>
 auto kernel_of(int rows, bool side, bool large) {
-    if (large) return paged_attend_kernel<E, D, 1, false, true>;
-    if constexpr (sizeof(E) == 2)
-        if (side) return paged_attend_kernel<E, D, 2, true>;
-    return rows == 16 ? paged_attend_kernel<E, D, 1, false> : paged_attend_kernel<E, D, 2, false>;
+    return large ? kernel_of<E, D, true>(rows, side) : kernel_of<E, D, false>(rows, side);
 }
 }  // namespace
 
@@ -1058,10 +1060,11 @@ int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format,
     PagedQuery q = query;
     q.by_kv = shpd::fast_div((unsigned)c.kv);
     q.by_group = shpd::fast_div((unsigned)q.group);
-    if (p.large) {
+    const bool large = q.cap >= kLargeCap;
+    if (large) {
         // A row of q enters the products as numbers up to 1, scale and cap with their digits only, so that pieces of
         // 16 bits hold them; the powers of two come back behind the sums (a denormal score loses 2^-150 of the cap,
-        // 2^-22 at most).  Half of the cap is finite in units of log2 as well.  A kernel of its own: instructions for
+        // 2^-22 at most).  Half of the cap is finite in units of log2 as well.  Kernels of their own: instructions for
         // this in the others, behind a branch, cost 1 to 3 % of calls that never take it.
         const int down = std::ilogb(q.cap), up = q.scale == 0.0f ? 0 : std::ilogb(q.scale);
         q.lift = up - down;
@@ -1070,7 +1073,7 @@ int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format,
     }
     with_format(format, [&](auto e) {
         using E = decltype(e);
-        auto kern = head_dim == 64 ? kernel_of<E, 64>(p.rows, p.side, p.large) : kernel_of<E, 128>(p.rows, p.side, p.large);
+        auto kern = head_dim == 64 ? kernel_of<E, 64>(p.rows, p.side, large) : kernel_of<E, 128>(p.rows, p.side, large);
         hipLaunchKernelGGL(kern, dim3(p.grid, p.row_blocks), dim3(p.side ? 64 : 256), 0, s, c, q, p.target, p.least, scratch, counters);
     });
     SHP_HIP_CHECK(hipGetLastError());

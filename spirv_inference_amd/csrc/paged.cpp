@@ -173,14 +173,12 @@ int shp_paged_attend(shp_ctx* ctx, const shp_paged* cache, const shp_paged_atten
     q.n = a->n; q.heads = a->n_heads; q.group = a->n_heads / c.kv; q.window = a->window;
     q.scale = a->scale; q.cap = a->cap;
     const int64_t rows = (int64_t)q.n * q.group;
-    const bool large = q.cap >= shp::kLargeCap;
-    shp::PagedPlan plan = shp::paged_attend_plan(c, cache->head_dim, cache->format, rows, x->cu_count, true, large);
+    shp::PagedPlan plan = shp::paged_attend_plan(c, cache->head_dim, cache->format, rows, x->cu_count, true);
     float* scratch = nullptr;
     if (plan.scratch) {
         rc = x->scratch(plan.scratch, &scratch);
         if (rc) return rc;
-        if (!scratch)
-            plan = shp::paged_attend_plan(c, cache->head_dim, cache->format, rows, x->cu_count, false, large);
+        if (!scratch) plan = shp::paged_attend_plan(c, cache->head_dim, cache->format, rows, x->cu_count, false);
     }
     return x->timed("paged_attend", [&] {
         return shp::paged_attend_launch(x->stream, c, cache->head_dim, cache->format, q, plan, scratch,

@@ -47,7 +47,6 @@ struct PagedQuery {
 constexpr float kLargeCap = 0x1p64f;
 // How attention shares out rows and tokens, and the floats of scratch that takes (0: none).
 struct PagedPlan {
-    bool large;            // the kernel for large caps, which exists for 16 rows and four wavefronts
     int rows;              // a workgroup owns: 16 or 32
     bool side;             // a workgroup is one wavefront, else four, which share the tokens
     int target;            // workgroups that the tokens are shared out for; 0: a workgroup takes all of them
@@ -55,8 +54,7 @@ struct PagedPlan {
     int grid, row_blocks;  // workgroups: over KV heads and blocks of rows, or (row_blocks 1) over shares
     size_t scratch;
 };
-PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t rows, int cu_count, bool may_split,
-                            bool large = false);
+PagedPlan paged_attend_plan(const Paged& c, int head_dim, int format, int64_t rows, int cu_count, bool may_split);
 int paged_attend_launch(hipStream_t s, const Paged& c, int head_dim, int format, const PagedQuery& q,
                         const PagedPlan& p, float* scratch, int* counters);
 
